@@ -453,6 +453,124 @@ int mi355_merge_attn_states(void* out, float* out_lse, const void* a, const floa
                             const int64_t* a_lse_strides, const int64_t* b_lse_strides,
                             void* stream);
 
+/* --------------------------------------------------- paged 8-bit KV cache --
+ * The four entry points below serve models that read a prompt in pieces and go on token by token
+ * beside the DiT.  They were added to revision 12 without changing anything in it.
+ *
+ * The cache: e4m3 codes [num_blocks, block_size, Hk, D] for keys and for values (any strides, D
+ * contiguous) and fp32 scales [num_blocks, Hk] (dense) for each; a value is code * scale.  A
+ * sequence's tokens 0, 1, ... lie in the blocks that its row of the table names, block_size
+ * (a power of two in [16, 1024]) to a block.  Lengths, tables and slots live on the device; no
+ * call reads them on the host.
+ *
+ * Block tables and slot maps of one step, from request lengths.  Request b holds context_lens[b]
+ * tokens in the blocks that its row of block_table (int32 [B, table_width], rows table_stride
+ * apart) already names, and gets new_lens[b] more; negative lengths count as 0.  The blocks it
+ * needs besides are taken from free_blocks[free_begin[0] ...] in the order of the requests and
+ * written into its row.  Out:
+ *   cu_seqlens_q int32 [B + 1]  running sum of new_lens;   seq_lens int32 [B]  context + new
+ *   slot_mapping int64 [max_tokens]  block * block_size + place in the block, for each new token
+ *     in the order of the requests; -1 behind the last one, and for a token whose entry of the
+ *     table is not in [0, num_blocks)
+ *   positions int64 [max_tokens]  place of the token in its sequence; 0 behind the last one
+ *   free_end int32 [1]  free_begin + blocks taken
+ *   status int32 [3]  blocks that the free list lacks, tokens beyond max_tokens, requests that
+ *     outgrow table_width (counts saturate).  If any is not 0 nothing is given to anybody: the table is left as it
+ *     was, seq_lens = context_lens, all slots -1, cu_seqlens_q 0, free_end = free_begin.
+ * seq_lens and free_end must not be the memory of an input.  B <= 8192. */
+int mi355_kv_block_plan(const int32_t* context_lens, const int32_t* new_lens, int64_t B,
+                        int32_t* block_table, int64_t table_stride, int64_t table_width,
+                        const int32_t* free_blocks, int64_t num_free, const int32_t* free_begin,
+                        int64_t block_size, int64_t num_blocks, int64_t* slot_mapping,
+                        int64_t* positions, int64_t max_tokens, int32_t* cu_seqlens_q,
+                        int32_t* seq_lens, int32_t* free_end, int32_t* status, void* stream);
+
+/* Rotary positions from frequencies instead of a table of cosines: any position without a cache,
+ * any scaling for long contexts that is a change of frequencies and one factor.
+ *   (a, z) -> (a c - z s, z c + a s),  c = attn_factor * cos(position * inv_freq[i]), s alike,
+ * the angle in fp64, one rounding to bf16.  inv_freq [rot_dim / 2], fp64 or fp32; pairs are
+ * (i, i + rot_dim / 2) (is_neox) or (2 i, 2 i + 1); elements from rot_dim on are copied.
+ * q [tokens, Hq, head_size], k [tokens, Hk, head_size] bf16 with token and head strides, outputs
+ * with their own; an output may be its input, and must not overlap it otherwise.  Either tensor
+ * may have no heads.  rot_dim % 16 == 0, head_size % 8 == 0 and <= 256, strides % 8 == 0, rows
+ * 16-byte aligned.  |position| < 2^40. */
+int mi355_rope_scaled(const int64_t* positions, const void* q, void* q_out, const void* k, void* k_out,
+                      int64_t tokens, int64_t Hq, int64_t Hk, int64_t head_size, int64_t rot_dim,
+                      int64_t q_st, int64_t q_sh, int64_t qo_st, int64_t qo_sh, int64_t k_st,
+                      int64_t k_sh, int64_t ko_st, int64_t ko_sh, const void* inv_freq,
+                      int inv_freq_is_f64, float attn_factor, int is_neox, void* stream);
+
+/* Keys and values of new tokens into the cache, at slot_mapping[t] (tokens whose slot is outside
+ * the pool are skipped).  A block's scale (for each head, keys and values apart) is the smallest
+ * 2^e, e >= -64, with which its largest finite value stays within 448; a call that writes a
+ * block's first token starts it anew, any other call can only raise it, and then the codes of the
+ * tokens before are rounded to the larger step.  What is not finite is stored as NaN and takes no
+ * part in the scale.  Tokens of one call that go to one block follow each other in the call and
+ * in the block; a slot is given once.
+ * positions != NULL: keys are first rotated as by mi355_rope_scaled (and rounded to bf16), and
+ * the queries q (Hq heads, or 0) are rotated into q_out in the same launch.
+ * k, v [tokens, Hk, D] bf16, D 64 or 128; strides in elements (of the cache: bytes). */
+typedef struct {
+  const void* k;
+  const void* v;
+  int64_t k_st, k_sh, v_st, v_sh;
+  void* k_cache;
+  void* v_cache;
+  int64_t kc_sb, kc_st, kc_sh, vc_sb, vc_st, vc_sh; /* block, token, head */
+  float* k_scale;
+  float* v_scale;
+  const int64_t* slot_mapping;
+  int64_t tokens, Hk, D, block_size, num_blocks;
+  const int64_t* positions;
+  const void* inv_freq;
+  int64_t rot_dim;
+  int inv_freq_is_f64, is_neox;
+  float attn_factor;
+  int64_t Hq;
+  const void* q;
+  void* q_out;
+  int64_t q_st, q_sh, qo_st, qo_sh;
+} mi355_kv_store_args;
+int mi355_kv_store_fp8(const mi355_kv_store_args* args, void* stream);
+
+/* Attention of the newest tokens of each sequence over the cache: `fwd` with page_table, e4m3
+ * caches and k_descale / v_descale of [num_blocks, Hk] (schema sgl-kernel/csrc/
+ * flash_extension.cc:25-63).  Sequence b holds cache_seqlens[b] tokens, the new ones among them;
+ * new token i of n stands at cache_seqlens[b] - n + i.  causal: it sees the keys up to its own
+ * place; window_left >= 0 (with causal): and no further back than window_left.  A row that sees
+ * nothing gives 0 and a log-sum-exp of -infinity.
+ * q, out bf16: [Sq, H, D] packed with cu_seqlens_q int32 [B + 1] (rows behind the last sequence
+ * are left as they are), or [B, Sq, H, D] with cu_seqlens_q == NULL.  lse fp32 or NULL, element
+ * (row, head) at b * lse_sb + head * lse_sh + row.  max_seqlen_q chooses the kernel; any value is
+ * right.  Lengths beyond the table count as its length; entries of the table that are not in
+ * [0, num_blocks) are skipped as if their tokens were masked; entries behind a sequence's end are
+ * not read.  Scales are positive, value scales between 2^-64 and 2^120.
+ * D 64 or 128.  workspace: mi355_paged_attn_workspace_bytes(args) of device memory (16-byte
+ * aligned, no initial contents) that no other call in flight uses. */
+typedef struct {
+  const void* q;
+  void* out;
+  float* lse;
+  const void* k_cache;
+  const void* v_cache;
+  const float* k_scale;
+  const float* v_scale;
+  const int32_t* cu_seqlens_q;
+  const int32_t* cache_seqlens;
+  const int32_t* page_table;
+  int64_t B, Sq, H, Hk, D, max_seqlen_q;
+  int64_t q_sb, q_ss, q_sh, o_sb, o_ss, o_sh, lse_sb, lse_sh;
+  int64_t kc_sb, kc_st, kc_sh, vc_sb, vc_st, vc_sh; /* bytes: block, token, head */
+  int64_t table_stride, table_width, num_blocks, block_size;
+  float softmax_scale;
+  int causal;
+  int64_t window_left; /* < 0: none */
+  void* workspace;
+  int64_t workspace_bytes;
+} mi355_paged_attn_args;
+int64_t mi355_paged_attn_workspace_bytes(const mi355_paged_attn_args* args);
+int mi355_paged_attn_fp8(const mi355_paged_attn_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

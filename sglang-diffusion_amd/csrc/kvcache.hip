@@ -1,0 +1,585 @@
+// What stands around a paged 8-bit key/value cache, for gfx950: block tables and slot maps from
+// request lengths, rotary positions from scaled frequencies, and the store that rounds keys and
+// values into the cache.  The attention that reads the cache is in paged_attention.hip.
+#include "common.h"
+
+namespace {
+
+constexpr int KV_BLOCK_MIN = 16, KV_BLOCK_MAX = 1024;
+constexpr int SCALE_EXP_MIN = -64;  // exponent of the scale of a block without a nonzero value
+
+inline bool block_size_ok(int64_t bs) {
+  return bs >= KV_BLOCK_MIN && bs <= KV_BLOCK_MAX && (bs & (bs - 1)) == 0;
+}
+inline int log2_of(int64_t bs) { return __builtin_ctzll((unsigned long long)bs); }
+
+// ------------------------------------------------------------------------------------ plan --
+// One launch.  Every workgroup adds up the lengths of all requests for itself (B values out of
+// L2 and one scan over 256 threads, about as long as the gap between two launches) and then
+// fills the slots of its own 1024 tokens, so nothing has to be handed from one workgroup to
+// another.  Entries of the table that a workgroup reads (blocks held before the call) and
+// entries that any workgroup writes (fresh blocks) are different ones.
+constexpr int PLAN_THREADS = 256, PLAN_TOKENS = 1024;
+constexpr int64_t PLAN_MAX_REQUESTS = 8192;  // two ints each in LDS: 64 KiB
+
+struct PlanParams {
+  const int32_t *context_lens, *new_lens, *free_blocks, *free_begin;
+  int32_t *table, *cu, *seq_lens, *free_end, *status;
+  int64_t *slots, *positions;
+  int64_t table_stride, table_width, num_free, num_blocks, max_tokens;
+  int B, lb;
+};
+
+__global__ __launch_bounds__(PLAN_THREADS) void kv_block_plan_kernel(PlanParams p) {
+  extern __shared__ int32_t lds_plan[];
+  int32_t* cu = lds_plan;             // [B] first token of a request
+  int32_t* fresh_at = lds_plan + p.B; // [B] its first entry among the fresh blocks
+  __shared__ long long wave_tok[4], wave_fresh[4];
+  __shared__ int wave_wide[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t bs = 1ll << p.lb;
+  // a thread owns `per` requests that follow each other: one scan over the threads is enough
+  const int per = (p.B + PLAN_THREADS - 1) / PLAN_THREADS;
+  const int i0 = tid * per, i1 = min(p.B, i0 + per);
+  long long tok = 0, fresh = 0;
+  int wide = 0;
+  for (int i = i0; i < i1; ++i) {
+    const int64_t c = max(p.context_lens[i], 0), n = max(p.new_lens[i], 0);
+    const int64_t held = (c + bs - 1) >> p.lb, need = (c + n + bs - 1) >> p.lb;
+    tok += n;
+    fresh += need - held;
+    wide += need > p.table_width;
+  }
+  long long tok_in = tok, fresh_in = fresh;  // inclusive over the wave
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const long long a = __shfl_up(tok_in, o, 64), b = __shfl_up(fresh_in, o, 64);
+    if (lane >= o) {
+      tok_in += a;
+      fresh_in += b;
+    }
+    wide += __shfl_xor(wide, o, 64);
+  }
+  if (lane == 63) {
+    wave_tok[wave] = tok_in;
+    wave_fresh[wave] = fresh_in;
+    wave_wide[wave] = wide;
+  }
+  __syncthreads();
+  long long tok_all = 0, fresh_all = 0, tok_at = tok_in - tok, fresh_from = fresh_in - fresh;
+  int wide_all = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (w < wave) {
+      tok_at += wave_tok[w];
+      fresh_from += wave_fresh[w];
+    }
+    tok_all += wave_tok[w];
+    fresh_all += wave_fresh[w];
+    wide_all += wave_wide[w];
+  }
+  const int64_t begin = max(p.free_begin[0], 0);
+  const int64_t lacking = max((int64_t)0, begin + fresh_all - p.num_free);
+  const int64_t over = max((int64_t)0, (int64_t)tok_all - p.max_tokens);
+  const bool good = lacking == 0 && over == 0 && wide_all == 0;
+  const bool first_group = blockIdx.x == 0;
+  for (int i = i0; i < i1; ++i) {
+    const int64_t c = max(p.context_lens[i], 0), n = max(p.new_lens[i], 0);
+    if (good) {  // the sums fit: tokens are below max_tokens, blocks below num_free
+      cu[i] = (int)tok_at;
+      fresh_at[i] = (int)fresh_from;
+    }
+    if (first_group) {
+      p.cu[i] = good ? (int)tok_at : 0;
+      p.seq_lens[i] = (int)(good ? c + n : c);
+    }
+    tok_at += n;
+    fresh_from += ((c + n + bs - 1) >> p.lb) - ((c + bs - 1) >> p.lb);
+  }
+  if (first_group && tid == 0) {
+    p.cu[p.B] = good ? (int)tok_all : 0;
+    p.free_end[0] = (int)(begin + (good ? fresh_all : 0));
+    p.status[0] = (int)min(lacking, (int64_t)INT32_MAX);
+    p.status[1] = (int)min(over, (int64_t)INT32_MAX);
+    p.status[2] = wide_all;
+  }
+  __syncthreads();
+  const int64_t t_end = min(p.max_tokens, ((int64_t)blockIdx.x + 1) * PLAN_TOKENS);
+  for (int64_t t = (int64_t)blockIdx.x * PLAN_TOKENS + tid; t < t_end; t += PLAN_THREADS) {
+    int64_t slot = -1, place = 0;
+    if (good && t < tok_all) {
+      int lo = 0, hi = p.B;  // the last request that begins at or before t is the one that holds it
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (cu[mid] <= (int)t) lo = mid;
+        else hi = mid;
+      }
+      const int64_t c = max(p.context_lens[lo], 0);
+      place = c + (t - cu[lo]);
+      const int64_t j = place >> p.lb, held = (c + bs - 1) >> p.lb;
+      int32_t* entry = p.table + lo * p.table_stride + j;
+      const int id = j < held ? *entry : p.free_blocks[begin + fresh_at[lo] + (j - held)];
+      if ((place & (bs - 1)) == 0) *entry = id;  // a block's first token: never one held before
+      if (id >= 0 && id < p.num_blocks) slot = ((int64_t)id << p.lb) + (place & (bs - 1));
+    }
+    p.slots[t] = slot;
+    p.positions[t] = place;
+  }
+}
+
+// ------------------------------------------------------------------------------------ rope --
+struct Rope {
+  const int64_t* positions;
+  const void* inv_freq;  // [half], fp64 or fp32
+  int f64, half, neox;
+  float factor;
+};
+
+// cos and sin of position * frequency, times the factor.  The product is formed in turns and in
+// fp64 (a position of 10^6 leaves fp32 0.06 rad of it), reduced exactly to an eighth of a turn
+// on either side of the nearest quarter, and evaluated by the Taylor sums up to the terms that
+// stay below 2e-9.
+__device__ __forceinline__ float2 rope_cos_sin(const Rope& r, int64_t pos, int i) {
+  const double w = r.f64 ? reinterpret_cast<const double*>(r.inv_freq)[i]
+                         : (double)reinterpret_cast<const float*>(r.inv_freq)[i];
+  const double quarters = (double)pos * (w * 0.63661977236758134308);  // 2 / pi
+  const double whole = rint(quarters);
+  const float a = (float)((quarters - whole) * 1.57079632679489661923);
+  const int quadrant = (int)(whole - 4.0 * floor(whole * 0.25));
+  const float a2 = a * a;
+  const float s = a + a * a2 * fmaf(a2, fmaf(a2, fmaf(a2, 2.7557319e-6f, -1.9841270e-4f), 8.3333333e-3f), -0.16666667f);
+  const float c = 1.f + a2 * fmaf(a2, fmaf(a2, fmaf(a2, fmaf(a2, -2.7557319e-7f, 2.4801587e-5f), -1.3888889e-3f),
+                                           4.1666667e-2f), -0.5f);
+  const float cq = quadrant & 1 ? s : c, sq = quadrant & 1 ? c : s;
+  return make_float2((quadrant == 1 || quadrant == 2 ? -cq : cq) * r.factor,
+                     (quadrant >= 2 ? -sq : sq) * r.factor);
+}
+
+__device__ __forceinline__ void unpack8(u32x4 v, float (&f)[8]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    f[2 * j] = __uint_as_float(v[j] << 16);
+    f[2 * j + 1] = __uint_as_float(v[j] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ u32x4 pack8(const float (&f)[8]) {
+  return u32x4{pack_bf2(f[0], f[1]), pack_bf2(f[2], f[3]), pack_bf2(f[4], f[5]), pack_bf2(f[6], f[7])};
+}
+__device__ __forceinline__ void turn(float& a, float& z, float2 cs) {
+  const float u = fmaf(-z, cs.y, __fmul_rn(a, cs.x));
+  z = fmaf(a, cs.y, __fmul_rn(z, cs.x));
+  a = u;
+}
+
+// Rows of one tensor: [tokens, heads, D] with its own strides, in and out (which may be the same).
+struct RopeRows {
+  const unsigned short* x;
+  unsigned short* out;
+  int64_t st, sh, ot, oh;
+  int heads;
+};
+
+// One piece of a row.  Pieces [0, turned) hold pairs: 8 elements of each half (half layout) or 8
+// neighbours (interleaved); the pieces behind them are copied as they are.
+__device__ __forceinline__ void rope_piece(const Rope& r, const unsigned short* x, unsigned short* out,
+                                           int piece, int turned, const float2* cs) {
+  if (piece >= turned) {
+    const int at = 2 * r.half + (piece - turned) * 8;
+    *reinterpret_cast<u32x4*>(out + at) = *reinterpret_cast<const u32x4*>(x + at);
+    return;
+  }
+  float f[8];
+  if (r.neox) {
+    float g[8];
+    const int at = piece * 8;
+    unpack8(*reinterpret_cast<const u32x4*>(x + at), f);
+    unpack8(*reinterpret_cast<const u32x4*>(x + at + r.half), g);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) turn(f[j], g[j], cs[at + j]);
+    *reinterpret_cast<u32x4*>(out + at) = pack8(f);
+    *reinterpret_cast<u32x4*>(out + at + r.half) = pack8(g);
+  } else {
+    unpack8(*reinterpret_cast<const u32x4*>(x + piece * 8), f);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) turn(f[2 * j], f[2 * j + 1], cs[piece * 4 + j]);
+    *reinterpret_cast<u32x4*>(out + piece * 8) = pack8(f);
+  }
+}
+
+constexpr int ROPE_THREADS = 256, ROPE_MAX_HALF = 128, ROPE_MAX_TOKENS = 4;
+
+// The rows of tokens [t0, t0 + nt) of two tensors (the second may have no heads).  Cosine and
+// sine of a token are formed once for all its heads and kept in LDS: with 40 heads of 128 that
+// is 1/40 of the fp64 products that forming them at each pair would take.
+__device__ __forceinline__ void rope_tokens(const Rope& r, const RopeRows& a, const RopeRows& b, int D,
+                                            int64_t t0, int nt, float2* cs) {
+  for (int i = threadIdx.x; i < nt * r.half; i += ROPE_THREADS) {
+    const int k = i / r.half;
+    cs[i] = rope_cos_sin(r, r.positions[t0 + k], i - k * r.half);
+  }
+  __syncthreads();
+  const int turned = r.neox ? r.half / 8 : r.half / 4;
+  const int copied = (D - 2 * r.half) / 8;
+  const int pieces = turned + copied, heads = a.heads + b.heads;
+  for (int i = threadIdx.x; i < nt * heads * pieces; i += ROPE_THREADS) {
+    const int piece = i % pieces, row = i / pieces, head = row % heads, k = row / heads;
+    const RopeRows& m = head < a.heads ? a : b;
+    const int h = head < a.heads ? head : head - a.heads;
+    if (piece >= turned && m.x == m.out) continue;
+    rope_piece(r, m.x + (t0 + k) * m.st + h * m.sh, m.out + (t0 + k) * m.ot + h * m.oh, piece, turned,
+               cs + k * r.half);
+  }
+}
+
+__global__ __launch_bounds__(ROPE_THREADS) void rope_scaled_kernel(Rope r, RopeRows q, RopeRows k, int D,
+                                                                   int64_t tokens, int per_group) {
+  __shared__ float2 cs[ROPE_MAX_TOKENS * ROPE_MAX_HALF];
+  const int64_t t0 = (int64_t)blockIdx.x * per_group;
+  rope_tokens(r, q, k, D, t0, (int)min((int64_t)per_group, tokens - t0), cs);
+}
+
+// Tokens of one workgroup: one while there are few, for the sake of latency; four where that
+// still leaves eight workgroups to each CU.
+inline int rope_group(int64_t tokens) { return tokens >= 8192 ? ROPE_MAX_TOKENS : 1; }
+
+// ----------------------------------------------------------------------------------- store --
+// A wave owns one run: the tokens of a call that follow each other into one block, for one head
+// and one of the two caches.  The wave whose token begins a run (the token before it goes to
+// another block) takes it, so no two waves write one block's scale.  A row of D elements is held
+// by D / 8 lanes, 64 / (D / 8) rows at a time.
+struct StoreParams {
+  const unsigned short *k, *v;
+  int64_t k_st, k_sh, v_st, v_sh;
+  unsigned char *k_cache, *v_cache;
+  int64_t kc_sb, kc_st, kc_sh, vc_sb, vc_st, vc_sh;
+  float *k_scale, *v_scale;  // [blocks, heads]
+  const int64_t* slots;
+  int64_t tokens, num_blocks;
+  int Hk, lb, group;
+  unsigned kv_groups;  // workgroups before those that turn the queries
+  int q_group;
+  Rope rope;           // positions == nullptr: keys are stored as they are
+  RopeRows q;
+};
+
+__device__ __forceinline__ bool finite(float x) {
+  return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u;
+}
+
+// 8 values times a power of two -> 8 e4m3 bytes, to the nearest, ties to even; what is not
+// finite becomes NaN (e4m3 has no infinity)
+__device__ __forceinline__ u32x2 round_fp8(const float (&f)[8], float inv) {
+  u32x2 o;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float g[4];
+    unsigned bad = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float x = f[4 * h + j];
+      if (!finite(x)) bad |= 0x7fu << (8 * j);
+      g[j] = finite(x) ? clamp_fp8(x * inv, -FP8_E4M3_MAX, FP8_E4M3_MAX) : 0.f;
+    }
+    o[h] = cvt4_fp8(g[0], g[1], g[2], g[3]) | bad;
+  }
+  return o;
+}
+
+template <int D, bool KEYS>
+__device__ __forceinline__ void load_row(const StoreParams& p, int64_t t, int head, int c, bool live,
+                                         float (&f)[8]) {
+  constexpr int LPR = D / 8;
+  u32x4 raw = u32x4{0, 0, 0, 0};
+  if (live)
+    raw = *reinterpret_cast<const u32x4*>((KEYS ? p.k + t * p.k_st + head * p.k_sh
+                                                : p.v + t * p.v_st + head * p.v_sh) + 8 * c);
+  unpack8(raw, f);
+  if constexpr (KEYS) {
+    if (p.rope.positions) {
+      const Rope& r = p.rope;
+      const bool mine = 8 * c < 2 * r.half;
+      const int64_t pos = live ? p.rope.positions[t] : 0;
+      if (r.neox) {
+        // the other element of each pair is `half` away: `half / 8` lanes, in the same row
+        const int away = r.half / 8;
+        const bool second = c >= away;
+        const int lane = threadIdx.x & 63;
+        const int from = mine ? (second ? lane - away : lane + away) : lane;
+        u32x4 other;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) other[j] = __shfl(raw[j], from, 64);
+        float g[8];
+        unpack8(other, g);
+        if (mine) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float2 cs = rope_cos_sin(r, pos, (second ? c - away : c) * 8 + j);
+            if (second) turn(g[j], f[j], cs);
+            else turn(f[j], g[j], cs);
+          }
+        }
+      } else if (mine) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) turn(f[2 * j], f[2 * j + 1], rope_cos_sin(r, pos, c * 4 + j));
+      }
+      // the rotated key is a bf16 value before it is rounded to 8 bits, as it would be between
+      // the rotary operator and the store
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = rbf(f[j]);
+    }
+  }
+  static_assert(64 % LPR == 0, "rows of a wave");
+}
+
+template <int D, bool KEYS>
+__device__ void store_run(const StoreParams& p, int64_t t0, int64_t block, int head) {
+  constexpr int LPR = D / 8, RPI = 64 / LPR;
+  const int lane = threadIdx.x & 63, c = lane % LPR, sub = lane / LPR;
+  const int bs = 1 << p.lb;
+  // length of the run, the largest finite magnitude, the smallest place in the block
+  int64_t len = 0;
+  for (;;) {
+    const int64_t t = t0 + len + lane;
+    const int64_t s = t < p.tokens ? p.slots[t] : -1;
+    const unsigned long long out = __ballot(s < 0 || (s >> p.lb) != block);
+    if (out) {
+      len += __ffsll((unsigned long long)out) - 1;
+      break;
+    }
+    len += 64;
+  }
+  float top = 0.f;
+  int first = bs;
+  for (int64_t i = 0; i < len; i += RPI) {
+    const bool live = i + sub < len;
+    const int64_t t = t0 + (live ? i + sub : 0);
+    float f[8];
+    load_row<D, KEYS>(p, t, head, c, live, f);
+    if (live) {
+      first = min(first, (int)(p.slots[t] & (bs - 1)));
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (finite(f[j])) top = fmaxf(top, fabsf(f[j]));
+    }
+  }
+  top = group_max<64>(top);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) first = min(first, __shfl_xor(first, o, 64));
+  // the smallest power of two with top <= 448 * 2^e: 448 = 1.75 * 2^8
+  const unsigned bits = __float_as_uint(top);
+  const int e = max(SCALE_EXP_MIN, (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0));
+  float scale = __uint_as_float((unsigned)(e + 127) << 23);
+  float* scale_at = (KEYS ? p.k_scale : p.v_scale) + block * p.Hk + head;
+  unsigned char* cache = (KEYS ? p.k_cache : p.v_cache) + block * (KEYS ? p.kc_sb : p.vc_sb) +
+                         head * (KEYS ? p.kc_sh : p.vc_sh) + 8 * c;
+  const int64_t row_bytes = KEYS ? p.kc_st : p.vc_st;
+  if (first > 0) {
+    const float old = *scale_at;
+    if (old >= scale) {
+      scale = old;
+    } else if (old > 0.f) {  // the block's earlier tokens to the larger step
+      const float shrink = old / scale;
+      for (int i = sub; i < first; i += RPI) {
+        u32x2* at = reinterpret_cast<u32x2*>(cache + i * row_bytes);
+        const u32x2 w = *at;
+        u32x2 n;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w[h], false);
+          const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(w[h], true);
+          unsigned nan = 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (((w[h] >> (8 * j)) & 0x7f) == 0x7f) nan |= 0x7fu << (8 * j);
+          n[h] = cvt4_fp8(lo[0] * shrink, lo[1] * shrink, hi[0] * shrink, hi[1] * shrink);
+          unsigned keep = 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if ((nan >> (8 * j)) & 0x7f) keep |= 0xffu << (8 * j);
+          n[h] = (n[h] & ~keep) | nan;
+        }
+        *at = n;
+      }
+    }
+  }
+  if (lane == 0) *scale_at = scale;
+  const float inv = 1.f / scale;  // exact: a power of two (a scale that a caller set may be any)
+  for (int64_t i = 0; i < len; i += RPI) {
+    const bool live = i + sub < len;
+    const int64_t t = t0 + (live ? i + sub : 0);
+    float f[8];
+    load_row<D, KEYS>(p, t, head, c, live, f);
+    if (live)
+      *reinterpret_cast<u32x2*>(cache + (p.slots[t] & (bs - 1)) * row_bytes) = round_fp8(f, inv);
+  }
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void kv_store_kernel(StoreParams p) {
+  __shared__ float2 cs[ROPE_MAX_HALF * ROPE_MAX_TOKENS];
+  if (blockIdx.x >= p.kv_groups) {
+    const int64_t t0 = (int64_t)(blockIdx.x - p.kv_groups) * p.q_group;
+    rope_tokens(p.rope, p.q, RopeRows{nullptr, nullptr, 0, 0, 0, 0, 0}, D, t0,
+                (int)min((int64_t)p.q_group, p.tokens - t0), cs);
+    return;
+  }
+  // a wave: (group of tokens, head, keys or values)
+  const int64_t unit = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int64_t which = unit % (2 * p.Hk), g = unit / (2 * p.Hk);
+  const int head = (int)(which >> 1);
+  const int64_t t = g * p.group + lane;
+  const int64_t limit = p.num_blocks << p.lb;
+  int64_t s = -1, before = -1;
+  if (lane < p.group && t < p.tokens) {
+    s = p.slots[t];
+    if (t > 0) before = p.slots[t - 1];
+  }
+  const bool leads = s >= 0 && s < limit && (before < 0 || (before >> p.lb) != (s >> p.lb));
+  unsigned long long todo = __ballot(leads);
+  while (todo) {
+    const int l = __ffsll(todo) - 1;
+    todo &= todo - 1;
+    const int64_t slot = p.slots[g * p.group + l];
+    if (which & 1) store_run<D, false>(p, g * p.group + l, slot >> p.lb, head);
+    else store_run<D, true>(p, g * p.group + l, slot >> p.lb, head);
+  }
+}
+
+bool rope_args_ok(const char* what, int64_t head_size, int64_t rot_dim, const void* inv_freq,
+                  const int64_t* positions, int64_t tokens) {
+  if (tokens && (!positions || !inv_freq)) {
+    mi355_set_error("%s: null pointer", what);
+    return false;
+  }
+  if (rot_dim <= 0 || rot_dim % 16 != 0 || rot_dim > head_size) {
+    mi355_set_error("%s: rot_dim %ld must be a multiple of 16 within the head size %ld", what,
+                    (long)rot_dim, (long)head_size);
+    return false;
+  }
+  return true;
+}
+
+}  // namespace
+
+extern "C" int mi355_kv_block_plan(const int32_t* context_lens, const int32_t* new_lens, int64_t B,
+                                   int32_t* block_table, int64_t table_stride, int64_t table_width,
+                                   const int32_t* free_blocks, int64_t num_free,
+                                   const int32_t* free_begin, int64_t block_size, int64_t num_blocks,
+                                   int64_t* slot_mapping, int64_t* positions, int64_t max_tokens,
+                                   int32_t* cu_seqlens_q, int32_t* seq_lens, int32_t* free_end,
+                                   int32_t* status, void* stream) {
+  MI355_REQUIRE(B >= 0 && B <= PLAN_MAX_REQUESTS, "kv_block_plan: %ld requests, at most %ld in one call",
+                (long)B, (long)PLAN_MAX_REQUESTS);
+  MI355_REQUIRE(block_size_ok(block_size), "kv_block_plan: block size %ld must be a power of two in [16, 1024]",
+                (long)block_size);
+  MI355_REQUIRE(max_tokens >= 0 && max_tokens < (1ll << 31) && num_free >= 0 && num_free < (1ll << 31) &&
+                    num_blocks >= 0 && num_blocks < (1ll << 31) && table_width >= 0 &&
+                    (B <= 1 || table_stride >= table_width),
+                "kv_block_plan: bad size");
+  MI355_REQUIRE(free_begin && cu_seqlens_q && free_end && status, "kv_block_plan: null pointer");
+  MI355_REQUIRE(B == 0 || (context_lens && new_lens && seq_lens && (block_table || table_width == 0)),
+                "kv_block_plan: null pointer");
+  MI355_REQUIRE(max_tokens == 0 || (slot_mapping && positions), "kv_block_plan: null pointer");
+  MI355_REQUIRE(num_free == 0 || free_blocks, "kv_block_plan: null pointer");
+  // every workgroup reads these while the first one writes those
+  MI355_REQUIRE((const void*)free_end != free_begin && (B == 0 || ((const void*)seq_lens != context_lens &&
+                (const void*)seq_lens != new_lens)),
+                "kv_block_plan: seq_lens and free_end must not share memory with the inputs");
+  PlanParams p = {context_lens, new_lens, free_blocks, free_begin, block_table, cu_seqlens_q, seq_lens,
+                  free_end, status, slot_mapping, positions, table_stride, table_width, num_free, num_blocks,
+                  max_tokens, (int)B, log2_of(block_size)};
+  const int64_t groups = max_tokens ? (max_tokens + PLAN_TOKENS - 1) / PLAN_TOKENS : 1;
+  const size_t lds = (size_t)(2 * B) * sizeof(int32_t);
+  hipLaunchKernelGGL(kv_block_plan_kernel, dim3((unsigned)groups), dim3(PLAN_THREADS), lds,
+                     (hipStream_t)stream, p);
+  MI355_CHECK_LAUNCH("kv_block_plan");
+  return MI355_OK;
+}
+
+extern "C" int mi355_rope_scaled(const int64_t* positions, const void* q, void* q_out, const void* k,
+                                 void* k_out, int64_t tokens, int64_t Hq, int64_t Hk, int64_t head_size,
+                                 int64_t rot_dim, int64_t q_st, int64_t q_sh, int64_t qo_st, int64_t qo_sh,
+                                 int64_t k_st, int64_t k_sh, int64_t ko_st, int64_t ko_sh,
+                                 const void* inv_freq, int inv_freq_is_f64, float attn_factor, int is_neox,
+                                 void* stream) {
+  MI355_REQUIRE(tokens >= 0 && Hq >= 0 && Hk >= 0 && tokens < (1ll << 31) && Hq < 65536 && Hk < 65536,
+                "rope_scaled: bad shape");
+  if (tokens == 0 || Hq + Hk == 0) return MI355_OK;
+  MI355_REQUIRE(head_size > 0 && head_size % 8 == 0 && head_size <= 2 * ROPE_MAX_HALF,
+                "rope_scaled: head size %ld must be a multiple of 8, at most 256", (long)head_size);
+  if (!rope_args_ok("rope_scaled", head_size, rot_dim, inv_freq, positions, tokens)) return MI355_EINVAL;
+  MI355_REQUIRE((Hq == 0 || (q && q_out)) && (Hk == 0 || (k && k_out)), "rope_scaled: null pointer");
+  const int64_t strides[] = {q_st, q_sh, qo_st, qo_sh, k_st, k_sh, ko_st, ko_sh};
+  for (int64_t s : strides)
+    MI355_REQUIRE(s % 8 == 0, "rope_scaled: strides must be multiples of 8 elements");
+  MI355_REQUIRE(((uintptr_t)q | (uintptr_t)q_out | (uintptr_t)k | (uintptr_t)k_out) % 16 == 0,
+                "rope_scaled: rows must be 16-byte aligned");
+  Rope r = {positions, inv_freq, inv_freq_is_f64, (int)(rot_dim / 2), is_neox != 0, attn_factor};
+  RopeRows a = {(const unsigned short*)q, (unsigned short*)q_out, q_st, q_sh, qo_st, qo_sh, (int)Hq};
+  RopeRows b = {(const unsigned short*)k, (unsigned short*)k_out, k_st, k_sh, ko_st, ko_sh, (int)Hk};
+  const int per = rope_group(tokens);
+  hipLaunchKernelGGL(rope_scaled_kernel, dim3((unsigned)((tokens + per - 1) / per)), dim3(ROPE_THREADS), 0,
+                     (hipStream_t)stream, r, a, b, (int)head_size, tokens, per);
+  MI355_CHECK_LAUNCH("rope_scaled");
+  return MI355_OK;
+}
+
+extern "C" int mi355_kv_store_fp8(const mi355_kv_store_args* a, void* stream) {
+  MI355_REQUIRE(a != nullptr, "kv_store_fp8: null args");
+  MI355_REQUIRE(a->D == 64 || a->D == 128, "kv_store_fp8: head size %ld not in {64,128}", (long)a->D);
+  MI355_REQUIRE(block_size_ok(a->block_size), "kv_store_fp8: block size %ld must be a power of two in [16, 1024]",
+                (long)a->block_size);
+  MI355_REQUIRE(a->tokens >= 0 && a->tokens < (1ll << 31) && a->Hk > 0 && a->Hk < 65536 && a->Hq >= 0 &&
+                    a->Hq < 65536 && a->num_blocks >= 0 && a->num_blocks < (1ll << 31),
+                "kv_store_fp8: bad shape");
+  if (a->tokens == 0) return MI355_OK;
+  MI355_REQUIRE(a->k && a->v && a->slot_mapping, "kv_store_fp8: null pointer");
+  MI355_REQUIRE(a->num_blocks == 0 || (a->k_cache && a->v_cache && a->k_scale && a->v_scale),
+                "kv_store_fp8: null pointer");
+  const int64_t strides[] = {a->k_st, a->k_sh, a->v_st, a->v_sh, a->kc_sb, a->kc_st, a->kc_sh, a->vc_sb,
+                             a->vc_st, a->vc_sh, a->q_st, a->q_sh, a->qo_st, a->qo_sh};
+  for (int64_t s : strides)
+    MI355_REQUIRE(s % 8 == 0, "kv_store_fp8: strides must be multiples of 8 elements");
+  MI355_REQUIRE(((uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->q | (uintptr_t)a->q_out) % 16 == 0 &&
+                    ((uintptr_t)a->k_cache | (uintptr_t)a->v_cache) % 8 == 0,
+                "kv_store_fp8: rows must be 16-byte aligned (cache rows 8-byte)");
+  const bool turn_keys = a->positions != nullptr;
+  if (turn_keys &&
+      !rope_args_ok("kv_store_fp8", a->D, a->rot_dim, a->inv_freq, a->positions, a->tokens))
+    return MI355_EINVAL;
+  MI355_REQUIRE(a->Hq == 0 || (turn_keys && a->q && a->q_out),
+                "kv_store_fp8: queries need positions and both their pointers");
+  StoreParams p;
+  p.k = (const unsigned short*)a->k;
+  p.v = (const unsigned short*)a->v;
+  p.k_st = a->k_st; p.k_sh = a->k_sh; p.v_st = a->v_st; p.v_sh = a->v_sh;
+  p.k_cache = (unsigned char*)a->k_cache;
+  p.v_cache = (unsigned char*)a->v_cache;
+  p.kc_sb = a->kc_sb; p.kc_st = a->kc_st; p.kc_sh = a->kc_sh;
+  p.vc_sb = a->vc_sb; p.vc_st = a->vc_st; p.vc_sh = a->vc_sh;
+  p.k_scale = a->k_scale;
+  p.v_scale = a->v_scale;
+  p.slots = a->slot_mapping;
+  p.tokens = a->tokens;
+  p.num_blocks = a->num_blocks;
+  p.Hk = (int)a->Hk;
+  p.lb = log2_of(a->block_size);
+  // Tokens that a wave looks at for the beginning of a run: one while there are few tokens (each
+  // may be a request of its own, and runs that one wave finds are stored one after the other),
+  // sixteen where tokens mostly follow each other and waves without a run would only be launched.
+  p.group = a->tokens <= 2048 ? 1 : 16;
+  const int64_t units = (a->tokens + p.group - 1) / p.group * 2 * a->Hk;
+  p.kv_groups = (unsigned)((units + 3) / 4);
+  p.q_group = rope_group(a->tokens);
+  const unsigned q_groups = a->Hq ? (unsigned)((a->tokens + p.q_group - 1) / p.q_group) : 0;
+  p.rope = Rope{a->positions, a->inv_freq, a->inv_freq_is_f64, (int)(a->rot_dim / 2), a->is_neox != 0,
+                a->attn_factor};
+  p.q = RopeRows{(const unsigned short*)a->q, (unsigned short*)a->q_out, a->q_st, a->q_sh, a->qo_st, a->qo_sh,
+                 (int)a->Hq};
+  const dim3 grid(p.kv_groups + q_groups), block(256);
+  if (a->D == 128) hipLaunchKernelGGL(kv_store_kernel<128>, grid, block, 0, (hipStream_t)stream, p);
+  else hipLaunchKernelGGL(kv_store_kernel<64>, grid, block, 0, (hipStream_t)stream, p);
+  MI355_CHECK_LAUNCH("kv_store_fp8");
+  return MI355_OK;
+}

@@ -1,0 +1,1015 @@
+// Attention of new tokens over a paged key/value cache held in 8 bits, for gfx950.
+//
+//   out[i] = sum_j softmax_j(q_i . k_j * scale) v_j,  k_j = ks[block(j), head] * e4m3 codes, v alike;
+//   token i of the n new ones of a sequence of L tokens stands at place L - n + i and sees the keys
+//   j <= place (causal), j >= place - window.
+//
+// The query heads that share a key/value head are rows of one product, so every cache byte is
+// read once for all of them.  Codes are widened to bf16 (keys) and half (values) without loss and
+// go through the 16-bit matrix instructions; scales never touch the codes:
+//   p~_j = exp2(s_j * (ks * scale * log2 e) + log2(vs_j) - m)      one exponential for each score
+//   O   += p~_j * codes_j,   l += p~_j / vs_j,   out = O / l
+// with m a running reference near the row's maximum of the exponent.  So a value block's scale
+// costs one addend in the exponent, and p~ in half keeps its 11 bits whatever the scales are.
+//
+// Work is cut into items: a tile of rows of one sequence and key/value head against a chunk of
+// its keys.  Lengths are known on the device only, so each workgroup adds up the work of all
+// sequences, from that takes the length of a chunk that makes about as many items as the chip
+// holds workgroups, and finds its own item.  Chunks of one row tile are joined by a second kernel.
+#include <atomic>
+
+#include "common.h"
+
+namespace {
+
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __fp16 hw_f16x4 __attribute__((__vector_size__(4 * sizeof(__fp16))));
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int KT = 64;               // keys of a tile
+constexpr float M_START = -1e30f;    // reference of a row that has seen nothing yet
+constexpr float LAZY_SUM = 8192.f;   // a lane's sum of a tile's exponentials up to which m stays
+
+struct PagedParams {
+  const unsigned short* q;
+  unsigned short* o;
+  float* lse;
+  const unsigned char *kc, *vc;
+  const float *ks, *vs;
+  const int32_t *cu, *lens, *table;
+  int64_t q_sb, q_ss, q_sh, o_sb, o_ss, o_sh, lse_sb, lse_sh;
+  int64_t kc_sb, kc_st, kc_sh, vc_sb, vc_st, vc_sh;
+  int64_t table_stride;
+  int B, Hk, G, Sq;  // Sq: rows of q (packed) or of each sequence (cu == nullptr)
+  int cap;           // tokens that a row of the table has room for
+  int num_blocks, lb, causal, window;
+  float scale_log2;
+  // items
+  int items, target, chunk_min, split;
+  float* part;       // [Hk * items][M][D + 2]
+  int32_t* info;     // [items][4]: sequence, row tile, chunk, chunks
+};
+
+struct Seq {
+  int first, n, len;  // first row of q, new tokens, tokens in all
+};
+__device__ __forceinline__ Seq seq_of(const PagedParams& p, int b) {
+  Seq s;
+  s.len = min(max(p.lens[b], 0), p.cap);
+  if (p.cu) {
+    s.first = min(max(p.cu[b], 0), p.Sq);
+    s.n = max(min(p.cu[b + 1], p.Sq) - s.first, 0);
+  } else {
+    s.first = 0;
+    s.n = p.Sq;
+  }
+  return s;
+}
+// tiles of keys that any row of the sequence sees: [lo, hi)
+__device__ __forceinline__ void seq_tiles(const PagedParams& p, const Seq& s, int& lo, int& hi) {
+  const int64_t first = p.window >= 0 ? (int64_t)s.len - s.n - p.window : 0;
+  lo = first > 0 ? (int)(first / KT) : 0;
+  hi = (s.len + KT - 1) / KT;
+  if (hi < lo) hi = lo;
+}
+
+struct Item {
+  int b, tile, chunk, chunks;  // sequence, row tile, chunk of keys and how many there are
+  int length;                  // tiles of a chunk
+};
+
+// Sum of a value over the 256 threads of the workgroup, and (second form) the sum over the
+// threads before this one.
+__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* total, int64_t (&wave_sum)[8]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int64_t in = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const long long a = __shfl_up((long long)in, o, 64);
+    if (lane >= o) in += a;
+  }
+  __syncthreads();
+  if (lane == 63) wave_sum[wave] = in;
+  __syncthreads();
+  int64_t before = in - v, all = 0;
+  const int waves = blockDim.x >> 6;
+  for (int w = 0; w < waves; ++w) {
+    if (w < wave) before += wave_sum[w];
+    all += wave_sum[w];
+  }
+  *total = all;
+  return before;
+}
+
+// The item'th item of a key/value head; false behind the last one.  Every thread of the
+// workgroup calls it.
+template <int M>
+__device__ bool find_item(const PagedParams& p, int item, bool writes_info, Item* out) {
+  __shared__ int64_t sums[8];
+  __shared__ Item found;
+  const int per = (p.B + blockDim.x - 1) / blockDim.x;
+  const int b0 = threadIdx.x * per, b1 = min(p.B, b0 + per);
+  int length = 1 << 30;
+  int64_t all;
+  if (threadIdx.x == 0) found.b = -1;
+  if (p.split) {
+    int64_t work = 0;
+    for (int b = b0; b < b1; ++b) {
+      const Seq s = seq_of(p, b);
+      int lo, hi;
+      seq_tiles(p, s, lo, hi);
+      work += (((int64_t)s.n * p.G + M - 1) / M) * (hi - lo);
+    }
+    block_scan(work, &all, sums);
+    length = (int)min((int64_t)(1 << 30), max((int64_t)p.chunk_min, (all + p.target - 1) / p.target));
+  }
+  int64_t mine = 0;
+  for (int b = b0; b < b1; ++b) {
+    const Seq s = seq_of(p, b);
+    int lo, hi;
+    seq_tiles(p, s, lo, hi);
+    mine += (((int64_t)s.n * p.G + M - 1) / M) * max(1, (hi - lo + length - 1) / length);
+  }
+  int64_t at = block_scan(mine, &all, sums);
+  if (item >= at && item < at + mine) {
+    for (int b = b0; b < b1; ++b) {
+      const Seq s = seq_of(p, b);
+      int lo, hi;
+      seq_tiles(p, s, lo, hi);
+      const int64_t tiles = ((int64_t)s.n * p.G + M - 1) / M;
+      const int chunks = max(1, (hi - lo + length - 1) / length);
+      if (item < at + tiles * chunks) {
+        const int k = (int)(item - at);
+        // causal rows further down see more: they begin first
+        found = Item{b, (int)tiles - 1 - k / chunks, k % chunks, chunks, length};
+        break;
+      }
+      at += tiles * chunks;
+    }
+  }
+  __syncthreads();
+  *out = found;
+  if (writes_info && p.split && threadIdx.x == 0) {
+    int32_t* to = p.info + 4 * (int64_t)item;
+    to[0] = found.b;
+    to[1] = found.tile;
+    to[2] = found.chunk;
+    to[3] = found.b < 0 ? 0 : found.chunks;
+  }
+  return found.b >= 0;
+}
+
+// What a workgroup reads of its item: rows, the tiles of keys and the places its rows stand at.
+struct Job {
+  Seq s;
+  int b, hk, rows, row0;       // rows of the sequence for this head, first one of the tile
+  int place_lo, place_hi;      // of the tile's first and last row
+  int t0, t1;                  // tiles of keys
+};
+template <int M>
+__device__ __forceinline__ Job job_of(const PagedParams& p, const Item& it, int hk) {
+  Job j;
+  j.s = seq_of(p, it.b);
+  j.b = it.b;
+  j.hk = hk;
+  j.rows = j.s.n * p.G;
+  j.row0 = it.tile * M;
+  const int base = j.s.len - j.s.n;
+  j.place_lo = base + j.row0 / p.G;
+  j.place_hi = base + min(j.row0 + M - 1, j.rows - 1) / p.G;
+  int lo, hi;
+  seq_tiles(p, j.s, lo, hi);
+  j.t0 = lo + it.chunk * it.length;
+  j.t1 = (int)min((int64_t)hi, (int64_t)j.t0 + it.length);
+  if (p.causal) j.t1 = min(j.t1, j.place_hi < 0 ? 0 : j.place_hi / KT + 1);
+  if (p.window >= 0 && j.place_lo - p.window > 0) j.t0 = max(j.t0, (j.place_lo - p.window) / KT);
+  return j;
+}
+
+// A 16-key piece of a tile lies in one block (blocks hold 16 tokens or more).  Pieces behind the
+// end and blocks that are not of the pool are not read: `ok` is false and the block is 0.
+struct Piece {
+  int block, off;
+  bool ok;
+};
+__device__ __forceinline__ Piece piece_of(const PagedParams& p, const Job& j, int key) {
+  Piece c;
+  c.ok = key < j.s.len;
+  c.off = key & ((1 << p.lb) - 1);
+  c.block = c.ok ? p.table[j.b * p.table_stride + (key >> p.lb)] : 0;
+  c.ok = c.ok && c.block >= 0 && c.block < p.num_blocks;
+  if (!c.ok) c.block = c.off = 0;
+  return c;
+}
+
+// scales of a piece: factor of the score, addend of the exponent, weight in the row sum
+struct Scales {
+  float k, v_log, v_inv;
+};
+__device__ __forceinline__ Scales scales_of(const PagedParams& p, const Piece& c, int hk) {
+  const int64_t at = (int64_t)c.block * p.Hk + hk;
+  const float vs = c.ok ? fminf(fmaxf(p.vs[at], 0x1p-64f), 0x1p120f) : 1.f;
+  return Scales{c.ok ? p.ks[at] * p.scale_log2 : 0.f, __builtin_amdgcn_logf(vs), 1.f / vs};
+}
+
+// Without branches on purpose: a conditional write into one element of a matrix instruction's
+// result, with control flow around it, has come out of the compiler with the write missing.
+__device__ __forceinline__ bool sees(bool ok, int key, int lo, int hi) {
+  return (int)ok & (int)(key >= lo) & (int)(key <= hi);
+}
+
+__device__ __forceinline__ bf16x8 widen_bf16(unsigned a, unsigned b) {
+  const bf16x2 x0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.f, false);
+  const bf16x2 x1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.f, true);
+  const bf16x2 x2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.f, false);
+  const bf16x2 x3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.f, true);
+  return bf16x8{x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
+}
+__device__ __forceinline__ f16x8 widen_f16(unsigned a, unsigned b) {
+  const f16x2 x0 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.f, false);
+  const f16x2 x1 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.f, true);
+  const f16x2 x2 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.f, false);
+  const f16x2 x3 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.f, true);
+  return f16x8{x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
+}
+// does any of the four e4m3 codes stand for NaN (0x7f, 0xff)?
+__device__ __forceinline__ unsigned nan_codes(unsigned w) {
+  return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+}
+// NaN values replaced by 0, and where they were by 1
+__device__ __forceinline__ f16x8 without_nan(f16x8 v, f16x8* where) {
+  f16x8 o;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const bool n = v[j] != v[j];
+    o[j] = n ? (_Float16)0.f : v[j];
+    (*where)[j] = n ? (_Float16)1.f : (_Float16)0.f;
+  }
+  return o;
+}
+
+// ----------------------------------------------------------------- few rows: 16 or 32 of them --
+// Four waves share the rows and take turns at the tiles of the chunk; each keeps its own m, l and
+// O, joined through LDS at the end.  A wave's tile: keys straight to registers (lane: key l & 15,
+// 16 bytes of the head at (l >> 4) * 16: two k-steps of the 16x16x32 product), values through its
+// own 64-row image in LDS, from which ds_read_b64_tr_b8 reads eight keys of one channel.  Both
+// are loaded one tile ahead into the registers that the current tile has just left.
+//   S^T[key][row] = K . Q^T: a lane holds row l & 15, keys 4 (l >> 4) + i of each piece;
+//   O^T[channel][row] += V^T . P^T: the same registers are the second operand, if the k index
+//   8 g + j counts keys 4 g + j of the first piece, then of the second one.
+template <int D, int RT>
+__global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
+  constexpr int M = 16 * RT, NH = D / 64, CPR = D / 16, DB = D / 16;
+  __shared__ __attribute__((aligned(16))) unsigned char vimg[4][KT * D];
+  __shared__ float wave_m[4][M], wave_l[4][M];
+  const int item = blockIdx.x / p.Hk, hk = blockIdx.x % p.Hk;
+  Item it;
+  if (!find_item<M>(p, item, hk == 0, &it)) return;
+  const Job job = job_of<M>(p, it, hk);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, g = lane >> 4;
+
+  bf16x8 qf[RT][NH][2];
+  int see_lo[RT], see_hi[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int row = min(job.row0 + 16 * rt + r, job.rows - 1), tok = row / p.G, h = row - tok * p.G;
+    const unsigned short* qp = p.q + job.b * p.q_sb + (int64_t)(job.s.first + tok) * p.q_ss +
+                               (int64_t)(hk * p.G + h) * p.q_sh + 16 * g;
+#pragma unroll
+    for (int h2 = 0; h2 < NH; ++h2)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) qf[rt][h2][u] = *reinterpret_cast<const bf16x8*>(qp + 64 * h2 + 8 * u);
+    const int place = job.s.len - job.s.n + tok;
+    see_hi[rt] = min(p.causal ? place : job.s.len - 1, job.s.len - 1);
+    see_lo[rt] = p.window >= 0 ? place - p.window : 0;
+  }
+
+  f32x4 o[RT][DB];
+  float m[RT], l[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    m[rt] = M_START;
+    l[rt] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) o[rt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  u32x4 kr[4][NH], vr[CPR];
+  auto load_k = [&](const Piece (&pc)[4]) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const unsigned char* at = p.kc + pc[c].block * p.kc_sb + (int64_t)pc[c].off * p.kc_st + hk * p.kc_sh +
+                                (int64_t)r * p.kc_st + 16 * g;
+#pragma unroll
+      for (int h = 0; h < NH; ++h) kr[c][h] = *reinterpret_cast<const u32x4*>(at + 64 * h);
+    }
+  };
+  auto load_v = [&](const Piece (&pc)[4]) {
+#pragma unroll
+    for (int i = 0; i < CPR; ++i) {
+      const int row = (i * 64 + lane) / CPR;
+      const Piece c = pc[i * 4 / CPR];
+      vr[i] = *reinterpret_cast<const u32x4*>(p.vc + c.block * p.vc_sb + (int64_t)(c.off + (row & 15)) * p.vc_st +
+                                              hk * p.vc_sh + (lane % CPR) * 16);
+    }
+  };
+  auto swz = [](int row) { return D == 128 ? (row >> 1) & 7 : (row >> 2) & 3; };
+  unsigned char* img = vimg[wave];
+  const int tr_row = (r >> 1) < 4 ? 4 * g + (r >> 1) : 12 + 4 * g + (r >> 1);
+  const int tr_swz = swz(tr_row);
+  const unsigned char* tr_at = img + tr_row * D + (r & 1) * 8;
+
+  Piece pc[4], nx[4];
+  int t = job.t0 + wave;
+  if (t < job.t1) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) pc[c] = piece_of(p, job, t * KT + 16 * c);
+    load_k(pc);
+    load_v(pc);
+  }
+  for (; t < job.t1; t += 4) {
+    const bool more = t + 4 < job.t1;
+    if (more) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) nx[c] = piece_of(p, job, (t + 4) * KT + 16 * c);
+    }
+    Scales sc[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) sc[c] = scales_of(p, pc[c], hk);
+    const int key0 = t * KT;
+    const bool whole = key0 + KT <= job.s.len && pc[0].ok && pc[1].ok && pc[2].ok && pc[3].ok;
+    const bool masked = !whole || (p.causal && key0 + KT - 1 > job.place_lo) ||
+                        (p.window >= 0 && key0 < job.place_hi - p.window);
+    // values into the image; rows that are no keys of the sequence as zeros (0 * NaN is NaN)
+    bool nan_values = false;
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < CPR; ++i) {
+        const int key = key0 + (i * 64 + lane) / CPR;
+        if (!pc[i * 4 / CPR].ok || key >= job.s.len) vr[i] = u32x4{0, 0, 0, 0};
+      }
+    }
+    if (masked) {
+      unsigned any = 0;
+#pragma unroll
+      for (int i = 0; i < CPR; ++i)
+        any |= nan_codes(vr[i][0]) | nan_codes(vr[i][1]) | nan_codes(vr[i][2]) | nan_codes(vr[i][3]);
+      nan_values = __builtin_amdgcn_ballot_w64(any != 0) != 0;
+    }
+#pragma unroll
+    for (int i = 0; i < CPR; ++i) {
+      const int row = (i * 64 + lane) / CPR;
+      *reinterpret_cast<u32x4*>(img + row * D + (((lane % CPR) ^ swz(row)) << 4)) = vr[i];
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (more) load_v(nx);
+
+    f32x4 s[RT][4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) s[rt][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int h = 0; h < NH; ++h)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const bf16x8 kf = widen_bf16(kr[c][h][2 * u], kr[c][h][2 * u + 1]);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
+            s[rt][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[rt][h][u], s[rt][c], 0, 0, 0);
+        }
+    }
+    if (more) load_k(nx);
+
+    f16x8 pf[RT][2], seen[RT][2];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      // exponents, then exponentials against the reference as it stands; it moves, and O and l
+      // with it, only where a lane's sum says that it has to
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[rt][c][i] = fmaf(s[rt][c][i], sc[c].k, sc[c].v_log);
+      if (masked) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            s[rt][c][i] = sees(pc[c].ok, key0 + 16 * c + 4 * g + i, see_lo[rt], see_hi[rt]) ? s[rt][c][i] : -INFINITY;
+      }
+      f32x4 e[4];
+      float sum[4], all;
+      auto exponentials = [&]() {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) e[c][i] = __builtin_amdgcn_exp2f(s[rt][c][i] - m[rt]);
+          sum[c] = (e[c][0] + e[c][1]) + (e[c][2] + e[c][3]);
+        }
+        all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      };
+      exponentials();
+      if (__builtin_amdgcn_ballot_w64(!(all <= LAZY_SUM)) != 0) {
+        float top = s[rt][0][0];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top = fmaxf(top, s[rt][c][i]);
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float now = fmaxf(m[rt], top), shrink = __builtin_amdgcn_exp2f(m[rt] - now);
+        m[rt] = now;
+        l[rt] *= shrink;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) o[rt][d] *= shrink;
+        exponentials();
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) l[rt] = fmaf(sum[c], sc[c].v_inv, l[rt]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pf[rt][c >> 1][4 * (c & 1) + i] = (_Float16)e[c][i];
+      if (nan_values) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            seen[rt][c >> 1][4 * (c & 1) + i] =
+                sees(pc[c].ok, key0 + 16 * c + 4 * g + i, see_lo[rt], see_hi[rt]) ? (_Float16)1.f : (_Float16)0.f;
+      }
+    }
+    auto values = [&](int st, int d) {
+      const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+          (__attribute__((address_space(3))) i32x2*)(tr_at + st * 32 * D + ((d ^ tr_swz) << 4)));
+      return widen_f16((unsigned)w[0], (unsigned)w[1]);
+    };
+    if (!nan_values) {
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+          const f16x8 vf = values(st, d);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
+            o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[rt][st], o[rt][d], 0, 0, 0);
+        }
+    } else {
+      // A tile that some row sees in part, with NaN among its values: a row must not get one from
+      // a key that it does not see.  The product runs without them, and a second one counts, for
+      // each row and channel, the NaN that the row does see.
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        f32x4 count[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) count[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+          f16x8 where;
+          const f16x8 vf = without_nan(values(st, d), &where);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) {
+            o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[rt][st], o[rt][d], 0, 0, 0);
+            count[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(where, seen[rt][st], count[rt], 0, 0, 0);
+          }
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (count[rt][i] > 0.f) o[rt][d][i] = __builtin_nanf("");
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int c = 0; c < 4; ++c) pc[c] = nx[c];
+  }
+
+  // ---- the four waves' parts of each row, joined ----
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    l[rt] += __shfl_xor(l[rt], 16, 64);
+    l[rt] += __shfl_xor(l[rt], 32, 64);
+    if (g == 0) {
+      wave_m[wave][16 * rt + r] = m[rt];
+      wave_l[wave][16 * rt + r] = l[rt];
+    }
+  }
+  float* part = nullptr;
+  if (it.chunks > 1) part = p.part + ((int64_t)hk * p.items + item) * (M * (D + 2));
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    __syncthreads();
+    float top = wave_m[0][16 * rt + r];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) top = fmaxf(top, wave_m[w][16 * rt + r]);
+    const float weight = __builtin_amdgcn_exp2f(m[rt] - top);
+    // [16 rows][D] fp32 in the wave's image (64 D bytes), 16-byte pieces turned by the row
+    float* mine = reinterpret_cast<float*>(vimg[wave]);
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+      *reinterpret_cast<f32x4*>(mine + r * D + (((4 * d + g) ^ (r & 7)) << 2)) = o[rt][d] * weight;
+    __syncthreads();
+    // four channels of a row for each thread
+    for (int i = threadIdx.x; i < 16 * D / 4; i += 256) {
+      const int row = i / (D / 4), c4 = i % (D / 4), at = row * D + ((c4 ^ (row & 7)) << 2);
+      f32x4 sum = *reinterpret_cast<const f32x4*>(reinterpret_cast<float*>(vimg[0]) + at);
+#pragma unroll
+      for (int w = 1; w < 4; ++w)
+        sum = sum + *reinterpret_cast<const f32x4*>(reinterpret_cast<float*>(vimg[w]) + at);
+      const int in_tile = 16 * rt + row;
+      float rm = wave_m[0][in_tile], rl = 0.f;
+#pragma unroll
+      for (int w = 1; w < 4; ++w) rm = fmaxf(rm, wave_m[w][in_tile]);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) rl = fmaf(wave_l[w][in_tile], __builtin_amdgcn_exp2f(wave_m[w][in_tile] - rm), rl);
+      if (part) {
+        *reinterpret_cast<f32x4*>(part + in_tile * D + 4 * c4) = sum;
+        if (c4 == 0) {
+          part[M * D + 2 * in_tile] = rm;
+          part[M * D + 2 * in_tile + 1] = rl;
+        }
+        continue;
+      }
+      const int q_row = job.row0 + in_tile;
+      if (q_row >= job.rows) continue;
+      const int tok = q_row / p.G, head = hk * p.G + q_row - tok * p.G;
+      const float inv = rl == 0.f ? 0.f : 1.f / rl;
+      *reinterpret_cast<u32x2*>(p.o + job.b * p.o_sb + (int64_t)(job.s.first + tok) * p.o_ss + head * p.o_sh +
+                                4 * c4) = u32x2{pack_bf2(sum[0] * inv, sum[1] * inv), pack_bf2(sum[2] * inv, sum[3] * inv)};
+      if (p.lse && c4 == 0)
+        p.lse[job.b * p.lse_sb + head * p.lse_sh + job.s.first + tok] =
+            rl == 0.f ? -INFINITY : (rm + __builtin_amdgcn_logf(rl)) * 0.6931471805599453f;
+    }
+  }
+}
+
+// --------------------------------------------------------------------------------- many rows --
+// 32 rows for each of four waves, which share the tiles of keys in LDS, widened to 16 bits once
+// for all of them while they are stored there: loaded to registers a tile ahead, converted, two
+// stages, one barrier for each tile.  Products and layouts are those of the dense kernel
+// (attention.hip): S^T = K . Q^T with 32x32x16 instructions, the row on the lane; P^T is the
+// second operand of O^T += V^T . P^T as it stands; values through the transposing LDS read.
+template <int D, int NW>
+__global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedParams p) {
+  constexpr int M = 32 * NW, ROWB = 2 * D, CPR = ROWB / 16, KSTEPS = D / 16, DVB = D / 32;
+  constexpr int TILE = KT * ROWB, LOADS = KT * D / 16 / (NW * 64);
+  static_assert(LOADS >= 1, "every thread loads");
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  __shared__ int nan_flag[2];
+  const int item = blockIdx.x / p.Hk, hk = blockIdx.x % p.Hk;
+  Item it;
+  if (!find_item<M>(p, item, hk == 0, &it)) return;
+  const Job job = job_of<M>(p, it, hk);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 31, hh = lane >> 5;
+  auto k_swz = [](int key) { return key & 15 & (CPR - 1); };
+  auto v_swz = [](int key) { return (((key & 3) << 2) | ((key >> 2) & 3)) & (CPR - 1); };
+
+  const int row = min(job.row0 + 32 * wave + r, job.rows - 1), tok = row / p.G, head = hk * p.G + row - tok * p.G;
+  const int base = job.s.len - job.s.n, place = base + tok;
+  const int see_hi = min(p.causal ? place : job.s.len - 1, job.s.len - 1);
+  const int see_lo = p.window >= 0 ? place - p.window : 0;
+  // places of the wave's first and last row
+  const int wave_row = min(job.row0 + 32 * wave, job.rows - 1);
+  const int w_lo = base + wave_row / p.G, w_hi = base + min(wave_row + 31, job.rows - 1) / p.G;
+  bf16x8 qf[KSTEPS];
+  {
+    const unsigned short* qp = p.q + job.b * p.q_sb + (int64_t)(job.s.first + tok) * p.q_ss + (int64_t)head * p.q_sh;
+#pragma unroll
+    for (int s = 0; s < KSTEPS; ++s) qf[s] = *reinterpret_cast<const bf16x8*>(qp + 16 * s + 8 * hh);
+  }
+
+  u32x4 kr[LOADS], vr[LOADS];
+  // thread's 16 bytes of a tile: row (i * threads + tid) / (D / 16), all of a wave in one piece
+  auto load = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int key = (i * NW * 64 + tid) / (D / 16), c = tid % (D / 16);
+      const int piece = __builtin_amdgcn_readfirstlane(key >> 4);
+      const Piece pc = piece_of(p, job, t * KT + 16 * piece);
+      const int64_t off = pc.off + (key & 15);
+      kr[i] = *reinterpret_cast<const u32x4*>(p.kc + pc.block * p.kc_sb + off * p.kc_st + hk * p.kc_sh + 16 * c);
+      vr[i] = *reinterpret_cast<const u32x4*>(p.vc + pc.block * p.vc_sb + off * p.vc_st + hk * p.vc_sh + 16 * c);
+      if (!pc.ok || t * KT + key >= job.s.len) vr[i] = u32x4{0, 0, 0, 0};
+    }
+  };
+  auto store = [&](int t, int buf) {
+    unsigned any = 0;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int key = (i * NW * 64 + tid) / (D / 16), c = tid % (D / 16);
+      unsigned char* kt = smem + buf * 2 * TILE + key * ROWB;
+      unsigned char* vt = kt + TILE;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        *reinterpret_cast<bf16x8*>(kt + (((2 * c + h) ^ k_swz(key)) << 4)) = widen_bf16(kr[i][2 * h], kr[i][2 * h + 1]);
+        *reinterpret_cast<f16x8*>(vt + (((2 * c + h) ^ v_swz(key)) << 4)) = widen_f16(vr[i][2 * h], vr[i][2 * h + 1]);
+      }
+      any |= nan_codes(vr[i][0]) | nan_codes(vr[i][1]) | nan_codes(vr[i][2]) | nan_codes(vr[i][3]);
+    }
+    if (any) nan_flag[buf] = t + 1;  // this tile's mark: never one left by an earlier tile
+  };
+
+  int koff[KSTEPS];
+#pragma unroll
+  for (int s = 0; s < KSTEPS; ++s) koff[s] = r * ROWB + (((2 * s + hh) ^ k_swz(r)) << 4);
+  const int li = lane & 15, qq = li >> 2, pp = li & 3, g2 = (lane >> 4) & 1;
+  int vlane[DVB][2];
+#pragma unroll
+  for (int d = 0; d < DVB; ++d)
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int key = half * 8 + 4 * hh + qq, col = d * 32 + g2 * 16 + 4 * pp;
+      vlane[d][half] = key * ROWB + (((col >> 3) ^ v_swz(key)) << 4) + ((col & 7) << 1);
+    }
+
+  f32x16 o[DVB];
+#pragma unroll
+  for (int d = 0; d < DVB; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
+  float m = M_START, l = 0.f;
+
+  if (tid < 2) nan_flag[tid] = 0;
+  __syncthreads();
+  if (job.t0 < job.t1) {
+    load(job.t0);
+    store(job.t0, 0);
+  }
+  for (int t = job.t0; t < job.t1; ++t) {
+    const int buf = (t - job.t0) & 1, key0 = t * KT;
+    __syncthreads();
+    const bool more = t + 1 < job.t1;
+    if (more) load(t + 1);
+    if (!(p.causal && key0 > w_hi) && !(p.window >= 0 && key0 + KT - 1 < w_lo - p.window)) {
+      Piece pc[4];
+      Scales sc[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        pc[c] = piece_of(p, job, key0 + 16 * c);
+        sc[c] = scales_of(p, pc[c], hk);
+      }
+      const bool masked = key0 + KT > job.s.len || !(pc[0].ok && pc[1].ok && pc[2].ok && pc[3].ok) ||
+                          (p.causal && key0 + KT - 1 > w_lo) || (p.window >= 0 && key0 < w_hi - p.window);
+      const unsigned char *kt = smem + buf * 2 * TILE, *vt = kt + TILE;
+      f32x16 s[2];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[kb][e] = 0.f;
+#pragma unroll
+      for (int st = 0; st < KSTEPS; ++st)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+          const bf16x8 kf = *reinterpret_cast<const bf16x8*>(kt + kb * 32 * ROWB + koff[st]);
+          s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[st], s[kb], 0, 0, 0);
+        }
+      auto visible = [&](int kb, int e) {
+        return sees(pc[2 * kb + (e >> 3)].ok, key0 + kb * 32 + (e & 3) + 8 * (e >> 2) + 4 * hh, see_lo, see_hi);
+      };
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const Scales& c = sc[2 * kb + (e >> 3)];
+          s[kb][e] = fmaf(s[kb][e], c.k, c.v_log);
+        }
+      if (masked) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            s[kb][e] = visible(kb, e) ? s[kb][e] : -INFINITY;
+      }
+      float pe[2][16], sum[4], all;
+      auto exponentials = [&]() {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          sum[c] = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            pe[c >> 1][8 * (c & 1) + e] = __builtin_amdgcn_exp2f(s[c >> 1][8 * (c & 1) + e] - m);
+            sum[c] += pe[c >> 1][8 * (c & 1) + e];
+          }
+        }
+        all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      };
+      exponentials();
+      if (__builtin_amdgcn_ballot_w64(!(all <= LAZY_SUM)) != 0) {
+        float top = s[0][0];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) top = fmaxf(top, s[kb][e]);
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float now = fmaxf(m, top), shrink = __builtin_amdgcn_exp2f(m - now);
+        m = now;
+        l *= shrink;
+#pragma unroll
+        for (int d = 0; d < DVB; ++d)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[d][e] *= shrink;
+        exponentials();
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) l = fmaf(sum[c], sc[c].v_inv, l);
+      f16x8 pf[2][2];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int st = 0; st < 2; ++st)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) pf[kb][st][j] = (_Float16)pe[kb][8 * st + j];
+      auto values = [&](int kb, int st, int d) {
+        const unsigned char* at = vt + (kb * 32 + st * 16) * ROWB;
+        const f16x4 a = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16(
+            (__attribute__((address_space(3))) hw_f16x4*)(at + vlane[d][0])));
+        const f16x4 b = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16(
+            (__attribute__((address_space(3))) hw_f16x4*)(at + vlane[d][1])));
+        return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+      };
+      if (!masked || nan_flag[buf] != t + 1) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int st = 0; st < 2; ++st)
+#pragma unroll
+            for (int d = 0; d < DVB; ++d)
+              o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(values(kb, st, d), pf[kb][st], o[d], 0, 0, 0);
+      } else {  // as in the kernel above
+        f16x8 seen[2][2];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int st = 0; st < 2; ++st)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              seen[kb][st][j] = visible(kb, 8 * st + j) ? (_Float16)1.f : (_Float16)0.f;
+#pragma unroll
+        for (int d = 0; d < DVB; ++d) {
+          f32x16 count;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) count[e] = 0.f;
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int st = 0; st < 2; ++st) {
+              f16x8 where;
+              const f16x8 vf = without_nan(values(kb, st, d), &where);
+              o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[kb][st], o[d], 0, 0, 0);
+              count = __builtin_amdgcn_mfma_f32_32x32x16_f16(where, seen[kb][st], count, 0, 0, 0);
+            }
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (count[e] > 0.f) o[d][e] = __builtin_nanf("");
+        }
+      }
+    }
+    if (more) store(t + 1, buf ^ 1);
+  }
+
+  l += __shfl_xor(l, 32, 64);
+  const int in_tile = 32 * wave + r;
+  if (it.chunks > 1) {
+    float* part = p.part + ((int64_t)hk * p.items + item) * (M * (D + 2));
+#pragma unroll
+    for (int d = 0; d < DVB; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4*>(part + in_tile * D + d * 32 + 8 * g + 4 * hh) =
+            f32x4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+    if (hh == 0) {
+      part[M * D + 2 * in_tile] = m;
+      part[M * D + 2 * in_tile + 1] = l;
+    }
+    return;
+  }
+  const bool live = job.row0 + in_tile < job.rows;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (p.lse && live && hh == 0)
+    p.lse[job.b * p.lse_sb + head * p.lse_sh + job.s.first + tok] =
+        l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+  unsigned short* op = p.o + job.b * p.o_sb + (int64_t)(job.s.first + tok) * p.o_ss + head * p.o_sh;
+#pragma unroll
+  for (int d = 0; d < DVB; ++d) {
+    unsigned pk[4][2];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      pk[g][0] = pack_bf2(o[d][4 * g] * inv, o[d][4 * g + 1] * inv);
+      pk[g][1] = pack_bf2(o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv);
+    }
+#pragma unroll
+    for (int g = 0; g < 4; g += 2) {
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        auto sw = __builtin_amdgcn_permlane32_swap(pk[g][w], pk[g + 1][w], false, false);
+        pk[g][w] = sw[0];
+        pk[g + 1][w] = sw[1];
+      }
+      if (live)
+        *reinterpret_cast<u32x4*>(op + d * 32 + 8 * (g + hh)) = u32x4{pk[g][0], pk[g][1], pk[g + 1][0], pk[g + 1][1]};
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------- joint --
+// The chunks of one row tile: a wave for each row, its lanes over the channels.
+template <int D>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p, int M) {
+  const int item = blockIdx.x / p.Hk, hk = blockIdx.x % p.Hk;
+  const int32_t* info = p.info + 4 * (int64_t)item;
+  const int b = info[0], tile = info[1], chunk = info[2], chunks = info[3];
+  if (chunk != 0 || chunks <= 1) return;  // items behind the last one have no chunks
+  const Seq s = seq_of(p, b);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int in_tile = blockIdx.y * 4 + wave, row = tile * M + in_tile;
+  if (row >= s.n * p.G) return;
+  const int64_t step = (int64_t)M * (D + 2);
+  const float* part = p.part + ((int64_t)hk * p.items + item) * step;
+  float top = M_START;
+  for (int c = lane; c < chunks; c += 64) top = fmaxf(top, part[c * step + M * D + 2 * in_tile]);
+  top = group_max<64>(top);
+  constexpr int PER = D / 64;
+  float acc[PER], l = 0.f;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) acc[j] = 0.f;
+  for (int c = 0; c < chunks; ++c) {
+    const float* at = part + c * step;
+    const float w = __builtin_amdgcn_exp2f(at[M * D + 2 * in_tile] - top);
+    l = fmaf(at[M * D + 2 * in_tile + 1], w, l);
+#pragma unroll
+    for (int j = 0; j < PER; ++j) acc[j] = fmaf(at[in_tile * D + PER * lane + j], w, acc[j]);
+  }
+  const int tok = row / p.G, head = hk * p.G + row - tok * p.G;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  unsigned short* op = p.o + b * p.o_sb + (int64_t)(s.first + tok) * p.o_ss + head * p.o_sh + PER * lane;
+  if constexpr (PER == 2) *reinterpret_cast<unsigned*>(op) = pack_bf2(acc[0] * inv, acc[1] * inv);
+  else *op = f2bf(acc[0] * inv);
+  if (p.lse && lane == 0)
+    p.lse[b * p.lse_sb + head * p.lse_sh + s.first + tok] =
+        l == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+}
+
+// -------------------------------------------------------------------------------------- host --
+int cu_count() {
+  static std::atomic<int> cus{0};
+  int n = cus.load(std::memory_order_relaxed);
+  if (n == 0) {
+    int d = 0;
+    (void)hipGetDevice(&d);
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, d) != hipSuccess || n <= 0) n = 256;
+    cus.store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+struct Plan {
+  int M, few;          // rows of a tile; which kernel
+  int64_t items, target;
+  int chunk_min, split;
+  int64_t part_bytes, info_bytes;
+};
+
+// Which kernel, how many items at most, and whether keys may be split.
+Plan plan_of(const mi355_paged_attn_args* a) {
+  Plan w;
+  const int64_t G = a->H / a->Hk, rows = a->max_seqlen_q * G;
+  const int64_t all_rows = (a->cu_seqlens_q ? a->Sq : a->Sq * a->B) * G;
+  w.few = rows <= 16 ? 1 : rows <= 32 ? 2 : 0;
+  w.M = w.few ? 16 * w.few : 128;
+  const int64_t tiles = all_rows / w.M + a->B;  // row tiles: at most one not full for each sequence
+  // two workgroups of either kernel fit a CU
+  const int64_t want = 2 * (int64_t)cu_count();
+  w.target = (want + a->Hk - 1) / a->Hk;
+  w.chunk_min = w.few ? 4 : 8;
+  const int64_t cap = a->table_width * a->block_size;
+  w.split = cap > (int64_t)w.chunk_min * KT && (all_rows / w.M) * a->Hk < 2 * want;
+  w.items = tiles + (w.split ? w.target : 0);
+  w.part_bytes = w.split ? a->Hk * w.items * w.M * (a->D + 2) * (int64_t)sizeof(float) : 0;
+  w.info_bytes = w.split ? w.items * 4 * (int64_t)sizeof(int32_t) : 0;
+  return w;
+}
+
+int check(const mi355_paged_attn_args* a) {
+  MI355_REQUIRE(a != nullptr, "paged_attn_fp8: null args");
+  MI355_REQUIRE(a->D == 64 || a->D == 128, "paged_attn_fp8: head size %ld not in {64,128}", (long)a->D);
+  MI355_REQUIRE(a->B >= 0 && a->B < (1 << 24) && a->Sq >= 0 && a->Sq < (1ll << 31) && a->H > 0 && a->H < 65536 &&
+                    a->Hk > 0 && a->H % a->Hk == 0 && a->max_seqlen_q >= 0 && a->max_seqlen_q < (1ll << 31),
+                "paged_attn_fp8: bad shape B=%ld Sq=%ld H=%ld Hk=%ld", (long)a->B, (long)a->Sq, (long)a->H,
+                (long)a->Hk);
+  MI355_REQUIRE((a->cu_seqlens_q ? a->Sq : a->Sq * a->B) * (a->H / a->Hk) < (1ll << 31),
+                "paged_attn_fp8: too many rows");
+  MI355_REQUIRE(a->block_size >= 16 && a->block_size <= 1024 && (a->block_size & (a->block_size - 1)) == 0,
+                "paged_attn_fp8: block size %ld must be a power of two in [16, 1024]", (long)a->block_size);
+  MI355_REQUIRE(a->num_blocks >= 0 && a->num_blocks < (1ll << 31) && a->table_width >= 0 &&
+                    a->table_width * a->block_size < (1ll << 31) && (a->B <= 1 || a->table_stride >= a->table_width),
+                "paged_attn_fp8: bad page table");
+  MI355_REQUIRE(a->window_left < 0 || a->causal, "paged_attn_fp8: a window needs causal masking");
+  return MI355_OK;
+}
+
+template <int D>
+int launch(const PagedParams& p, const Plan& w, hipStream_t st) {
+  const dim3 grid((unsigned)(w.items * p.Hk));
+  if (w.few == 1) {
+    hipLaunchKernelGGL((paged_few_rows_kernel<D, 1>), grid, dim3(256), 0, st, p);
+  } else if (w.few == 2) {
+    hipLaunchKernelGGL((paged_few_rows_kernel<D, 2>), grid, dim3(256), 0, st, p);
+  } else {
+    constexpr int LDS = 4 * KT * D * 2;  // two stages of keys and values
+    // the limit of dynamic LDS is an attribute of the function on each device
+    static std::atomic<unsigned long long> known{0};
+    int dev = 0;
+    (void)hipGetDevice(&dev);
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (!(known.load(std::memory_order_acquire) & bit)) {
+      const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(paged_many_rows_kernel<D, 4>),
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+      if (e != hipSuccess) {
+        mi355_set_error("paged_attn_fp8: cannot reserve %d B of LDS: %s", LDS, hipGetErrorString(e));
+        return MI355_EHIP;
+      }
+      known.fetch_or(bit, std::memory_order_release);
+    }
+    hipLaunchKernelGGL((paged_many_rows_kernel<D, 4>), grid, dim3(256), LDS, st, p);
+  }
+  MI355_CHECK_LAUNCH("paged_attn_fp8");
+  if (w.split) {
+    hipLaunchKernelGGL(paged_join_kernel<D>, dim3(grid.x, (unsigned)(w.M / 4)), dim3(256), 0, st, p, w.M);
+    MI355_CHECK_LAUNCH("paged_attn_fp8 (join)");
+  }
+  return MI355_OK;
+}
+
+}  // namespace
+
+extern "C" int64_t mi355_paged_attn_workspace_bytes(const mi355_paged_attn_args* a) {
+  if (check(a) != MI355_OK) return MI355_EINVAL;
+  if (a->B == 0 || a->Sq == 0) return 0;
+  const Plan w = plan_of(a);
+  return w.part_bytes + w.info_bytes;
+}
+
+extern "C" int mi355_paged_attn_fp8(const mi355_paged_attn_args* a, void* stream) {
+  if (int rc = check(a)) return rc;
+  if (a->B == 0 || a->Sq == 0) return MI355_OK;
+  MI355_REQUIRE(a->q && a->out && a->cache_seqlens, "paged_attn_fp8: null pointer");
+  MI355_REQUIRE(a->table_width == 0 || (a->page_table && a->num_blocks > 0 && a->k_cache && a->v_cache &&
+                                        a->k_scale && a->v_scale),
+                "paged_attn_fp8: null pointer or no blocks");
+  const int64_t strides[] = {a->q_sb, a->q_ss, a->q_sh, a->o_sb, a->o_ss, a->o_sh};
+  for (int64_t s : strides)
+    MI355_REQUIRE(s % 8 == 0, "paged_attn_fp8: strides of q and out must be multiples of 8 elements");
+  const int64_t cache_strides[] = {a->kc_sb, a->kc_st, a->kc_sh, a->vc_sb, a->vc_st, a->vc_sh};
+  for (int64_t s : cache_strides)
+    MI355_REQUIRE(s % 16 == 0, "paged_attn_fp8: strides of the caches must be multiples of 16 bytes");
+  MI355_REQUIRE(((uintptr_t)a->q | (uintptr_t)a->out | (uintptr_t)a->k_cache | (uintptr_t)a->v_cache) % 16 == 0,
+                "paged_attn_fp8: q, out and the caches must be 16-byte aligned");
+  const Plan w = plan_of(a);
+  MI355_REQUIRE(w.items * a->Hk < (1ll << 31), "paged_attn_fp8: too many row tiles");
+  MI355_REQUIRE(a->workspace_bytes >= w.part_bytes + w.info_bytes && (!w.split || a->workspace) &&
+                    (uintptr_t)a->workspace % 16 == 0,
+                "paged_attn_fp8: workspace of %ld bytes needed (16-byte aligned), %ld given",
+                (long)(w.part_bytes + w.info_bytes), (long)a->workspace_bytes);
+  PagedParams p;
+  p.q = (const unsigned short*)a->q;
+  p.o = (unsigned short*)a->out;
+  p.lse = a->lse;
+  p.kc = (const unsigned char*)a->k_cache;
+  p.vc = (const unsigned char*)a->v_cache;
+  p.ks = a->k_scale;
+  p.vs = a->v_scale;
+  p.cu = a->cu_seqlens_q;
+  p.lens = a->cache_seqlens;
+  p.table = a->page_table;
+  p.q_sb = a->q_sb; p.q_ss = a->q_ss; p.q_sh = a->q_sh;
+  p.o_sb = a->o_sb; p.o_ss = a->o_ss; p.o_sh = a->o_sh;
+  p.lse_sb = a->lse_sb; p.lse_sh = a->lse_sh;
+  p.kc_sb = a->kc_sb; p.kc_st = a->kc_st; p.kc_sh = a->kc_sh;
+  p.vc_sb = a->vc_sb; p.vc_st = a->vc_st; p.vc_sh = a->vc_sh;
+  p.table_stride = a->table_stride;
+  p.B = (int)a->B;
+  p.Hk = (int)a->Hk;
+  p.G = (int)(a->H / a->Hk);
+  p.Sq = (int)a->Sq;
+  p.cap = (int)(a->table_width * a->block_size);
+  p.num_blocks = (int)a->num_blocks;
+  p.lb = __builtin_ctzll((unsigned long long)a->block_size);
+  p.causal = a->causal != 0;
+  p.window = a->window_left < 0 ? -1 : (int)(a->window_left < (1 << 30) ? a->window_left : (1 << 30));
+  p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
+  p.items = (int)w.items;
+  p.target = (int)w.target;
+  p.chunk_min = w.chunk_min;
+  p.split = w.split;
+  p.part = (float*)a->workspace;
+  p.info = (int32_t*)((char*)a->workspace + w.part_bytes);
+  return a->D == 128 ? launch<128>(p, w, (hipStream_t)stream) : launch<64>(p, w, (hipStream_t)stream);
+}

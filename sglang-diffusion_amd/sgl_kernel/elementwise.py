@@ -46,3 +46,21 @@ def apply_rope_with_cos_sin_cache_inplace(positions: torch.Tensor, query: torch.
 def rotary_embedding(positions: torch.Tensor, query: torch.Tensor, key: Optional[torch.Tensor],
                      head_size: int, cos_sin_cache: torch.Tensor, is_neox: bool = True):
     torch.ops.sgl_kernel.rotary_embedding.default(positions, query, key, head_size, cos_sin_cache, is_neox)
+
+
+def rotary_embedding_scaled(positions: torch.Tensor, query: torch.Tensor, key: Optional[torch.Tensor],
+                            inv_freq: torch.Tensor, attn_factor: float = 1.0, is_neox: bool = True,
+                            query_out: Optional[torch.Tensor] = None,
+                            key_out: Optional[torch.Tensor] = None) -> None:
+    """Rotary positions from frequencies, without a table of cosines: `query` [T, H, D] and `key`
+    [T, Hk, D] bf16 turned by positions[t] * inv_freq[i] (int64, fp64 or fp32; the angle in fp64),
+    cosine and sine times `attn_factor`.  The first 2 * len(inv_freq) elements of a head are turned,
+    in halves (is_neox) or in neighbouring pairs; the others are copied.  In place without
+    `query_out` / `key_out`.  sglang_diffusion_amd.layers.rotary.scaled_inv_freq makes the frequencies
+    of the usual long-context scalings."""
+    if query_out is None:
+        query_out = query
+    if key is not None and key_out is None:
+        key_out = key
+    torch.ops.sgl_kernel.rotary_embedding_scaled.default(positions, query, key, inv_freq, attn_factor, is_neox,
+                                                         query_out, key_out)

@@ -1,5 +1,6 @@
 """`flash_attn_varlen_func` with the reference's signature
-(sgl-kernel/python/sgl_kernel/flash_attn.py:228-311), issuing `torch.ops.sgl_kernel.fwd`."""
+(sgl-kernel/python/sgl_kernel/flash_attn.py:228-311), and `flash_attn_with_kvcache` beside it, issuing
+`torch.ops.sgl_kernel.fwd`."""
 from __future__ import annotations
 
 import torch
@@ -31,4 +32,40 @@ def flash_attn_varlen_func(q, k, v, cu_seqlens_q=None, cu_seqlens_k=None, max_se
         q_descale, k_descale, v_descale, softmax_scale, causal, window_size[0], window_size[1],
         attention_chunk, softcap, is_rotary_interleaved=False, scheduler_metadata=None,
         num_splits=num_splits, pack_gqa=pack_gqa, sm_margin=sm_margin, sinks=sinks)
+    return (out, softmax_lse, *rest) if return_softmax_lse else out
+
+
+def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, qv=None, rotary_cos=None, rotary_sin=None,
+                            cache_seqlens=None, cache_batch_idx=None, cache_leftpad=None, page_table=None,
+                            cu_seqlens_q=None, cu_seqlens_k_new=None, max_seqlen_q=None, rotary_seqlens=None,
+                            q_descale=None, k_descale=None, v_descale=None, softmax_scale=None, causal=False,
+                            window_size=(-1, -1), attention_chunk=None, softcap=0.0, rotary_interleaved=True,
+                            scheduler_metadata=None, num_splits=0, pack_gqa=None, sm_margin=0,
+                            return_softmax_lse=False, sinks=None, score_mod=None, aux_tensors=None, ver=3):
+    """Attention of the newest tokens of each sequence over a paged cache in 8 bits.
+
+    `k_cache`, `v_cache` e4m3 [blocks, block_size, Hk, D] (any strides, D contiguous) with `k_descale`,
+    `v_descale` fp32 [blocks, Hk]: one scale for each block of tokens and head.  `page_table` int32
+    [B, blocks of a sequence], `cache_seqlens` int32 [B] (or one int) counts the new tokens too: they are
+    in the cache already (`store_kv_cache_fp8`).  `q` bf16 [B, S, H, D], or packed [T, H, D] with
+    `cu_seqlens_q`; rows of a packed q behind the last sequence are not written.  New token i of n stands
+    at cache_seqlens - n + i; `causal` hides later keys, `window_size` (w, 0) also those more than w back.
+    A row that sees no key gives 0, and -inf as its log-sum-exp (fp32 [H, T] or [B, H, S]).
+    Everything else of the signature raises RuntimeError instead of being ignored; `num_splits`,
+    `pack_gqa` and `sm_margin` are hints that this kernel does not need."""
+    if score_mod is not None or aux_tensors is not None:
+        raise NotImplementedError("score_mod / aux_tensors are not implemented")
+    if page_table is None:
+        raise RuntimeError("flash_attn_with_kvcache: only paged caches are implemented (page_table)")
+    if k_cache.dtype != torch.float8_e4m3fn:
+        raise RuntimeError("flash_attn_with_kvcache: only float8_e4m3fn caches are implemented")
+    if isinstance(cache_seqlens, int):
+        cache_seqlens = torch.full((page_table.shape[0],), cache_seqlens, dtype=torch.int32, device=q.device)
+    out, softmax_lse, *rest = torch.ops.sgl_kernel.fwd.default(
+        q, k_cache, v_cache, k, v, qv, None, cu_seqlens_q, None, cu_seqlens_k_new, None, cache_seqlens,
+        max_seqlen_q, None, page_table, cache_batch_idx, cache_leftpad, rotary_cos, rotary_sin, rotary_seqlens,
+        q_descale, k_descale, v_descale, softmax_scale, causal, window_size[0], window_size[1],
+        0 if attention_chunk is None else int(attention_chunk), softcap,
+        is_rotary_interleaved=rotary_interleaved, scheduler_metadata=scheduler_metadata, num_splits=num_splits,
+        pack_gqa=pack_gqa, sm_margin=sm_margin, sinks=sinks)
     return (out, softmax_lse, *rest) if return_softmax_lse else out

@@ -75,6 +75,31 @@ class AttnArgs(ctypes.Structure):
     )
 
 
+class KvStoreArgs(ctypes.Structure):
+    _fields_ = (
+        [("k", _ptr), ("v", _ptr)] + [(n, _i64) for n in ("k_st", "k_sh", "v_st", "v_sh")]
+        + [("k_cache", _ptr), ("v_cache", _ptr)]
+        + [(n, _i64) for n in ("kc_sb", "kc_st", "kc_sh", "vc_sb", "vc_st", "vc_sh")]
+        + [("k_scale", _ptr), ("v_scale", _ptr), ("slot_mapping", _ptr)]
+        + [(n, _i64) for n in ("tokens", "Hk", "D", "block_size", "num_blocks")]
+        + [("positions", _ptr), ("inv_freq", _ptr), ("rot_dim", _i64), ("inv_freq_is_f64", _int),
+           ("is_neox", _int), ("attn_factor", _f32), ("Hq", _i64), ("q", _ptr), ("q_out", _ptr)]
+        + [(n, _i64) for n in ("q_st", "q_sh", "qo_st", "qo_sh")]
+    )
+
+
+class PagedAttnArgs(ctypes.Structure):
+    _fields_ = (
+        [(n, _ptr) for n in ("q", "out", "lse", "k_cache", "v_cache", "k_scale", "v_scale", "cu_seqlens_q",
+                             "cache_seqlens", "page_table")]
+        + [(n, _i64) for n in ("B", "Sq", "H", "Hk", "D", "max_seqlen_q", "q_sb", "q_ss", "q_sh", "o_sb", "o_ss",
+                               "o_sh", "lse_sb", "lse_sh", "kc_sb", "kc_st", "kc_sh", "vc_sb", "vc_st", "vc_sh",
+                               "table_stride", "table_width", "num_blocks", "block_size")]
+        + [("softmax_scale", _f32), ("causal", _int), ("window_left", _i64), ("workspace", _ptr),
+           ("workspace_bytes", _i64)]
+    )
+
+
 # every symbol include/mi355_dit.h declares, with its argument types
 SIGNATURES = {
     "mi355_last_error": (ctypes.c_char_p, []),
@@ -143,6 +168,14 @@ SIGNATURES = {
     "mi355_cfg_normalize": (_int, [_ptr, _ptr, _f32, _i64, _ptr, _ptr]),
     "mi355_guidance_rescale": (_int, [_ptr, _ptr, _f32, _i64, _i64, _ptr, _ptr]),
     "mi355_guidance_rescale_static": (_int, [_ptr, _ptr, _f32, _i64, _i64, _ptr]),
+    "mi355_kv_block_plan": (
+        _int,
+        [_ptr, _ptr, _i64, _ptr, _i64, _i64, _ptr, _i64, _ptr, _i64, _i64, _ptr, _ptr, _i64] + [_ptr] * 5,
+    ),
+    "mi355_rope_scaled": (_int, [_ptr] * 5 + [_i64] * 13 + [_ptr, _int, _f32, _int, _ptr]),
+    "mi355_kv_store_fp8": (_int, [ctypes.POINTER(KvStoreArgs), _ptr]),
+    "mi355_paged_attn_workspace_bytes": (_i64, [ctypes.POINTER(PagedAttnArgs)]),
+    "mi355_paged_attn_fp8": (_int, [ctypes.POINTER(PagedAttnArgs), _ptr]),
 }
 
 _lib = None
@@ -749,3 +782,79 @@ def guidance_rescale_static(noise, cond, rescale: float) -> None:
             ),
             "guidance_rescale_static",
         )
+
+
+# ------------------------------------------------------------------- paged 8-bit KV cache --
+def kv_block_plan(context_lens, new_lens, block_table, free_blocks, free_begin, block_size, num_blocks,
+                  slot_mapping, positions, cu_seqlens_q, seq_lens, free_end, status) -> None:
+    B, width = block_table.shape
+    _check(
+        load_library().mi355_kv_block_plan(
+            context_lens.data_ptr(), new_lens.data_ptr(), B, block_table.data_ptr(), block_table.stride(0), width,
+            free_blocks.data_ptr(), free_blocks.numel(), free_begin.data_ptr(), block_size, num_blocks,
+            slot_mapping.data_ptr(), positions.data_ptr(), slot_mapping.numel(), cu_seqlens_q.data_ptr(),
+            seq_lens.data_ptr(), free_end.data_ptr(), status.data_ptr(), _stream(slot_mapping),
+        ),
+        "kv_block_plan",
+    )
+
+
+def rope_scaled(positions, q, k, inv_freq, attn_factor, is_neox, q_out, k_out) -> None:
+    """q [T, Hq, D], k [T, Hk, D] or None (last dim contiguous), written to q_out / k_out."""
+    T, H, D = q.shape
+    ks = (0, 0, 0, 0) if k is None else (k.stride(0), k.stride(1), k_out.stride(0), k_out.stride(1))
+    _check(
+        load_library().mi355_rope_scaled(
+            positions.data_ptr(), q.data_ptr(), q_out.data_ptr(), _p(k), _p(k_out), T, H,
+            0 if k is None else k.shape[1], D, 2 * inv_freq.numel(), q.stride(0), q.stride(1), q_out.stride(0),
+            q_out.stride(1), *ks, inv_freq.data_ptr(), int(inv_freq.dtype == torch.float64), float(attn_factor),
+            int(bool(is_neox)), _stream(q),
+        ),
+        "rope_scaled",
+    )
+
+
+def kv_store_fp8(k, v, k_cache, v_cache, k_scale, v_scale, slot_mapping, q=None, positions=None, inv_freq=None,
+                 attn_factor=1.0, is_neox=True, q_out=None) -> None:
+    """k, v [T, Hk, D] bf16 into caches [blocks, block_size, Hk, D] (e4m3) with scales [blocks, Hk];
+    positions given: keys, and q [T, Hq, D] into q_out, are rotated."""
+    T, Hk, D = k.shape
+    a = KvStoreArgs(
+        k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1), k_cache.data_ptr(),
+        v_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2), v_cache.stride(0),
+        v_cache.stride(1), v_cache.stride(2), k_scale.data_ptr(), v_scale.data_ptr(), slot_mapping.data_ptr(),
+        T, Hk, D, k_cache.shape[1], k_cache.shape[0])
+    if positions is not None:
+        a.positions, a.inv_freq = positions.data_ptr(), inv_freq.data_ptr()
+        a.rot_dim, a.inv_freq_is_f64 = 2 * inv_freq.numel(), inv_freq.dtype == torch.float64
+        a.is_neox, a.attn_factor = bool(is_neox), attn_factor
+    if q is not None:
+        a.Hq, a.q, a.q_out = q.shape[1], q.data_ptr(), q_out.data_ptr()
+        a.q_st, a.q_sh, a.qo_st, a.qo_sh = q.stride(0), q.stride(1), q_out.stride(0), q_out.stride(1)
+    _check(load_library().mi355_kv_store_fp8(ctypes.byref(a), _stream(k)), "kv_store_fp8")
+
+
+def paged_attention_fp8(q, k_cache, v_cache, k_scale, v_scale, page_table, cache_seqlens, cu_seqlens_q,
+                        max_seqlen_q, out, lse, softmax_scale, causal, window_left) -> None:
+    """q, out [T, H, D] with cu_seqlens_q, or [B, Sq, H, D] without; lse [H, T] or [B, H, Sq]
+    (dense fp32) or None.  The workspace comes from the caching allocator, so it belongs to the
+    current stream, or to the graph that is being captured."""
+    packed = q.dim() == 3
+    Sq, H, D = q.shape[-3:]
+    B = cache_seqlens.numel()
+    s, os_ = q.stride(), out.stride()
+    a = PagedAttnArgs(
+        q.data_ptr(), out.data_ptr(), _p(lse), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+        v_scale.data_ptr(), _p(cu_seqlens_q), cache_seqlens.data_ptr(), page_table.data_ptr(), B, Sq, H,
+        k_cache.shape[2], D, max_seqlen_q, 0 if packed else s[0], s[-3], s[-2], 0 if packed else os_[0], os_[-3],
+        os_[-2], 0 if packed else H * Sq, Sq, *k_cache.stride()[:3], *v_cache.stride()[:3], page_table.stride(0),
+        page_table.shape[1], k_cache.shape[0], k_cache.shape[1], softmax_scale, causal, window_left)
+    lib = load_library()
+    stream = _stream(q)
+    need = lib.mi355_paged_attn_workspace_bytes(ctypes.byref(a))
+    if need < 0:
+        _check(need, "paged_attn_fp8")
+    if need:
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), need
+    _check(lib.mi355_paged_attn_fp8(ctypes.byref(a), stream), "paged_attn_fp8")

@@ -7,6 +7,7 @@ rotary_embedding/utils.py:42-121 and runs the fused HIP kernel.
 """
 from __future__ import annotations
 
+import math
 from typing import List, Optional, Tuple
 
 import torch
@@ -82,3 +83,49 @@ def apply_flashinfer_rope_qk_inplace(q: torch.Tensor, k: torch.Tensor,
         q, k = q.contiguous(), k.contiguous()
     _C.qk_norm_rope(q, k, None, None, None, None, 0, 0.0, cos, sin, not is_neox)
     return q, k
+
+
+def scaled_inv_freq(rot_dim: int, base: float = 10000.0, scaling: Optional[dict] = None,
+                    device=None) -> Tuple[torch.Tensor, float]:
+    """Frequencies base^(-2i / rot_dim) in float64, scaled for contexts longer than the trained one,
+    and the factor on cosine and sine that goes with them: the `inv_freq` and `attn_factor` of
+    `sgl_kernel.rotary_embedding_scaled` and `store_kv_cache_fp8`.  `scaling` is the `rope_scaling`
+    entry of a model's config, with its names:
+
+    * {"rope_type": "linear", "factor": f}: all frequencies divided by f.
+    * {"rope_type": "llama3", "factor", "low_freq_factor", "high_freq_factor",
+      "original_max_position_embeddings"}: pairs that turn fewer than low_freq_factor times over the
+      trained length divided by f, those above high_freq_factor kept, the share between
+      interpolated over the number of turns.
+    * {"rope_type": "yarn", "factor", "original_max_position_embeddings", "beta_fast" (32),
+      "beta_slow" (1), "attention_factor"}: a ramp over the pair index between the pairs that turn
+      beta_fast and beta_slow times; attention_factor defaults to 0.1 ln f + 1."""
+    if rot_dim <= 0 or rot_dim % 2:
+        raise ValueError(f"rot_dim must be positive and even, got {rot_dim}")
+    freq = base ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64) / rot_dim)
+    attn_factor = 1.0
+    kind = (scaling or {}).get("rope_type", (scaling or {}).get("type", "default"))
+    if kind == "linear":
+        freq = freq / scaling["factor"]
+    elif kind == "llama3":
+        turns = scaling["original_max_position_embeddings"] * freq / (2 * math.pi)
+        low, high = scaling["low_freq_factor"], scaling["high_freq_factor"]
+        keep = ((turns - low) / (high - low)).clamp(0.0, 1.0)
+        freq = freq * (keep + (1.0 - keep) / scaling["factor"])
+    elif kind == "yarn":
+        trained, factor = scaling["original_max_position_embeddings"], scaling["factor"]
+
+        def pair_that_turns(times):
+            return rot_dim * math.log(trained / (times * 2 * math.pi)) / (2 * math.log(base))
+
+        first = max(math.floor(pair_that_turns(scaling.get("beta_fast") or 32)), 0)
+        last = min(math.ceil(pair_that_turns(scaling.get("beta_slow") or 1)), rot_dim - 1)
+        ramp = (torch.arange(rot_dim // 2, dtype=torch.float64) - first) / (max(last - first, 0.001))
+        keep = 1.0 - ramp.clamp(0.0, 1.0)
+        freq = freq * (keep + (1.0 - keep) / factor)
+        attn_factor = scaling.get("attention_factor")
+        if attn_factor is None:
+            attn_factor = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+    elif kind != "default":
+        raise ValueError(f"unknown rope_type {kind!r}")
+    return freq.to(device), float(attn_factor)
