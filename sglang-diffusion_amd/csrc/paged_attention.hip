@@ -17,6 +17,7 @@
 // sequences, from that takes the length of a chunk that makes about as many items as the chip
 // holds workgroups, and finds its own item.  Chunks of one row tile are joined by a second kernel.
 #include <atomic>
+#include <type_traits>
 
 #include "common.h"
 
@@ -41,7 +42,8 @@ struct PagedParams {
   const float *ks, *vs;
   const int32_t *cu, *lens, *table;
   int64_t q_sb, q_ss, q_sh, o_sb, o_ss, o_sh, lse_sb, lse_sh;
-  int64_t kc_sb, kc_st, kc_sh, vc_sb, vc_st, vc_sh;
+  int64_t kc_sb, kc_sh, vc_sb, vc_sh;
+  int kc_st, vc_st;
   int64_t table_stride;
   int B, Hk, G, Sq;  // Sq: rows of q (packed) or of each sequence (cu == nullptr)
   int cap;           // tokens that a row of the table has room for
@@ -189,30 +191,50 @@ __device__ __forceinline__ Job job_of(const PagedParams& p, const Item& it, int 
   return j;
 }
 
-// A 16-key piece of a tile lies in one block (blocks hold 16 tokens or more).  Pieces behind the
-// end and blocks that are not of the pool are not read: `ok` is false and the block is 0.
-struct Piece {
-  int block, off;
-  bool ok;
+// A tile is four pieces of 16 keys, each inside one block (blocks hold 16 tokens or more).  Table
+// entries are fetched two tiles ahead of the products and scales one, so that neither the entry a
+// block's address hangs on nor the scale its scores need is waited for.
+// What a wave keeps of the tiles ahead of it, piece l & 3 in lane l: a block (0 where there is
+// none), and which of the four pieces there are.  Kept in vector registers and loaded by vector
+// loads: scalar loads return out of order, and waiting for one drains the LDS queue with it.
+struct Ahead {
+  int block;
+  unsigned ok;  // bit c: piece c is there
 };
-__device__ __forceinline__ Piece piece_of(const PagedParams& p, const Job& j, int key) {
-  Piece c;
-  c.ok = key < j.s.len;
-  c.off = key & ((1 << p.lb) - 1);
-  c.block = c.ok ? p.table[j.b * p.table_stride + (key >> p.lb)] : 0;
-  c.ok = c.ok && c.block >= 0 && c.block < p.num_blocks;
-  if (!c.ok) c.block = c.off = 0;
-  return c;
+__device__ __forceinline__ int load_entry(const PagedParams& p, const Job& j, int t) {
+  const int key = min(t * KT + 16 * (int)(threadIdx.x & 3), j.s.len - 1);
+  return p.table[j.b * p.table_stride + (key >> p.lb)];
 }
-
-// scales of a piece: factor of the score, addend of the exponent, weight in the row sum
+__device__ __forceinline__ Ahead resolve(const PagedParams& p, const Job& j, int t, int entry) {
+  const bool ok = (int)(t * KT + 16 * (int)(threadIdx.x & 3) < j.s.len) & (int)(entry >= 0) &
+                  (int)(entry < p.num_blocks);
+  return Ahead{ok ? entry : 0, (unsigned)__builtin_amdgcn_ballot_w64(ok) & 15u};
+}
+// the first byte of a piece (wave-uniform)
+__device__ __forceinline__ const unsigned char* piece_at(const PagedParams& p, const unsigned char* head, int64_t sb,
+                                                         int st, const Ahead& a, int t, int c) {
+  const int block = __builtin_amdgcn_readlane(a.block, c);
+  const int off = (a.ok >> c) & 1 ? (t * KT + 16 * c) & ((1 << p.lb) - 1) : 0;
+  return head + (block * sb + (int64_t)off * st);
+}
+// scales of a tile's pieces: factor of the score, addend of the exponent, weight in the row sum
 struct Scales {
-  float k, v_log, v_inv;
+  float k[4], v_log[4], v_inv[4];
 };
-__device__ __forceinline__ Scales scales_of(const PagedParams& p, const Piece& c, int hk) {
-  const int64_t at = (int64_t)c.block * p.Hk + hk;
-  const float vs = c.ok ? fminf(fmaxf(p.vs[at], 0x1p-64f), 0x1p120f) : 1.f;
-  return Scales{c.ok ? p.ks[at] * p.scale_log2 : 0.f, __builtin_amdgcn_logf(vs), 1.f / vs};
+__device__ __forceinline__ float lane_value(float x, int c) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), c));
+}
+__device__ __forceinline__ Scales scales_of(const PagedParams& p, float ks, float vs) {
+  vs = fminf(fmaxf(vs, 0x1p-64f), 0x1p120f);
+  const float k = ks * p.scale_log2, lg = __builtin_amdgcn_logf(vs), inv = __builtin_amdgcn_rcpf(vs);
+  Scales s;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    s.k[c] = lane_value(k, c);
+    s.v_log[c] = lane_value(lg, c);
+    s.v_inv[c] = lane_value(inv, c);
+  }
+  return s;
 }
 
 // Without branches on purpose: a conditional write into one element of a matrix instruction's
@@ -235,20 +257,21 @@ __device__ __forceinline__ f16x8 widen_f16(unsigned a, unsigned b) {
   const f16x2 x3 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.f, true);
   return f16x8{x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
 }
-// does any of the four e4m3 codes stand for NaN (0x7f, 0xff)?
-__device__ __forceinline__ unsigned nan_codes(unsigned w) {
+// A row must not get a NaN from a value that it does not see, and 0 * NaN is NaN: in tiles that
+// some row sees in part, NaN codes (0x7f, 0xff) go into the product as zeros, and the rows that do
+// see them get theirs afterwards (poison, below), from the cache, where it costs the loop nothing.
+__device__ __forceinline__ unsigned nan_codes(unsigned w) {  // 0x80 in each byte that is one
   return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
 }
-// NaN values replaced by 0, and where they were by 1
-__device__ __forceinline__ f16x8 without_nan(f16x8 v, f16x8* where) {
-  f16x8 o;
+__device__ __forceinline__ unsigned clear_nan(u32x4& v) {
+  unsigned any = 0;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const bool n = v[j] != v[j];
-    o[j] = n ? (_Float16)0.f : v[j];
-    (*where)[j] = n ? (_Float16)1.f : (_Float16)0.f;
+  for (int j = 0; j < 4; ++j) {
+    const unsigned n = nan_codes(v[j]);
+    any |= n;
+    v[j] &= ~((n >> 7) * 0xffu);
   }
-  return o;
+  return any;
 }
 
 // ----------------------------------------------------------------- few rows: 16 or 32 of them --
@@ -299,22 +322,24 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
   }
 
   u32x4 kr[4][NH], vr[CPR];
-  auto load_k = [&](const Piece (&pc)[4]) {
+  const unsigned char *k_head = p.kc + hk * p.kc_sh, *v_head = p.vc + hk * p.vc_sh;
+  const unsigned k_lane = (unsigned)(r * p.kc_st + 16 * g);
+  const unsigned v_lane = (unsigned)((lane / CPR) * p.vc_st + (lane % CPR) * 16);
+  auto load_k = [&](const Ahead& a, int t) {
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const unsigned char* at = p.kc + pc[c].block * p.kc_sb + (int64_t)pc[c].off * p.kc_st + hk * p.kc_sh +
-                                (int64_t)r * p.kc_st + 16 * g;
+      const unsigned char* at = piece_at(p, k_head, p.kc_sb, p.kc_st, a, t, c);
 #pragma unroll
-      for (int h = 0; h < NH; ++h) kr[c][h] = *reinterpret_cast<const u32x4*>(at + 64 * h);
+      for (int h = 0; h < NH; ++h) kr[c][h] = *reinterpret_cast<const u32x4*>(at + (k_lane + 64 * h));
     }
   };
-  auto load_v = [&](const Piece (&pc)[4]) {
+  auto load_v = [&](const Ahead& a, int t) {
 #pragma unroll
-    for (int i = 0; i < CPR; ++i) {
-      const int row = (i * 64 + lane) / CPR;
-      const Piece c = pc[i * 4 / CPR];
-      vr[i] = *reinterpret_cast<const u32x4*>(p.vc + c.block * p.vc_sb + (int64_t)(c.off + (row & 15)) * p.vc_st +
-                                              hk * p.vc_sh + (lane % CPR) * 16);
+    for (int c = 0; c < 4; ++c) {
+      const unsigned char* at = piece_at(p, v_head, p.vc_sb, p.vc_st, a, t, c);
+#pragma unroll
+      for (int i = 0; i < CPR / 4; ++i)  // 64 / CPR rows at a time
+        vr[c * CPR / 4 + i] = *reinterpret_cast<const u32x4*>(at + (v_lane + (unsigned)(i * (64 / CPR) * p.vc_st)));
     }
   };
   auto swz = [](int row) { return D == 128 ? (row >> 1) & 7 : (row >> 2) & 3; };
@@ -322,43 +347,38 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
   const int tr_row = (r >> 1) < 4 ? 4 * g + (r >> 1) : 12 + 4 * g + (r >> 1);
   const int tr_swz = swz(tr_row);
   const unsigned char* tr_at = img + tr_row * D + (r & 1) * 8;
+  // does some row of the tile not see some key of it?
+  auto in_part = [&](int t, unsigned ok) {
+    return t * KT + KT > job.s.len || ok != 15u || (p.causal && t * KT + KT - 1 > job.place_lo) ||
+           (p.window >= 0 && t * KT < job.place_hi - p.window);
+  };
 
-  Piece pc[4], nx[4];
+  bool nan_values = false;
   int t = job.t0 + wave;
+  Ahead now{0, 0}, next{0, 0};
+  Scales sc{};
   if (t < job.t1) {
-#pragma unroll
-    for (int c = 0; c < 4; ++c) pc[c] = piece_of(p, job, t * KT + 16 * c);
-    load_k(pc);
-    load_v(pc);
+    now = resolve(p, job, t, load_entry(p, job, t));
+    load_k(now, t);
+    load_v(now, t);
+    next = resolve(p, job, t + 4, load_entry(p, job, t + 4));
+    const int64_t at = (int64_t)now.block * p.Hk + hk;
+    sc = scales_of(p, p.ks[at], p.vs[at]);
   }
   for (; t < job.t1; t += 4) {
     const bool more = t + 4 < job.t1;
-    if (more) {
-#pragma unroll
-      for (int c = 0; c < 4; ++c) nx[c] = piece_of(p, job, (t + 4) * KT + 16 * c);
-    }
-    Scales sc[4];
-#pragma unroll
-    for (int c = 0; c < 4; ++c) sc[c] = scales_of(p, pc[c], hk);
     const int key0 = t * KT;
-    const bool whole = key0 + KT <= job.s.len && pc[0].ok && pc[1].ok && pc[2].ok && pc[3].ok;
-    const bool masked = !whole || (p.causal && key0 + KT - 1 > job.place_lo) ||
-                        (p.window >= 0 && key0 < job.place_hi - p.window);
-    // values into the image; rows that are no keys of the sequence as zeros (0 * NaN is NaN)
-    bool nan_values = false;
-    if (!whole) {
-#pragma unroll
-      for (int i = 0; i < CPR; ++i) {
-        const int key = key0 + (i * 64 + lane) / CPR;
-        if (!pc[i * 4 / CPR].ok || key >= job.s.len) vr[i] = u32x4{0, 0, 0, 0};
-      }
-    }
+    const bool masked = in_part(t, now.ok);
+    // values into the image
     if (masked) {
       unsigned any = 0;
 #pragma unroll
-      for (int i = 0; i < CPR; ++i)
-        any |= nan_codes(vr[i][0]) | nan_codes(vr[i][1]) | nan_codes(vr[i][2]) | nan_codes(vr[i][3]);
-      nan_values = __builtin_amdgcn_ballot_w64(any != 0) != 0;
+      for (int i = 0; i < CPR; ++i) {
+        const int row = (i * 64 + lane) / CPR;
+        if (!((now.ok >> (row >> 4)) & 1) || key0 + row >= job.s.len) vr[i] = u32x4{0, 0, 0, 0};
+        any |= clear_nan(vr[i]);
+      }
+      nan_values |= __builtin_amdgcn_ballot_w64(any != 0) != 0;
     }
 #pragma unroll
     for (int i = 0; i < CPR; ++i) {
@@ -367,7 +387,11 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    if (more) load_v(nx);
+    // entries of the tile after the next, values and scales of the next
+    const int entry = load_entry(p, job, t + 8);
+    const int64_t scale_at = (int64_t)next.block * p.Hk + hk;
+    const float ks = p.ks[scale_at], vs = p.vs[scale_at];
+    if (more) load_v(next, t + 4);
 
     f32x4 s[RT][4];
 #pragma unroll
@@ -384,111 +408,96 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
             s[rt][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[rt][h][u], s[rt][c], 0, 0, 0);
         }
     }
-    if (more) load_k(nx);
+    if (more) load_k(next, t + 4);
 
-    f16x8 pf[RT][2], seen[RT][2];
+    f16x8 pf[RT][2];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       // exponents, then exponentials against the reference as it stands; it moves, and O and l
       // with it, only where a lane's sum says that it has to
+      float x[4][4], e[4][4], sum[4], all;
 #pragma unroll
       for (int c = 0; c < 4; ++c)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[rt][c][i] = fmaf(s[rt][c][i], sc[c].k, sc[c].v_log);
+        for (int i = 0; i < 4; ++i) x[c][i] = fmaf(s[rt][c][i], sc.k[c], sc.v_log[c]);
       if (masked) {
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            s[rt][c][i] = sees(pc[c].ok, key0 + 16 * c + 4 * g + i, see_lo[rt], see_hi[rt]) ? s[rt][c][i] : -INFINITY;
+            x[c][i] = sees((now.ok >> c) & 1, key0 + 16 * c + 4 * g + i, see_lo[rt], see_hi[rt]) ? x[c][i] : -INFINITY;
       }
-      f32x4 e[4];
-      float sum[4], all;
       auto exponentials = [&]() {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) e[c][i] = __builtin_amdgcn_exp2f(s[rt][c][i] - m[rt]);
+          for (int i = 0; i < 4; ++i) e[c][i] = __builtin_amdgcn_exp2f(x[c][i] - m[rt]);
           sum[c] = (e[c][0] + e[c][1]) + (e[c][2] + e[c][3]);
         }
         all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
       };
       exponentials();
       if (__builtin_amdgcn_ballot_w64(!(all <= LAZY_SUM)) != 0) {
-        float top = s[rt][0][0];
+        float top = x[0][0];
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) top = fmaxf(top, s[rt][c][i]);
+          for (int i = 0; i < 4; ++i) top = fmaxf(top, x[c][i]);
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const float now = fmaxf(m[rt], top), shrink = __builtin_amdgcn_exp2f(m[rt] - now);
-        m[rt] = now;
+        const float higher = fmaxf(m[rt], top), shrink = __builtin_amdgcn_exp2f(m[rt] - higher);
+        m[rt] = higher;
         l[rt] *= shrink;
 #pragma unroll
         for (int d = 0; d < DB; ++d) o[rt][d] *= shrink;
         exponentials();
       }
 #pragma unroll
-      for (int c = 0; c < 4; ++c) l[rt] = fmaf(sum[c], sc[c].v_inv, l[rt]);
+      for (int c = 0; c < 4; ++c) l[rt] = fmaf(sum[c], sc.v_inv[c], l[rt]);
 #pragma unroll
       for (int c = 0; c < 4; ++c)
 #pragma unroll
         for (int i = 0; i < 4; ++i) pf[rt][c >> 1][4 * (c & 1) + i] = (_Float16)e[c][i];
-      if (nan_values) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            seen[rt][c >> 1][4 * (c & 1) + i] =
-                sees(pc[c].ok, key0 + 16 * c + 4 * g + i, see_lo[rt], see_hi[rt]) ? (_Float16)1.f : (_Float16)0.f;
-      }
     }
-    auto values = [&](int st, int d) {
-      const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-          (__attribute__((address_space(3))) i32x2*)(tr_at + st * 32 * D + ((d ^ tr_swz) << 4)));
-      return widen_f16((unsigned)w[0], (unsigned)w[1]);
-    };
-    if (!nan_values) {
 #pragma unroll
-      for (int d = 0; d < DB; ++d)
+    for (int d = 0; d < DB; ++d)
 #pragma unroll
-        for (int st = 0; st < 2; ++st) {
-          const f16x8 vf = values(st, d);
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt)
-            o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[rt][st], o[rt][d], 0, 0, 0);
-        }
-    } else {
-      // A tile that some row sees in part, with NaN among its values: a row must not get one from
-      // a key that it does not see.  The product runs without them, and a second one counts, for
-      // each row and channel, the NaN that the row does see.
-#pragma unroll
-      for (int d = 0; d < DB; ++d) {
-        f32x4 count[RT];
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) count[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int st = 0; st < 2; ++st) {
-          f16x8 where;
-          const f16x8 vf = without_nan(values(st, d), &where);
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) {
-            o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[rt][st], o[rt][d], 0, 0, 0);
-            count[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(where, seen[rt][st], count[rt], 0, 0, 0);
-          }
-        }
+      for (int st = 0; st < 2; ++st) {
+        const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+            (__attribute__((address_space(3))) i32x2*)(tr_at + st * 32 * D + ((d ^ tr_swz) << 4)));
+        const f16x8 vf = widen_f16((unsigned)w[0], (unsigned)w[1]);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (count[rt][i] > 0.f) o[rt][d][i] = __builtin_nanf("");
+          o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[rt][st], o[rt][d], 0, 0, 0);
       }
-    }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
+    if (more) {
+      now = next;
+      next = resolve(p, job, t + 8, entry);
+      sc = scales_of(p, ks, vs);
+    }
+  }
+  if (nan_values) {  // poison: the NaN among the values of tiles seen in part, for the rows that see them
+    for (t = job.t0 + wave; t < job.t1; t += 4) {
+      now = resolve(p, job, t, load_entry(p, job, t));
+      if (!in_part(t, now.ok)) continue;
+      for (int k = 0; k < KT; ++k) {
+        const int key = t * KT + k;
+        if (!((now.ok >> (k >> 4)) & 1) || key >= job.s.len) continue;
+        const unsigned char* at = piece_at(p, v_head, p.vc_sb, p.vc_st, now, t, k >> 4) + (k & 15) * p.vc_st;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) pc[c] = nx[c];
+        for (int d = 0; d < DB; ++d) {
+          const unsigned n = nan_codes(*reinterpret_cast<const unsigned*>(at + 16 * d + 4 * g));
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              o[rt][d][i] = ((n >> (8 * i + 7)) & (unsigned)sees(true, key, see_lo[rt], see_hi[rt])) ? __builtin_nanf("")
+                                                                                                  : o[rt][d][i];
+        }
+      }
+    }
   }
 
   // ---- the four waves' parts of each row, joined ----
@@ -562,7 +571,7 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedP
   constexpr int TILE = KT * ROWB, LOADS = KT * D / 16 / (NW * 64);
   static_assert(LOADS >= 1, "every thread loads");
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  __shared__ int nan_flag[2];
+  __shared__ int nan_values;
   const int item = blockIdx.x / p.Hk, hk = blockIdx.x % p.Hk;
   Item it;
   if (!find_item<M>(p, item, hk == 0, &it)) return;
@@ -587,34 +596,46 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedP
   }
 
   u32x4 kr[LOADS], vr[LOADS];
-  // thread's 16 bytes of a tile: row (i * threads + tid) / (D / 16), all of a wave in one piece
-  auto load = [&](int t) {
+  const unsigned char *k_head = p.kc + hk * p.kc_sh, *v_head = p.vc + hk * p.vc_sh;
+  // thread's 16 bytes of a tile: key (i * threads + tid) / (D / 16), all keys of a wave in one piece
+  const int my_c = tid % (D / 16), my_key = tid / (D / 16);
+  auto load = [&](const Ahead& a, int t) {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int key = (i * NW * 64 + tid) / (D / 16), c = tid % (D / 16);
-      const int piece = __builtin_amdgcn_readfirstlane(key >> 4);
-      const Piece pc = piece_of(p, job, t * KT + 16 * piece);
-      const int64_t off = pc.off + (key & 15);
-      kr[i] = *reinterpret_cast<const u32x4*>(p.kc + pc.block * p.kc_sb + off * p.kc_st + hk * p.kc_sh + 16 * c);
-      vr[i] = *reinterpret_cast<const u32x4*>(p.vc + pc.block * p.vc_sb + off * p.vc_st + hk * p.vc_sh + 16 * c);
-      if (!pc.ok || t * KT + key >= job.s.len) vr[i] = u32x4{0, 0, 0, 0};
+      const int key = i * (NW * 64 * 16 / D) + my_key, c = __builtin_amdgcn_readfirstlane(key >> 4);
+      kr[i] = *reinterpret_cast<const u32x4*>(piece_at(p, k_head, p.kc_sb, p.kc_st, a, t, c) +
+                                              (unsigned)((key & 15) * p.kc_st + 16 * my_c));
+      vr[i] = *reinterpret_cast<const u32x4*>(piece_at(p, v_head, p.vc_sb, p.vc_st, a, t, c) +
+                                              (unsigned)((key & 15) * p.vc_st + 16 * my_c));
     }
   };
-  auto store = [&](int t, int buf) {
-    unsigned any = 0;
+  // does some row of the workgroup not see some key of the tile?
+  auto in_part = [&](int t, unsigned ok) {
+    return t * KT + KT > job.s.len || ok != 15u || (p.causal && t * KT + KT - 1 > job.place_lo) ||
+           (p.window >= 0 && t * KT < job.place_hi - p.window);
+  };
+  auto store = [&](const Ahead& a, int t, int buf) {
+    if (in_part(t, a.ok)) {
+      unsigned any = 0;
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int key = i * (NW * 64 * 16 / D) + my_key;
+        if (!((a.ok >> (key >> 4)) & 1) || t * KT + key >= job.s.len) vr[i] = u32x4{0, 0, 0, 0};
+        any |= clear_nan(vr[i]);
+      }
+      if (any) nan_values = 1;
+    }
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int key = (i * NW * 64 + tid) / (D / 16), c = tid % (D / 16);
+      const int key = i * (NW * 64 * 16 / D) + my_key;
       unsigned char* kt = smem + buf * 2 * TILE + key * ROWB;
       unsigned char* vt = kt + TILE;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        *reinterpret_cast<bf16x8*>(kt + (((2 * c + h) ^ k_swz(key)) << 4)) = widen_bf16(kr[i][2 * h], kr[i][2 * h + 1]);
-        *reinterpret_cast<f16x8*>(vt + (((2 * c + h) ^ v_swz(key)) << 4)) = widen_f16(vr[i][2 * h], vr[i][2 * h + 1]);
+        *reinterpret_cast<bf16x8*>(kt + (((2 * my_c + h) ^ k_swz(key)) << 4)) = widen_bf16(kr[i][2 * h], kr[i][2 * h + 1]);
+        *reinterpret_cast<f16x8*>(vt + (((2 * my_c + h) ^ v_swz(key)) << 4)) = widen_f16(vr[i][2 * h], vr[i][2 * h + 1]);
       }
-      any |= nan_codes(vr[i][0]) | nan_codes(vr[i][1]) | nan_codes(vr[i][2]) | nan_codes(vr[i][3]);
     }
-    if (any) nan_flag[buf] = t + 1;  // this tile's mark: never one left by an earlier tile
   };
 
   int koff[KSTEPS];
@@ -637,65 +658,74 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedP
     for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
   float m = M_START, l = 0.f;
 
-  if (tid < 2) nan_flag[tid] = 0;
+  if (tid == 0) nan_values = 0;
   __syncthreads();
+  Ahead now{0, 0}, next{0, 0};
+  Scales sc{};
   if (job.t0 < job.t1) {
-    load(job.t0);
-    store(job.t0, 0);
+    now = resolve(p, job, job.t0, load_entry(p, job, job.t0));
+    load(now, job.t0);
+    next = resolve(p, job, job.t0 + 1, load_entry(p, job, job.t0 + 1));
+    const int64_t at = (int64_t)now.block * p.Hk + hk;
+    sc = scales_of(p, p.ks[at], p.vs[at]);
+    store(now, job.t0, 0);
   }
-  for (int t = job.t0; t < job.t1; ++t) {
-    const int buf = (t - job.t0) & 1, key0 = t * KT;
+  const bool live_wave = job.row0 + 32 * wave < job.rows;
+  auto tile = [&](auto bufc, int t) {
+    constexpr int buf = decltype(bufc)::value;
+    const int key0 = t * KT;
     __syncthreads();
     const bool more = t + 1 < job.t1;
-    if (more) load(t + 1);
-    if (!(p.causal && key0 > w_hi) && !(p.window >= 0 && key0 + KT - 1 < w_lo - p.window)) {
-      Piece pc[4];
-      Scales sc[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        pc[c] = piece_of(p, job, key0 + 16 * c);
-        sc[c] = scales_of(p, pc[c], hk);
-      }
-      const bool masked = key0 + KT > job.s.len || !(pc[0].ok && pc[1].ok && pc[2].ok && pc[3].ok) ||
-                          (p.causal && key0 + KT - 1 > w_lo) || (p.window >= 0 && key0 < w_hi - p.window);
+    // entries of the tile after the next, keys, values and scales of the next
+    const int entry = load_entry(p, job, t + 2);
+    const int64_t scale_at = (int64_t)next.block * p.Hk + hk;
+    const float ks = p.ks[scale_at], vs = p.vs[scale_at];
+    if (more) load(next, t + 1);
+    if (live_wave && !(p.causal && key0 > w_hi) && !(p.window >= 0 && key0 + KT - 1 < w_lo - p.window)) {
       const unsigned char *kt = smem + buf * 2 * TILE, *vt = kt + TILE;
       f32x16 s[2];
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[kb][e] = 0.f;
+      bf16x8 kf[2][2];
 #pragma unroll
-      for (int st = 0; st < KSTEPS; ++st)
+      for (int kb = 0; kb < 2; ++kb) kf[0][kb] = *reinterpret_cast<const bf16x8*>(kt + kb * 32 * ROWB + koff[0]);
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          const bf16x8 kf = *reinterpret_cast<const bf16x8*>(kt + kb * 32 * ROWB + koff[st]);
-          s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[st], s[kb], 0, 0, 0);
+      for (int st = 0; st < KSTEPS; ++st) {
+        if (st + 1 < KSTEPS) {
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+            kf[(st + 1) & 1][kb] = *reinterpret_cast<const bf16x8*>(kt + kb * 32 * ROWB + koff[st + 1]);
         }
-      auto visible = [&](int kb, int e) {
-        return sees(pc[2 * kb + (e >> 3)].ok, key0 + kb * 32 + (e & 3) + 8 * (e >> 2) + 4 * hh, see_lo, see_hi);
-      };
+        __builtin_amdgcn_sched_barrier(0);  // the reads of a step stay ahead of the products before it
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+          s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[st & 1][kb], qf[st], s[kb], 0, 0, 0);
+      }
+      const bool masked = key0 + KT > job.s.len || now.ok != 15u || (p.causal && key0 + KT - 1 > w_lo) ||
+                          (p.window >= 0 && key0 < w_hi - p.window);
+      float x[2][16], sum[4], all;
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const Scales& c = sc[2 * kb + (e >> 3)];
-          s[kb][e] = fmaf(s[kb][e], c.k, c.v_log);
-        }
+        for (int e = 0; e < 16; ++e) x[kb][e] = fmaf(s[kb][e], sc.k[2 * kb + (e >> 3)], sc.v_log[2 * kb + (e >> 3)]);
       if (masked) {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            s[kb][e] = visible(kb, e) ? s[kb][e] : -INFINITY;
+            x[kb][e] = sees((now.ok >> (2 * kb + (e >> 3))) & 1, key0 + kb * 32 + (e & 3) + 8 * (e >> 2) + 4 * hh,
+                            see_lo, see_hi) ? x[kb][e] : -INFINITY;
       }
-      float pe[2][16], sum[4], all;
+      float pe[2][16];
       auto exponentials = [&]() {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           sum[c] = 0.f;
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            pe[c >> 1][8 * (c & 1) + e] = __builtin_amdgcn_exp2f(s[c >> 1][8 * (c & 1) + e] - m);
+            pe[c >> 1][8 * (c & 1) + e] = __builtin_amdgcn_exp2f(x[c >> 1][8 * (c & 1) + e] - m);
             sum[c] += pe[c >> 1][8 * (c & 1) + e];
           }
         }
@@ -703,14 +733,14 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedP
       };
       exponentials();
       if (__builtin_amdgcn_ballot_w64(!(all <= LAZY_SUM)) != 0) {
-        float top = s[0][0];
+        float top = x[0][0];
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) top = fmaxf(top, s[kb][e]);
+          for (int e = 0; e < 16; ++e) top = fmaxf(top, x[kb][e]);
         top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const float now = fmaxf(m, top), shrink = __builtin_amdgcn_exp2f(m - now);
-        m = now;
+        const float higher = fmaxf(m, top), shrink = __builtin_amdgcn_exp2f(m - higher);
+        m = higher;
         l *= shrink;
 #pragma unroll
         for (int d = 0; d < DVB; ++d)
@@ -719,7 +749,7 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedP
         exponentials();
       }
 #pragma unroll
-      for (int c = 0; c < 4; ++c) l = fmaf(sum[c], sc[c].v_inv, l);
+      for (int c = 0; c < 4; ++c) l = fmaf(sum[c], sc.v_inv[c], l);
       f16x8 pf[2][2];
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
@@ -727,52 +757,52 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedP
         for (int st = 0; st < 2; ++st)
 #pragma unroll
           for (int j = 0; j < 8; ++j) pf[kb][st][j] = (_Float16)pe[kb][8 * st + j];
-      auto values = [&](int kb, int st, int d) {
-        const unsigned char* at = vt + (kb * 32 + st * 16) * ROWB;
-        const f16x4 a = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16(
-            (__attribute__((address_space(3))) hw_f16x4*)(at + vlane[d][0])));
-        const f16x4 b = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16(
-            (__attribute__((address_space(3))) hw_f16x4*)(at + vlane[d][1])));
-        return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-      };
-      if (!masked || nan_flag[buf] != t + 1) {
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+      for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-          for (int st = 0; st < 2; ++st)
+        for (int st = 0; st < 2; ++st)
 #pragma unroll
-            for (int d = 0; d < DVB; ++d)
-              o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(values(kb, st, d), pf[kb][st], o[d], 0, 0, 0);
-      } else {  // as in the kernel above
-        f16x8 seen[2][2];
+          for (int d = 0; d < DVB; ++d) {
+            const unsigned char* at = vt + (kb * 32 + st * 16) * ROWB;
+            const f16x4 a = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16(
+                (__attribute__((address_space(3))) hw_f16x4*)(at + vlane[d][0])));
+            const f16x4 b = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16(
+                (__attribute__((address_space(3))) hw_f16x4*)(at + vlane[d][1])));
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7),
+                                                          pf[kb][st], o[d], 0, 0, 0);
+          }
+    }
+    if (more) {
+      store(next, t + 1, buf ^ 1);
+      now = next;
+      next = resolve(p, job, t + 2, entry);
+      sc = scales_of(p, ks, vs);
+    }
+  };
+  for (int t = job.t0; t < job.t1; t += 2) {
+    tile(std::integral_constant<int, 0>{}, t);
+    if (t + 1 < job.t1) tile(std::integral_constant<int, 1>{}, t + 1);
+  }
+  __syncthreads();
+  if (nan_values) {  // poison, as above
+    for (int t = job.t0; t < job.t1; ++t) {
+      now = resolve(p, job, t, load_entry(p, job, t));
+      if (!in_part(t, now.ok)) continue;
+      for (int k = 0; k < KT; ++k) {
+        const int key = t * KT + k;
+        if (!((now.ok >> (k >> 4)) & 1) || key >= job.s.len) continue;
+        const unsigned char* at = piece_at(p, v_head, p.vc_sb, p.vc_st, now, t, k >> 4) + (k & 15) * p.vc_st + 4 * hh;
+        const unsigned seen = (unsigned)sees(true, key, see_lo, see_hi);
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int d = 0; d < DVB; ++d)
 #pragma unroll
-          for (int st = 0; st < 2; ++st)
+          for (int g = 0; g < 4; ++g) {
+            const unsigned n = nan_codes(*reinterpret_cast<const unsigned*>(at + 32 * d + 8 * g));
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              seen[kb][st][j] = visible(kb, 8 * st + j) ? (_Float16)1.f : (_Float16)0.f;
-#pragma unroll
-        for (int d = 0; d < DVB; ++d) {
-          f32x16 count;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) count[e] = 0.f;
-#pragma unroll
-          for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-            for (int st = 0; st < 2; ++st) {
-              f16x8 where;
-              const f16x8 vf = without_nan(values(kb, st, d), &where);
-              o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[kb][st], o[d], 0, 0, 0);
-              count = __builtin_amdgcn_mfma_f32_32x32x16_f16(where, seen[kb][st], count, 0, 0, 0);
-            }
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (count[e] > 0.f) o[d][e] = __builtin_nanf("");
-        }
+            for (int i = 0; i < 4; ++i) o[d][4 * g + i] = ((n >> (8 * i + 7)) & seen) ? __builtin_nanf("") : o[d][4 * g + i];
+          }
       }
     }
-    if (more) store(t + 1, buf ^ 1);
   }
 
   l += __shfl_xor(l, 32, 64);
@@ -909,7 +939,7 @@ int check(const mi355_paged_attn_args* a) {
   MI355_REQUIRE(a->block_size >= 16 && a->block_size <= 1024 && (a->block_size & (a->block_size - 1)) == 0,
                 "paged_attn_fp8: block size %ld must be a power of two in [16, 1024]", (long)a->block_size);
   MI355_REQUIRE(a->num_blocks >= 0 && a->num_blocks < (1ll << 31) && a->table_width >= 0 &&
-                    a->table_width * a->block_size < (1ll << 31) && (a->B <= 1 || a->table_stride >= a->table_width),
+                    a->table_width * a->block_size <= (1ll << 31) - 4096 && (a->B <= 1 || a->table_stride >= a->table_width),
                 "paged_attn_fp8: bad page table");
   MI355_REQUIRE(a->window_left < 0 || a->causal, "paged_attn_fp8: a window needs causal masking");
   return MI355_OK;
@@ -970,6 +1000,8 @@ extern "C" int mi355_paged_attn_fp8(const mi355_paged_attn_args* a, void* stream
   const int64_t cache_strides[] = {a->kc_sb, a->kc_st, a->kc_sh, a->vc_sb, a->vc_st, a->vc_sh};
   for (int64_t s : cache_strides)
     MI355_REQUIRE(s % 16 == 0, "paged_attn_fp8: strides of the caches must be multiples of 16 bytes");
+  MI355_REQUIRE(a->kc_st >= 0 && a->kc_st < (1 << 24) && a->vc_st >= 0 && a->vc_st < (1 << 24),
+                "paged_attn_fp8: token stride of a cache too large");
   MI355_REQUIRE(((uintptr_t)a->q | (uintptr_t)a->out | (uintptr_t)a->k_cache | (uintptr_t)a->v_cache) % 16 == 0,
                 "paged_attn_fp8: q, out and the caches must be 16-byte aligned");
   const Plan w = plan_of(a);
@@ -992,8 +1024,8 @@ extern "C" int mi355_paged_attn_fp8(const mi355_paged_attn_args* a, void* stream
   p.q_sb = a->q_sb; p.q_ss = a->q_ss; p.q_sh = a->q_sh;
   p.o_sb = a->o_sb; p.o_ss = a->o_ss; p.o_sh = a->o_sh;
   p.lse_sb = a->lse_sb; p.lse_sh = a->lse_sh;
-  p.kc_sb = a->kc_sb; p.kc_st = a->kc_st; p.kc_sh = a->kc_sh;
-  p.vc_sb = a->vc_sb; p.vc_st = a->vc_st; p.vc_sh = a->vc_sh;
+  p.kc_sb = a->kc_sb; p.kc_st = (int)a->kc_st; p.kc_sh = a->kc_sh;
+  p.vc_sb = a->vc_sb; p.vc_st = (int)a->vc_st; p.vc_sh = a->vc_sh;
   p.table_stride = a->table_stride;
   p.B = (int)a->B;
   p.Hk = (int)a->Hk;

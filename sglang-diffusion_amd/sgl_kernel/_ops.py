@@ -247,8 +247,9 @@ def _fwd(q, k, v, k_new, v_new, q_v, out, cu_seqlens_q, cu_seqlens_k, cu_seqlens
                      cu_seqlens_k_new=cu_seqlens_k_new, seqused_q=seqused_q, kv_batch_idx=kv_batch_idx,
                      leftpad_k=leftpad_k, rotary_cos=rotary_cos, rotary_sin=rotary_sin,
                      seqlens_rotary=seqlens_rotary, q_descale=q_descale, sinks=sinks)
-        bad = [n for n, t in other.items() if t is not None]
-        _require(not bad, f"fwd: arguments not supported with a paged 8-bit cache: {bad}")
+        if any(t is not None for t in other.values()):
+            _fail("fwd: arguments not supported with a paged 8-bit cache: "
+                  f"{[n for n, t in other.items() if t is not None]}")
         _require(attention_chunk == 0 and softcap == 0.0, "fwd: attention_chunk / softcap are not implemented")
         return _fwd_paged(q, k, v, out, cu_seqlens_q, seqused_k, max_seqlen_q, page_table, k_descale, v_descale,
                           softmax_scale, is_causal, window_left, window_right)
@@ -305,98 +306,116 @@ def _fwd(q, k, v, k_new, v_new, q_v, out, cu_seqlens_q, cu_seqlens_k, cu_seqlens
     return out, lse, empty, empty
 
 
+# The checks of the operators around the paged cache run at every step of a serving loop, whose
+# kernels take a few microseconds: messages are only formed when something is wrong.
+def _fail(msg):
+    raise RuntimeError(msg)
+
+
 def _check_cache(what, cache, scale, name, like):
-    _require(cache.dim() == 4 and cache.dtype == FP8 and cache.stride(3) == 1,
-             f"{what}: {name}_cache must be [blocks, block_size, heads, head_size] float8_e4m3fn with a "
-             "contiguous last dimension")
-    _require(scale is not None and scale.dtype == torch.float32 and scale.is_contiguous()
-             and scale.shape == (cache.shape[0], cache.shape[2]),
-             f"{what}: the scales of {name}_cache must be contiguous float32 [blocks, heads]")
-    _require(cache.device == like.device and scale.device == like.device,
-             f"{what}: all tensors must be on {like.device}")
+    if not (cache.dtype == FP8 and cache.dim() == 4 and cache.stride(3) == 1):
+        _fail(f"{what}: {name}_cache must be [blocks, block_size, heads, head_size] float8_e4m3fn with a "
+              "contiguous last dimension")
+    if not (scale is not None and scale.dtype == torch.float32 and scale.is_contiguous()
+            and scale.shape == (cache.shape[0], cache.shape[2])):
+        _fail(f"{what}: the scales of {name}_cache must be contiguous float32 [blocks, heads]")
+    if not cache.get_device() == scale.get_device() == like.get_device():
+        _fail(f"{what}: all tensors must be on {like.device}")
 
 
 def _check_ints(what, like, dtype, **tensors):
+    device = like.get_device()
     for name, t in tensors.items():
-        _require(t.dtype == dtype and t.dim() == 1 and t.is_contiguous(),
-                 f"{what}: {name} must be a contiguous 1-D {str(dtype)[6:]} tensor")
-        _require(t.device == like.device, f"{what}: all tensors must be on {like.device}")
+        if not (t.dtype == dtype and t.dim() == 1 and t.is_contiguous()):
+            _fail(f"{what}: {name} must be a contiguous 1-D {str(dtype)[6:]} tensor")
+        if t.get_device() != device:
+            _fail(f"{what}: all tensors must be on {like.device}")
+
+
+def _check_table(what, table, rows, name, like):
+    if not (table.dtype == torch.int32 and table.dim() == 2 and table.shape[0] == rows
+            and (table.shape[1] <= 1 or table.stride(1) == 1) and table.get_device() == like.get_device()):
+        _fail(f"{what}: {name} must be int32 [sequences, blocks] with contiguous rows, on {like.device}")
+
+
+def _check_heads(what, x, tokens, name, like):
+    if not (x.dtype == torch.bfloat16 and x.dim() == 3 and x.stride(2) == 1 and x.shape[0] == tokens):
+        _fail(f"{what}: {name} must be bfloat16 [tokens, heads, head_size] with a contiguous last dimension")
+    if x.get_device() != like.get_device():
+        _fail(f"{what}: all tensors must be on {like.device}")
+
+
+def _check_inv_freq(what, inv_freq, like):
+    if not (inv_freq.dtype in (torch.float64, torch.float32) and inv_freq.dim() == 1 and inv_freq.is_contiguous()
+            and inv_freq.get_device() == like.get_device()):
+        _fail(f"{what}: inv_freq must be a contiguous 1-D float64 or float32 tensor on {like.device}")
 
 
 def _fwd_paged(q, k_cache, v_cache, out, cu_seqlens_q, cache_seqlens, max_seqlen_q, page_table, k_descale, v_descale,
                softmax_scale, is_causal, window_left, window_right):
-    _require(q.dtype == torch.bfloat16 and q.dim() in (3, 4) and q.stride(-1) == 1,
-             "fwd: q must be bfloat16 [T,H,d] or [B,S,H,d] with a contiguous last dimension")
+    shape = q.shape
+    packed = len(shape) == 3
+    if not (q.dtype == torch.bfloat16 and (packed or len(shape) == 4) and q.stride(-1) == 1):
+        _fail("fwd: q must be bfloat16 [T,H,d] or [B,S,H,d] with a contiguous last dimension")
     _check_cache("fwd", k_cache, k_descale, "k", q)
     _check_cache("fwd", v_cache, v_descale, "v", q)
-    _require(v_cache.shape == k_cache.shape and k_cache.shape[3] == q.shape[-1],
-             "fwd: k_cache and v_cache must have one shape, with the head size of q")
-    _require(cache_seqlens is not None, "fwd: a paged cache needs the sequences' lengths (cache_seqlens)")
-    _check_ints("fwd", q, torch.int32, cache_seqlens=cache_seqlens)
+    if not (v_cache.shape == k_cache.shape and k_cache.shape[3] == shape[-1]):
+        _fail("fwd: k_cache and v_cache must have one shape, with the head size of q")
+    if cache_seqlens is None:
+        _fail("fwd: a paged cache needs the sequences' lengths (cache_seqlens)")
     B = cache_seqlens.numel()
-    _require(page_table.dim() == 2 and page_table.dtype == torch.int32 and page_table.shape[0] == B
-             and (page_table.shape[1] <= 1 or page_table.stride(1) == 1) and page_table.device == q.device,
-             "fwd: page_table must be int32 [batch, blocks] with contiguous rows, on the device of q")
-    if q.dim() == 3:
-        _require(cu_seqlens_q is not None, "fwd: packed q needs cu_seqlens_q")
-        _check_ints("fwd", q, torch.int32, cu_seqlens_q=cu_seqlens_q)
-        _require(cu_seqlens_q.numel() == B + 1, "fwd: cu_seqlens_q and cache_seqlens disagree")
+    _check_table("fwd", page_table, B, "page_table", q)
+    if packed:
+        if cu_seqlens_q is None:
+            _fail("fwd: packed q needs cu_seqlens_q")
+        _check_ints("fwd", q, torch.int32, cache_seqlens=cache_seqlens, cu_seqlens_q=cu_seqlens_q)
+        if cu_seqlens_q.numel() != B + 1:
+            _fail("fwd: cu_seqlens_q and cache_seqlens disagree")
         if max_seqlen_q is None:
-            max_seqlen_q = q.shape[0]
+            max_seqlen_q = shape[0]
     else:
-        _require(cu_seqlens_q is None and q.shape[0] == B,
-                 "fwd: batched q needs one sequence for each length and no cu_seqlens_q")
-        max_seqlen_q = q.shape[1]
-    H, Hk = q.shape[-2], k_cache.shape[2]
-    _require(Hk > 0 and H % Hk == 0 and H > 0, "fwd: the heads of q must be a multiple of the cache's")
-    _require(window_left < 0 and window_right < 0 or is_causal and window_right in (-1, 0),
-             "fwd: sliding windows need causal attention, and end at the token itself")
+        _check_ints("fwd", q, torch.int32, cache_seqlens=cache_seqlens)
+        if cu_seqlens_q is not None or shape[0] != B:
+            _fail("fwd: batched q needs one sequence for each length and no cu_seqlens_q")
+        max_seqlen_q = shape[1]
+    H, Hk = shape[-2], k_cache.shape[2]
+    if not (Hk > 0 and H > 0 and H % Hk == 0):
+        _fail("fwd: the heads of q must be a multiple of the cache's")
+    if not (window_left < 0 and window_right < 0 or is_causal and window_right in (-1, 0)):
+        _fail("fwd: sliding windows need causal attention, and end at the token itself")
+    device = q.device
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    else:
-        _require(out.shape == q.shape and out.dtype == q.dtype and out.stride(-1) == 1 and out.device == q.device,
-                 "fwd: out must match q")
-    lse = torch.empty((H, q.shape[0]) if q.dim() == 3 else (B, H, q.shape[1]), dtype=torch.float32, device=q.device)
+        out = torch.empty(shape, dtype=torch.bfloat16, device=device)
+    elif not (out.shape == shape and out.dtype == q.dtype and out.stride(-1) == 1 and out.device == device):
+        _fail("fwd: out must match q")
+    lse = torch.empty((H, shape[0]) if packed else (B, H, shape[1]), dtype=torch.float32, device=device)
     if softmax_scale is None:
-        softmax_scale = q.shape[-1] ** -0.5
+        softmax_scale = shape[-1] ** -0.5
     if q.numel() and B:
         _C.paged_attention_fp8(q, k_cache, v_cache, k_descale, v_descale, page_table, cache_seqlens, cu_seqlens_q,
                                max_seqlen_q, out, lse, softmax_scale, is_causal, window_left)
-    empty = torch.empty(0, dtype=torch.float32, device=q.device)
+    empty = torch.empty(0, dtype=torch.float32, device=device)
     return out, lse, empty, empty
 
 
 # --------------------------------------------------------------------- paged 8-bit KV cache --
 def _kv_block_plan(context_lens, new_lens, block_table, free_blocks, free_begin, block_size, num_blocks,
                    slot_mapping, positions, cu_seqlens_q, seq_lens, free_end, status):
-    like = slot_mapping
-    _check_ints("kv_block_plan", like, torch.int32, context_lens=context_lens, new_lens=new_lens,
+    what = "kv_block_plan"
+    _check_ints(what, slot_mapping, torch.int32, context_lens=context_lens, new_lens=new_lens,
                 free_blocks=free_blocks, free_begin=free_begin, cu_seqlens_q=cu_seqlens_q, seq_lens=seq_lens,
                 free_end=free_end, status=status)
-    _check_ints("kv_block_plan", like, torch.int64, slot_mapping=slot_mapping, positions=positions)
+    _check_ints(what, slot_mapping, torch.int64, slot_mapping=slot_mapping, positions=positions)
     B = context_lens.numel()
-    _require(new_lens.numel() == B and seq_lens.numel() == B and cu_seqlens_q.numel() == B + 1,
-             "kv_block_plan: new_lens and seq_lens must have one entry for each request, cu_seqlens_q one more")
-    _require(block_table.dim() == 2 and block_table.shape[0] == B and block_table.dtype == torch.int32
-             and (block_table.shape[1] <= 1 or block_table.stride(1) == 1) and block_table.device == like.device,
-             "kv_block_plan: block_table must be int32 [requests, blocks] with contiguous rows, on the same device")
-    _require(positions.numel() == slot_mapping.numel(), "kv_block_plan: positions and slot_mapping differ in length")
-    _require(free_begin.numel() == 1 and free_end.numel() == 1 and status.numel() == 3,
-             "kv_block_plan: free_begin and free_end must have 1 entry, status 3")
+    if not (new_lens.numel() == B and seq_lens.numel() == B and cu_seqlens_q.numel() == B + 1):
+        _fail("kv_block_plan: new_lens and seq_lens must have one entry for each request, cu_seqlens_q one more")
+    _check_table(what, block_table, B, "block_table", slot_mapping)
+    if positions.numel() != slot_mapping.numel():
+        _fail("kv_block_plan: positions and slot_mapping differ in length")
+    if not (free_begin.numel() == 1 and free_end.numel() == 1 and status.numel() == 3):
+        _fail("kv_block_plan: free_begin and free_end must have 1 entry, status 3")
     _C.kv_block_plan(context_lens, new_lens, block_table, free_blocks, free_begin, block_size, num_blocks,
                      slot_mapping, positions, cu_seqlens_q, seq_lens, free_end, status)
-
-
-def _check_heads(what, x, tokens, name, like):
-    _require(x.dim() == 3 and x.dtype == torch.bfloat16 and x.stride(2) == 1 and x.shape[0] == tokens,
-             f"{what}: {name} must be bfloat16 [tokens, heads, head_size] with a contiguous last dimension")
-    _require(x.device == like.device, f"{what}: all tensors must be on {like.device}")
-
-
-def _check_inv_freq(what, inv_freq, like):
-    _require(inv_freq.dim() == 1 and inv_freq.dtype in (torch.float32, torch.float64) and inv_freq.is_contiguous()
-             and inv_freq.device == like.device,
-             f"{what}: inv_freq must be a contiguous 1-D float64 or float32 tensor on {like.device}")
 
 
 def _rotary_embedding_scaled(positions, query, key, inv_freq, attn_factor, is_neox, query_out, key_out):
@@ -406,13 +425,15 @@ def _rotary_embedding_scaled(positions, query, key, inv_freq, attn_factor, is_ne
     T = positions.numel()
     _check_heads(what, query, T, "query", query)
     _check_heads(what, query_out, T, "query_out", query)
-    _require(query_out.shape == query.shape, f"{what}: query_out must have the shape of query")
-    _require((key is None) == (key_out is None), f"{what}: key and key_out come together")
+    if query_out.shape != query.shape:
+        _fail("rotary_embedding_scaled: query_out must have the shape of query")
+    if (key is None) != (key_out is None):
+        _fail("rotary_embedding_scaled: key and key_out come together")
     if key is not None:
         _check_heads(what, key, T, "key", query)
         _check_heads(what, key_out, T, "key_out", query)
-        _require(key_out.shape == key.shape and key.shape[2] == query.shape[2],
-                 f"{what}: key_out must have the shape of key, and both the head size of query")
+        if not (key_out.shape == key.shape and key.shape[2] == query.shape[2]):
+            _fail("rotary_embedding_scaled: key_out must have the shape of key, and both the head size of query")
     _C.rope_scaled(positions, query, key, inv_freq, attn_factor, is_neox, query_out, key_out)
 
 
@@ -425,20 +446,24 @@ def _store_kv_cache_fp8(key, value, k_cache, v_cache, k_scale, v_scale, slot_map
     _check_heads(what, value, T, "value", key)
     _check_cache(what, k_cache, k_scale, "k", key)
     _check_cache(what, v_cache, v_scale, "v", key)
-    _require(value.shape == key.shape and v_cache.shape == k_cache.shape and k_cache.shape[2:] == key.shape[1:],
-             f"{what}: key and value must have one shape, the caches too, with the same heads")
-    _require((positions is None) == (inv_freq is None), f"{what}: positions and inv_freq come together")
-    _require((query is None) == (query_out is None), f"{what}: query and query_out come together")
+    if not (value.shape == key.shape and v_cache.shape == k_cache.shape and k_cache.shape[2:] == key.shape[1:]):
+        _fail("store_kv_cache_fp8: key and value must have one shape, the caches too, with the same heads")
+    if (positions is None) != (inv_freq is None):
+        _fail("store_kv_cache_fp8: positions and inv_freq come together")
+    if (query is None) != (query_out is None):
+        _fail("store_kv_cache_fp8: query and query_out come together")
     if positions is not None:
         _check_ints(what, key, torch.int64, positions=positions)
         _check_inv_freq(what, inv_freq, key)
-        _require(positions.numel() == T, f"{what}: positions and slot_mapping differ in length")
+        if positions.numel() != T:
+            _fail("store_kv_cache_fp8: positions and slot_mapping differ in length")
     if query is not None:
-        _require(positions is not None, f"{what}: a query is given to be rotated, and needs positions")
+        if positions is None:
+            _fail("store_kv_cache_fp8: a query is given to be rotated, and needs positions")
         _check_heads(what, query, T, "query", key)
         _check_heads(what, query_out, T, "query_out", key)
-        _require(query_out.shape == query.shape and query.shape[2] == key.shape[2],
-                 f"{what}: query_out must have the shape of query, with the head size of key")
+        if not (query_out.shape == query.shape and query.shape[2] == key.shape[2]):
+            _fail("store_kv_cache_fp8: query_out must have the shape of query, with the head size of key")
     _C.kv_store_fp8(key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping, query, positions, inv_freq,
                     attn_factor, is_neox, query_out)
 

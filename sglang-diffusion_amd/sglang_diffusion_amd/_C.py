@@ -226,10 +226,12 @@ def _stream(t: torch.Tensor) -> int:
     device's state."""
     if not t.is_cuda:
         raise RuntimeError("mi355 kernels need tensors on a HIP device (got a CPU tensor)")
-    if t.device.index != torch.cuda.current_device():
-        raise RuntimeError(f"tensor on cuda:{t.device.index} but the current device is cuda:"
+    index = t.get_device()
+    if index != torch.cuda.current_device():
+        raise RuntimeError(f"tensor on cuda:{index} but the current device is cuda:"
                            f"{torch.cuda.current_device()}: wrap the call in torch.cuda.device(...)")
-    return torch.cuda.current_stream(t.device).cuda_stream
+    # (the raw handle: making a Stream object to ask it costs microseconds at every launch)
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _p(t: Optional[torch.Tensor]) -> Optional[int]:
