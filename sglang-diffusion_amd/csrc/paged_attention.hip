@@ -31,7 +31,7 @@ typedef __fp16 hw_f16x4 __attribute__((__vector_size__(4 * sizeof(__fp16))));
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int KT = 64;               // keys of a tile
-constexpr float M_START = -1e30f;    // reference of a row that has seen nothing yet
+constexpr float M_EMPTY = -1e30f;    // reference of a row without weight, among those that have some
 constexpr float LAZY_SUM = 8192.f;   // a lane's sum of a tile's exponentials up to which m stays
 
 struct PagedParams {
@@ -52,7 +52,7 @@ struct PagedParams {
   // items
   int items, target, chunk_min, split;
   float* part;       // [Hk * items][M][D + 2]
-  int32_t* info;     // [items][4]: sequence, row tile, chunk, chunks
+  int32_t* info;     // [B][2]: first item of the sequence, chunks of each of its row tiles
 };
 
 struct Seq {
@@ -109,7 +109,7 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* total, int64_t
 // The item'th item of a key/value head; false behind the last one.  Every thread of the
 // workgroup calls it.
 template <int M>
-__device__ bool find_item(const PagedParams& p, int item, bool writes_info, Item* out) {
+__device__ bool find_item(const PagedParams& p, int item, int hk, Item* out) {
   __shared__ int64_t sums[8];
   __shared__ Item found;
   const int per = (p.B + blockDim.x - 1) / blockDim.x;
@@ -147,6 +147,10 @@ __device__ bool find_item(const PagedParams& p, int item, bool writes_info, Item
         const int k = (int)(item - at);
         // causal rows further down see more: they begin first
         found = Item{b, (int)tiles - 1 - k / chunks, k % chunks, chunks, length};
+        if (p.split && k == 0 && hk == 0) {  // for the join
+          p.info[2 * b] = item;
+          p.info[2 * b + 1] = chunks;
+        }
         break;
       }
       at += tiles * chunks;
@@ -154,13 +158,6 @@ __device__ bool find_item(const PagedParams& p, int item, bool writes_info, Item
   }
   __syncthreads();
   *out = found;
-  if (writes_info && p.split && threadIdx.x == 0) {
-    int32_t* to = p.info + 4 * (int64_t)item;
-    to[0] = found.b;
-    to[1] = found.tile;
-    to[2] = found.chunk;
-    to[3] = found.b < 0 ? 0 : found.chunks;
-  }
   return found.b >= 0;
 }
 
@@ -237,6 +234,18 @@ __device__ __forceinline__ Scales scales_of(const PagedParams& p, float ks, floa
   return s;
 }
 
+// Where a row's reference goes, by the largest exponent of a tile (relative to the reference) and the
+// weight that the row has so far: up to that exponent, and for a row without weight yet (which
+// starts from 0) also down to it.  Rows that see nothing stay.
+struct Move {
+  float by, shrink;
+};
+__device__ __forceinline__ Move move_reference(float top, float mass) {
+  if (mass == 0.f) return Move{top == -INFINITY ? 0.f : top, 0.f};
+  const float by = fmaxf(top, 0.f);
+  return Move{by, __builtin_amdgcn_exp2f(-by)};
+}
+
 // Without branches on purpose: a conditional write into one element of a matrix instruction's
 // result, with control flow around it, has come out of the compiler with the write missing.
 __device__ __forceinline__ bool sees(bool ok, int key, int lo, int hi) {
@@ -290,7 +299,7 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
   __shared__ float wave_m[4][M], wave_l[4][M];
   const int item = blockIdx.x / p.Hk, hk = blockIdx.x % p.Hk;
   Item it;
-  if (!find_item<M>(p, item, hk == 0, &it)) return;
+  if (!find_item<M>(p, item, hk, &it)) return;
   const Job job = job_of<M>(p, it, hk);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, g = lane >> 4;
@@ -315,7 +324,7 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
   float m[RT], l[RT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    m[rt] = M_START;
+    m[rt] = 0.f;
     l[rt] = 0.f;
 #pragma unroll
     for (int d = 0; d < DB; ++d) o[rt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -413,13 +422,15 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
     f16x8 pf[RT][2];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      // exponents, then exponentials against the reference as it stands; it moves, and O and l
-      // with it, only where a lane's sum says that it has to
-      float x[4][4], e[4][4], sum[4], all;
+      // exponents against the reference as it stands, x, and their exponentials; the reference moves
+      // (move_reference) only where a lane's sum asks for it, or a row has had no weight yet
+      float x[4][4], e[4][4], sum[4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
+      for (int c = 0; c < 4; ++c) {
+        const float add = sc.v_log[c] - m[rt];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[c][i] = fmaf(s[rt][c][i], sc.k[c], sc.v_log[c]);
+        for (int i = 0; i < 4; ++i) x[c][i] = fmaf(s[rt][c][i], sc.k[c], add);
+      }
       if (masked) {
 #pragma unroll
         for (int c = 0; c < 4; ++c)
@@ -431,26 +442,34 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) e[c][i] = __builtin_amdgcn_exp2f(x[c][i] - m[rt]);
+          for (int i = 0; i < 4; ++i) e[c][i] = __builtin_amdgcn_exp2f(x[c][i]);
           sum[c] = (e[c][0] + e[c][1]) + (e[c][2] + e[c][3]);
         }
-        all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        return (sum[0] + sum[1]) + (sum[2] + sum[3]);
       };
-      exponentials();
-      if (__builtin_amdgcn_ballot_w64(!(all <= LAZY_SUM)) != 0) {
+      const float all = exponentials();
+      if (__builtin_amdgcn_ballot_w64(!(all <= LAZY_SUM) || l[rt] == 0.f) != 0) {
         float top = x[0][0];
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int i = 0; i < 4; ++i) top = fmaxf(top, x[c][i]);
-        top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const float higher = fmaxf(m[rt], top), shrink = __builtin_amdgcn_exp2f(m[rt] - higher);
-        m[rt] = higher;
-        l[rt] *= shrink;
+        float mass = l[rt];
 #pragma unroll
-        for (int d = 0; d < DB; ++d) o[rt][d] *= shrink;
-        exponentials();
+        for (int w = 16; w < 64; w <<= 1) {
+          top = fmaxf(top, __shfl_xor(top, w, 64));
+          mass += __shfl_xor(mass, w, 64);
+        }
+        const Move mv = move_reference(top, mass);
+        m[rt] += mv.by;
+        l[rt] *= mv.shrink;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) o[rt][d] *= mv.shrink;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[c][i] -= mv.by;
+        (void)exponentials();
       }
 #pragma unroll
       for (int c = 0; c < 4; ++c) l[rt] = fmaf(sum[c], sc.v_inv[c], l[rt]);
@@ -505,6 +524,7 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
   for (int rt = 0; rt < RT; ++rt) {
     l[rt] += __shfl_xor(l[rt], 16, 64);
     l[rt] += __shfl_xor(l[rt], 32, 64);
+    if (l[rt] == 0.f) m[rt] = M_EMPTY;
     if (g == 0) {
       wave_m[wave][16 * rt + r] = m[rt];
       wave_l[wave][16 * rt + r] = l[rt];
@@ -574,7 +594,7 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedP
   __shared__ int nan_values;
   const int item = blockIdx.x / p.Hk, hk = blockIdx.x % p.Hk;
   Item it;
-  if (!find_item<M>(p, item, hk == 0, &it)) return;
+  if (!find_item<M>(p, item, hk, &it)) return;
   const Job job = job_of<M>(p, it, hk);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 31, hh = lane >> 5;
@@ -656,7 +676,7 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedP
   for (int d = 0; d < DVB; ++d)
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
-  float m = M_START, l = 0.f;
+  float m = 0.f, l = 0.f;
 
   if (tid == 0) nan_values = 0;
   __syncthreads();
@@ -705,48 +725,53 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedP
       }
       const bool masked = key0 + KT > job.s.len || now.ok != 15u || (p.causal && key0 + KT - 1 > w_lo) ||
                           (p.window >= 0 && key0 < w_hi - p.window);
-      float x[2][16], sum[4], all;
+      // as in the kernel above: x[c][e] is element e of piece c
+      float x[4][8], pe[4][8], sum[4];
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
+      for (int c = 0; c < 4; ++c) {
+        const float add = sc.v_log[c] - m;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[kb][e] = fmaf(s[kb][e], sc.k[2 * kb + (e >> 3)], sc.v_log[2 * kb + (e >> 3)]);
+        for (int e = 0; e < 8; ++e) x[c][e] = fmaf(s[c >> 1][8 * (c & 1) + e], sc.k[c], add);
+      }
       if (masked) {
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int c = 0; c < 4; ++c)
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            x[kb][e] = sees((now.ok >> (2 * kb + (e >> 3))) & 1, key0 + kb * 32 + (e & 3) + 8 * (e >> 2) + 4 * hh,
-                            see_lo, see_hi) ? x[kb][e] : -INFINITY;
+          for (int e = 0; e < 8; ++e)
+            x[c][e] = sees((now.ok >> c) & 1, key0 + 16 * c + (e & 3) + 8 * (e >> 2) + 4 * hh, see_lo, see_hi)
+                          ? x[c][e] : -INFINITY;
       }
-      float pe[2][16];
       auto exponentials = [&]() {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           sum[c] = 0.f;
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            pe[c >> 1][8 * (c & 1) + e] = __builtin_amdgcn_exp2f(x[c >> 1][8 * (c & 1) + e] - m);
-            sum[c] += pe[c >> 1][8 * (c & 1) + e];
+            pe[c][e] = __builtin_amdgcn_exp2f(x[c][e]);
+            sum[c] += pe[c][e];
           }
         }
-        all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        return (sum[0] + sum[1]) + (sum[2] + sum[3]);
       };
-      exponentials();
-      if (__builtin_amdgcn_ballot_w64(!(all <= LAZY_SUM)) != 0) {
+      const float all = exponentials();
+      if (__builtin_amdgcn_ballot_w64(!(all <= LAZY_SUM) || l == 0.f) != 0) {
         float top = x[0][0];
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int c = 0; c < 4; ++c)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) top = fmaxf(top, x[kb][e]);
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const float higher = fmaxf(m, top), shrink = __builtin_amdgcn_exp2f(m - higher);
-        m = higher;
-        l *= shrink;
+          for (int e = 0; e < 8; ++e) top = fmaxf(top, x[c][e]);
+        const Move mv = move_reference(fmaxf(top, __shfl_xor(top, 32, 64)), l + __shfl_xor(l, 32, 64));
+        m += mv.by;
+        l *= mv.shrink;
 #pragma unroll
         for (int d = 0; d < DVB; ++d)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) o[d][e] *= shrink;
-        exponentials();
+          for (int e = 0; e < 16; ++e) o[d][e] *= mv.shrink;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[c][e] -= mv.by;
+        (void)exponentials();
       }
 #pragma unroll
       for (int c = 0; c < 4; ++c) l = fmaf(sum[c], sc.v_inv[c], l);
@@ -756,7 +781,7 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedP
 #pragma unroll
         for (int st = 0; st < 2; ++st)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) pf[kb][st][j] = (_Float16)pe[kb][8 * st + j];
+          for (int j = 0; j < 8; ++j) pf[kb][st][j] = (_Float16)pe[2 * kb + st][j];
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -816,7 +841,7 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedP
         *reinterpret_cast<f32x4*>(part + in_tile * D + d * 32 + 8 * g + 4 * hh) =
             f32x4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
     if (hh == 0) {
-      part[M * D + 2 * in_tile] = m;
+      part[M * D + 2 * in_tile] = l == 0.f ? M_EMPTY : m;
       part[M * D + 2 * in_tile + 1] = l;
     }
     return;
@@ -850,40 +875,82 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedP
 }
 
 // ------------------------------------------------------------------------------------- joint --
-// The chunks of one row tile: a wave for each row, its lanes over the channels.
+// The chunks of a row: a wave for each row of q.  Lane c weighs chunk c; the sums run over eight
+// chunks at a time, so that their loads are in flight together.
 template <int D>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p, int M) {
-  const int item = blockIdx.x / p.Hk, hk = blockIdx.x % p.Hk;
-  const int32_t* info = p.info + 4 * (int64_t)item;
-  const int b = info[0], tile = info[1], chunk = info[2], chunks = info[3];
-  if (chunk != 0 || chunks <= 1) return;  // items behind the last one have no chunks
-  const Seq s = seq_of(p, b);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int in_tile = blockIdx.y * 4 + wave, row = tile * M + in_tile;
-  if (row >= s.n * p.G) return;
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p, int M, int64_t rows) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row_of_q = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (row_of_q >= rows) return;
+  const int H = p.Hk * p.G;
+  const int64_t t = row_of_q / H;
+  const int head = (int)(row_of_q - t * H);
+  int b, tok;
+  if (p.cu) {  // the sequence whose rows t is among: those that end at or before t come before it
+    b = 0;
+    for (int i0 = 0; i0 < p.B; i0 += 64) {
+      const int i = i0 + lane;
+      const unsigned long long before = __builtin_amdgcn_ballot_w64(i < p.B && p.cu[min(i, p.B - 1) + 1] <= (int)t);
+      b += __popcll(before);
+      if (before != ~0ull) break;
+    }
+    if (b >= p.B) return;  // a row behind the last sequence
+    tok = (int)t - seq_of(p, b).first;
+  } else {
+    b = (int)(t / p.Sq);
+    tok = (int)(t - (int64_t)b * p.Sq);
+  }
+  const int hk = head / p.G, row = tok * p.G + head - hk * p.G;
+  const int n = seq_of(p, b).n;
+  if (tok < 0 || tok >= n) return;
+  const int base = p.info[2 * b], chunks = p.info[2 * b + 1];
+  const int tiles = (n * p.G + M - 1) / M;
+  // one chunk: written by the kernel itself.  (Running sums that are none would leave this unset.)
+  if (chunks <= 1 || base < 0 || base + (int64_t)tiles * chunks > p.items) return;
   const int64_t step = (int64_t)M * (D + 2);
-  const float* part = p.part + ((int64_t)hk * p.items + item) * step;
-  float top = M_START;
+  const int in_tile = row % M;
+  const float* part = p.part + ((int64_t)hk * p.items + base + (int64_t)(tiles - 1 - row / M) * chunks) * step;
+  float top = M_EMPTY;
   for (int c = lane; c < chunks; c += 64) top = fmaxf(top, part[c * step + M * D + 2 * in_tile]);
   top = group_max<64>(top);
-  constexpr int PER = D / 64;
-  float acc[PER], l = 0.f;
+  // lanes hold four channels; 256 / D chunks side by side
+  constexpr int SIDE = 256 / D, LANES = D / 4;
+  const int mine = lane / LANES, ch = lane % LANES;
+  f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+  float l = 0.f;
+  for (int c0 = 0; c0 < chunks; c0 += 64) {
+    const int c = min(c0 + lane, chunks - 1);
+    const float* ml = part + c * step + M * D + 2 * in_tile;
+    const float w = c0 + lane < chunks ? __builtin_amdgcn_exp2f(ml[0] - top) : 0.f;
+    l = fmaf(w != 0.f ? ml[1] : 0.f, w, l);
+    const int here = min(64, chunks - c0);
+    for (int k = 0; k < here; k += 4 * SIDE) {
+      f32x4 v[4];
+      float wv[4];
 #pragma unroll
-  for (int j = 0; j < PER; ++j) acc[j] = 0.f;
-  for (int c = 0; c < chunks; ++c) {
-    const float* at = part + c * step;
-    const float w = __builtin_amdgcn_exp2f(at[M * D + 2 * in_tile] - top);
-    l = fmaf(at[M * D + 2 * in_tile + 1], w, l);
+      for (int u = 0; u < 4; ++u) {
+        const int at = k + u * SIDE + mine;
+        wv[u] = __shfl(w, min(at, 63), 64);
+        v[u] = *reinterpret_cast<const f32x4*>(part + min(c0 + at, chunks - 1) * step + in_tile * D + 4 * ch);
+        if (at >= here) wv[u] = 0.f;
+      }
 #pragma unroll
-    for (int j = 0; j < PER; ++j) acc[j] = fmaf(at[in_tile * D + PER * lane + j], w, acc[j]);
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j] = wv[u] == 0.f ? acc[j] : fmaf(v[u][j], wv[u], acc[j]);
+    }
   }
-  const int tok = row / p.G, head = hk * p.G + row - tok * p.G;
+  l = group_sum<64>(l);
+#pragma unroll
+  for (int w = LANES; w < 64; w <<= 1)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[j] += __shfl_xor(acc[j], w, 64);
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  unsigned short* op = p.o + b * p.o_sb + (int64_t)(s.first + tok) * p.o_ss + head * p.o_sh + PER * lane;
-  if constexpr (PER == 2) *reinterpret_cast<unsigned*>(op) = pack_bf2(acc[0] * inv, acc[1] * inv);
-  else *op = f2bf(acc[0] * inv);
+  if (mine == 0)
+    *reinterpret_cast<u32x2*>(p.o + b * p.o_sb + (p.cu ? t : tok) * p.o_ss + head * p.o_sh + 4 * ch) =
+        u32x2{pack_bf2(acc[0] * inv, acc[1] * inv), pack_bf2(acc[2] * inv, acc[3] * inv)};
   if (p.lse && lane == 0)
-    p.lse[b * p.lse_sb + head * p.lse_sh + s.first + tok] =
+    p.lse[b * p.lse_sb + head * p.lse_sh + (p.cu ? t : tok)] =
         l == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
 }
 
@@ -916,14 +983,17 @@ Plan plan_of(const mi355_paged_attn_args* a) {
   w.M = w.few ? 16 * w.few : 128;
   const int64_t tiles = all_rows / w.M + a->B;  // row tiles: at most one not full for each sequence
   // two workgroups of either kernel fit a CU
-  const int64_t want = 2 * (int64_t)cu_count();
+#ifndef PAGED_WANT
+#define PAGED_WANT 2
+#endif
+  const int64_t want = (w.few ? PAGED_WANT : 2) * (int64_t)cu_count();
   w.target = (want + a->Hk - 1) / a->Hk;
   w.chunk_min = w.few ? 4 : 8;
   const int64_t cap = a->table_width * a->block_size;
   w.split = cap > (int64_t)w.chunk_min * KT && (all_rows / w.M) * a->Hk < 2 * want;
   w.items = tiles + (w.split ? w.target : 0);
   w.part_bytes = w.split ? a->Hk * w.items * w.M * (a->D + 2) * (int64_t)sizeof(float) : 0;
-  w.info_bytes = w.split ? w.items * 4 * (int64_t)sizeof(int32_t) : 0;
+  w.info_bytes = w.split ? a->B * 2 * (int64_t)sizeof(int32_t) : 0;
   return w;
 }
 
@@ -972,7 +1042,8 @@ int launch(const PagedParams& p, const Plan& w, hipStream_t st) {
   }
   MI355_CHECK_LAUNCH("paged_attn_fp8");
   if (w.split) {
-    hipLaunchKernelGGL(paged_join_kernel<D>, dim3(grid.x, (unsigned)(w.M / 4)), dim3(256), 0, st, p, w.M);
+    const int64_t rows = (int64_t)p.Sq * (p.cu ? 1 : p.B) * p.Hk * p.G;
+    hipLaunchKernelGGL(paged_join_kernel<D>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, p, w.M, rows);
     MI355_CHECK_LAUNCH("paged_attn_fp8 (join)");
   }
   return MI355_OK;
