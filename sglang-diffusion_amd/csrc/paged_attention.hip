@@ -50,7 +50,8 @@ struct PagedParams {
   int num_blocks, lb, causal, window;
   float scale_log2;
   // items
-  int items, target, chunk_min, split;
+  int items, chunk_min, split;
+  float inv_target;
   float* part;       // [Hk * items][M][D + 2]
   int32_t* info;     // [B][2]: first item of the sequence, chunks of each of its row tiles
 };
@@ -79,81 +80,81 @@ __device__ __forceinline__ void seq_tiles(const PagedParams& p, const Seq& s, in
 }
 
 struct Item {
-  int b, tile, chunk, chunks;  // sequence, row tile, chunk of keys and how many there are
+  Seq s;
+  int b, tile, chunk, chunks;  // sequence (-1: none), row tile, chunk of keys and how many there are
   int length;                  // tiles of a chunk
 };
 
-// Sum of a value over the 256 threads of the workgroup, and (second form) the sum over the
-// threads before this one.
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* total, int64_t (&wave_sum)[8]) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int64_t in = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const long long a = __shfl_up((long long)in, o, 64);
-    if (lane >= o) in += a;
-  }
-  __syncthreads();
-  if (lane == 63) wave_sum[wave] = in;
-  __syncthreads();
-  int64_t before = in - v, all = 0;
-  const int waves = blockDim.x >> 6;
-  for (int w = 0; w < waves; ++w) {
-    if (w < wave) before += wave_sum[w];
-    all += wave_sum[w];
-  }
-  *total = all;
-  return before;
+// Sum over the lanes up to this one, of a wave whose lanes are all active.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);  // row_shr:2
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);  // row_shr:4
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);  // row_shr:8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
+  return v;
 }
 
-// The item'th item of a key/value head; false behind the last one.  Every thread of the
-// workgroup calls it.
+// The item'th item of a key/value head, for the whole workgroup; false behind the last one.  One
+// wave adds up the sequences, `per` that follow each other to a lane, and hands the item on.
 template <int M>
 __device__ bool find_item(const PagedParams& p, int item, int hk, Item* out) {
-  __shared__ int64_t sums[8];
   __shared__ Item found;
-  const int per = (p.B + blockDim.x - 1) / blockDim.x;
-  const int b0 = threadIdx.x * per, b1 = min(p.B, b0 + per);
-  int length = 1 << 30;
-  int64_t all;
-  if (threadIdx.x == 0) found.b = -1;
-  if (p.split) {
-    int64_t work = 0;
-    for (int b = b0; b < b1; ++b) {
-      const Seq s = seq_of(p, b);
-      int lo, hi;
-      seq_tiles(p, s, lo, hi);
-      work += (((int64_t)s.n * p.G + M - 1) / M) * (hi - lo);
-    }
-    block_scan(work, &all, sums);
-    length = (int)min((int64_t)(1 << 30), max((int64_t)p.chunk_min, (all + p.target - 1) / p.target));
-  }
-  int64_t mine = 0;
-  for (int b = b0; b < b1; ++b) {
-    const Seq s = seq_of(p, b);
-    int lo, hi;
-    seq_tiles(p, s, lo, hi);
-    mine += (((int64_t)s.n * p.G + M - 1) / M) * max(1, (hi - lo + length - 1) / length);
-  }
-  int64_t at = block_scan(mine, &all, sums);
-  if (item >= at && item < at + mine) {
-    for (int b = b0; b < b1; ++b) {
-      const Seq s = seq_of(p, b);
-      int lo, hi;
-      seq_tiles(p, s, lo, hi);
-      const int64_t tiles = ((int64_t)s.n * p.G + M - 1) / M;
-      const int chunks = max(1, (hi - lo + length - 1) / length);
-      if (item < at + tiles * chunks) {
-        const int k = (int)(item - at);
-        // causal rows further down see more: they begin first
-        found = Item{b, (int)tiles - 1 - k / chunks, k % chunks, chunks, length};
-        if (p.split && k == 0 && hk == 0) {  // for the join
-          p.info[2 * b] = item;
-          p.info[2 * b + 1] = chunks;
-        }
-        break;
+  if (threadIdx.x < 64) {
+    const int lane = threadIdx.x;
+    const int per = (p.B + 63) >> 6;
+    const int b0 = lane * per, b1 = min(p.B, b0 + per);
+    int length = 1 << 30;
+    Seq s{0, 0, 0};
+    auto tiles_of = [&](const Seq& q) { return (q.n * p.G + M - 1) / M; };
+    if (p.split) {
+      // tiles of keys of all items, as a float: only the length of a chunk hangs on it, and every
+      // workgroup adds the same numbers in the same order
+      float work = 0.f;
+      for (int b = b0; b < b1; ++b) {
+        s = seq_of(p, b);
+        int lo, hi;
+        seq_tiles(p, s, lo, hi);
+        work += (float)tiles_of(s) * (float)(hi - lo);
       }
-      at += tiles * chunks;
+      work = group_sum<64>(work);
+      length = (int)fminf(1e9f, fmaxf((float)p.chunk_min, ceilf(work * p.inv_target)));
+    } else if (b0 < b1) {
+      s = seq_of(p, b0);
+    }
+    auto chunks_of = [&](const Seq& q) {
+      int lo, hi;
+      seq_tiles(p, q, lo, hi);
+      return max(1, (hi - lo + length - 1) / length);
+    };
+    int mine = 0;
+    if (per == 1) {
+      if (b0 < b1) mine = tiles_of(s) * chunks_of(s);
+    } else {
+      for (int b = b0; b < b1; ++b) {
+        s = seq_of(p, b);
+        mine += tiles_of(s) * chunks_of(s);
+      }
+    }
+    const int upto = wave_scan(mine);
+    if (lane == 0) found.b = -1;
+    int at = upto - mine;
+    if (item >= at && item < upto) {
+      for (int b = b0; b < b1; ++b) {
+        if (per > 1) s = seq_of(p, b);
+        const int tiles = tiles_of(s), chunks = chunks_of(s), k = item - at;
+        if (k >= 0 && k < (int64_t)tiles * chunks) {
+          // causal rows further down see more: they begin first
+          found = Item{s, b, tiles - 1 - k / chunks, k % chunks, chunks, length};
+          if (p.split && k == 0 && hk == 0) {  // for the join
+            p.info[2 * b] = item;
+            p.info[2 * b + 1] = chunks;
+          }
+          break;
+        }
+        at += tiles * chunks;
+      }
     }
   }
   __syncthreads();
@@ -171,7 +172,7 @@ struct Job {
 template <int M>
 __device__ __forceinline__ Job job_of(const PagedParams& p, const Item& it, int hk) {
   Job j;
-  j.s = seq_of(p, it.b);
+  j.s = it.s;
   j.b = it.b;
   j.hk = hk;
   j.rows = j.s.n * p.G;
@@ -1109,7 +1110,7 @@ extern "C" int mi355_paged_attn_fp8(const mi355_paged_attn_args* a, void* stream
   p.window = a->window_left < 0 ? -1 : (int)(a->window_left < (1 << 30) ? a->window_left : (1 << 30));
   p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
   p.items = (int)w.items;
-  p.target = (int)w.target;
+  p.inv_target = 1.f / (float)w.target;
   p.chunk_min = w.chunk_min;
   p.split = w.split;
   p.part = (float*)a->workspace;
