@@ -120,6 +120,7 @@ __device__ bool find_item(const PagedParams& p, int item, int hk, Item* out) {
       }
       work = group_sum<64>(work);
       length = (int)fminf(1e9f, fmaxf((float)p.chunk_min, ceilf(work * p.inv_target)));
+      if (M < 64) length = (length + 3) & ~3;  // whole turns of the four waves
     } else if (b0 < b1) {
       s = seq_of(p, b0);
     }
@@ -296,9 +297,9 @@ __device__ __forceinline__ unsigned clear_nan(u32x4& v) {
 template <int D, int RT>
 __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
   constexpr int M = 16 * RT, NH = D / 64, CPR = D / 16, DB = D / 16;
-  __shared__ __attribute__((aligned(16))) unsigned char vimg[4][KT * D];
+  __shared__ __attribute__((aligned(16))) unsigned char vimg[4][2 * KT * D];
   __shared__ float wave_m[4][M], wave_l[4][M];
-  const int item = blockIdx.x / p.Hk, hk = blockIdx.x % p.Hk;
+  const int item = (blockIdx.x / (8 * p.Hk)) * 8 + blockIdx.x % 8, hk = (blockIdx.x / 8) % p.Hk;
   Item it;
   if (!find_item<M>(p, item, hk, &it)) return;
   const Job job = job_of<M>(p, it, hk);
@@ -331,16 +332,17 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
     for (int d = 0; d < DB; ++d) o[rt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  u32x4 kr[4][NH], vr[CPR];
+  u32x4 kr[CPR], vr[CPR];
   const unsigned char *k_head = p.kc + hk * p.kc_sh, *v_head = p.vc + hk * p.vc_sh;
-  const unsigned k_lane = (unsigned)(r * p.kc_st + 16 * g);
+  const unsigned k_lane = (unsigned)((lane / CPR) * p.kc_st + (lane % CPR) * 16);
   const unsigned v_lane = (unsigned)((lane / CPR) * p.vc_st + (lane % CPR) * 16);
   auto load_k = [&](const Ahead& a, int t) {
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       const unsigned char* at = piece_at(p, k_head, p.kc_sb, p.kc_st, a, t, c);
 #pragma unroll
-      for (int h = 0; h < NH; ++h) kr[c][h] = *reinterpret_cast<const u32x4*>(at + (k_lane + 64 * h));
+      for (int i = 0; i < CPR / 4; ++i)
+        kr[c * CPR / 4 + i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at + (k_lane + (unsigned)(i * (64 / CPR) * p.kc_st))));
     }
   };
   auto load_v = [&](const Ahead& a, int t) {
@@ -349,7 +351,7 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
       const unsigned char* at = piece_at(p, v_head, p.vc_sb, p.vc_st, a, t, c);
 #pragma unroll
       for (int i = 0; i < CPR / 4; ++i)  // 64 / CPR rows at a time
-        vr[c * CPR / 4 + i] = *reinterpret_cast<const u32x4*>(at + (v_lane + (unsigned)(i * (64 / CPR) * p.vc_st)));
+        vr[c * CPR / 4 + i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at + (v_lane + (unsigned)(i * (64 / CPR) * p.vc_st))));
     }
   };
   auto swz = [](int row) { return D == 128 ? (row >> 1) & 7 : (row >> 2) & 3; };
@@ -394,9 +396,11 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
     for (int i = 0; i < CPR; ++i) {
       const int row = (i * 64 + lane) / CPR;
       *reinterpret_cast<u32x4*>(img + row * D + (((lane % CPR) ^ swz(row)) << 4)) = vr[i];
+      *reinterpret_cast<u32x4*>(img + KT * D + row * D + (((lane % CPR) ^ swz(row)) << 4)) = kr[i];
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
+    if (more) load_k(next, t + 4);
     // entries of the tile after the next, values and scales of the next
     const int entry = load_entry(p, job, t + 8);
     const int64_t scale_at = (int64_t)next.block * p.Hk + hk;
@@ -409,16 +413,17 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) s[rt][c] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int h = 0; h < NH; ++h)
+      for (int h = 0; h < NH; ++h) {
+        const u32x4 kk = *reinterpret_cast<const u32x4*>(img + KT * D + (16 * c + r) * D + (((4 * h + g) ^ swz(16 * c + r)) << 4));
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const bf16x8 kf = widen_bf16(kr[c][h][2 * u], kr[c][h][2 * u + 1]);
+          const bf16x8 kf = widen_bf16(kk[2 * u], kk[2 * u + 1]);
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt)
             s[rt][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[rt][h][u], s[rt][c], 0, 0, 0);
         }
+      }
     }
-    if (more) load_k(next, t + 4);
 
     f16x8 pf[RT][2];
 #pragma unroll
@@ -983,13 +988,14 @@ Plan plan_of(const mi355_paged_attn_args* a) {
   w.few = rows <= 16 ? 1 : rows <= 32 ? 2 : 0;
   w.M = w.few ? 16 * w.few : 128;
   const int64_t tiles = all_rows / w.M + a->B;  // row tiles: at most one not full for each sequence
-  // two workgroups of either kernel fit a CU
-#ifndef PAGED_WANT
-#define PAGED_WANT 2
-#endif
-  const int64_t want = (w.few ? PAGED_WANT : 2) * (int64_t)cu_count();
+  // Two workgroups of either kernel fit a CU.  With few rows, twice as many items as that: chunks
+  // end unevenly, and the next one takes the place (4 x 1 token over 128k keys 178 us, with one
+  // round of items 205 us, with three 195 us).  With many rows the parts that are joined are
+  // larger, and one round is better (509 tokens behind 30k, D 64: 112 us either way, the join 8 us
+  // against 14).
+  const int64_t want = (w.few ? 4 : 2) * (int64_t)cu_count();
   w.target = (want + a->Hk - 1) / a->Hk;
-  w.chunk_min = w.few ? 4 : 8;
+  w.chunk_min = 4;
   const int64_t cap = a->table_width * a->block_size;
   w.split = cap > (int64_t)w.chunk_min * KT && (all_rows / w.M) * a->Hk < 2 * want;
   w.items = tiles + (w.split ? w.target : 0);
@@ -1018,7 +1024,7 @@ int check(const mi355_paged_attn_args* a) {
 
 template <int D>
 int launch(const PagedParams& p, const Plan& w, hipStream_t st) {
-  const dim3 grid((unsigned)(w.items * p.Hk));
+  const dim3 grid((unsigned)((w.few ? (w.items + 7) / 8 * 8 : w.items) * p.Hk));
   if (w.few == 1) {
     hipLaunchKernelGGL((paged_few_rows_kernel<D, 1>), grid, dim3(256), 0, st, p);
   } else if (w.few == 2) {
