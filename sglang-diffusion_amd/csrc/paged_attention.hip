@@ -17,7 +17,6 @@
 // sequences, from that takes the length of a chunk that makes about as many items as the chip
 // holds workgroups, and finds its own item.  Chunks of one row tile are joined by a second kernel.
 #include <atomic>
-#include <type_traits>
 
 #include "common.h"
 
@@ -32,7 +31,7 @@ typedef int i32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int KT = 64;               // keys of a tile
 constexpr float M_EMPTY = -1e30f;    // reference of a row without weight, among those that have some
-constexpr float LAZY_SUM = 8192.f;   // a lane's sum of a tile's exponentials up to which m stays
+constexpr float LAZY = 13.f;         // largest exponent against a reference that need not move: 2^13
 
 struct PagedParams {
   const unsigned short* q;
@@ -377,6 +376,14 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
     const int64_t at = (int64_t)now.block * p.Hk + hk;
     sc = scales_of(p, p.ks[at], p.vs[at]);
   }
+  // the queries are here before the loop begins: waited for inside it, they would hold up the loads
+  // of the next tile with them at every turn
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+    for (int h2 = 0; h2 < NH; ++h2)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) asm volatile("" : "+v"(qf[rt][h2][u]));
   for (; t < job.t1; t += 4) {
     const bool more = t + 4 < job.t1;
     const int key0 = t * KT;
@@ -428,9 +435,9 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
     f16x8 pf[RT][2];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      // exponents against the reference as it stands, x, and their exponentials; the reference moves
-      // (move_reference) only where a lane's sum asks for it, or a row has had no weight yet
-      float x[4][4], e[4][4], sum[4];
+      // exponents against the reference as it stands; it moves (move_reference), and O and l with
+      // it, only where one of them is too large for a half, or a row has had no weight yet
+      float x[4][4], sum[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const float add = sc.v_log[c] - m[rt];
@@ -444,22 +451,12 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
           for (int i = 0; i < 4; ++i)
             x[c][i] = sees((now.ok >> c) & 1, key0 + 16 * c + 4 * g + i, see_lo[rt], see_hi[rt]) ? x[c][i] : -INFINITY;
       }
-      auto exponentials = [&]() {
+      float top = x[0][0];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < 4; ++c)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) e[c][i] = __builtin_amdgcn_exp2f(x[c][i]);
-          sum[c] = (e[c][0] + e[c][1]) + (e[c][2] + e[c][3]);
-        }
-        return (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      };
-      const float all = exponentials();
-      if (__builtin_amdgcn_ballot_w64(!(all <= LAZY_SUM) || l[rt] == 0.f) != 0) {
-        float top = x[0][0];
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) top = fmaxf(top, x[c][i]);
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, x[c][i]);
+      if (__builtin_amdgcn_ballot_w64(top > LAZY || l[rt] == 0.f) != 0) {
         float mass = l[rt];
 #pragma unroll
         for (int w = 16; w < 64; w <<= 1) {
@@ -475,14 +472,19 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
         for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int i = 0; i < 4; ++i) x[c][i] -= mv.by;
-        (void)exponentials();
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[c][i] = __builtin_amdgcn_exp2f(x[c][i]);
+        sum[c] = (x[c][0] + x[c][1]) + (x[c][2] + x[c][3]);
       }
 #pragma unroll
       for (int c = 0; c < 4; ++c) l[rt] = fmaf(sum[c], sc.v_inv[c], l[rt]);
 #pragma unroll
       for (int c = 0; c < 4; ++c)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) pf[rt][c >> 1][4 * (c & 1) + i] = (_Float16)e[c][i];
+        for (int i = 0; i < 4; ++i) pf[rt][c >> 1][4 * (c & 1) + i] = (_Float16)x[c][i];
     }
 #pragma unroll
     for (int d = 0; d < DB; ++d)
@@ -497,11 +499,10 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
       }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    if (more) {
-      now = next;
-      next = resolve(p, job, t + 8, entry);
-      sc = scales_of(p, ks, vs);
-    }
+    if (!more) break;  // (so that whatever was loaded has been used before the next turn)
+    now = next;
+    next = resolve(p, job, t + 8, entry);
+    sc = scales_of(p, ks, vs);
   }
   if (nan_values) {  // poison: the NaN among the values of tiles seen in part, for the rows that see them
     for (t = job.t0 + wave; t < job.t1; t += 4) {
@@ -594,7 +595,7 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
 template <int D, int NW>
 __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedParams p) {
   constexpr int M = 32 * NW, ROWB = 2 * D, CPR = ROWB / 16, KSTEPS = D / 16, DVB = D / 32;
-  constexpr int TILE = KT * ROWB, LOADS = KT * D / 16 / (NW * 64);
+  constexpr int TILE = KT * ROWB, LOADS = KT * D / 16 / (NW * 32);
   static_assert(LOADS >= 1, "every thread loads");
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   __shared__ int nan_values;
@@ -621,18 +622,21 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedP
     for (int s = 0; s < KSTEPS; ++s) qf[s] = *reinterpret_cast<const bf16x8*>(qp + 16 * s + 8 * hh);
   }
 
-  u32x4 kr[LOADS], vr[LOADS];
-  const unsigned char *k_head = p.kc + hk * p.kc_sh, *v_head = p.vc + hk * p.vc_sh;
-  // thread's 16 bytes of a tile: key (i * threads + tid) / (D / 16), all keys of a wave in one piece
-  const int my_c = tid % (D / 16), my_key = tid / (D / 16);
+  // One half of the waves stages keys, the other values: 16 bytes of a key (or value) for each
+  // thread and load, all of a wave in one piece.
+  const bool loads_v = wave >= NW / 2;
+  const unsigned char* head_at = loads_v ? p.vc + hk * p.vc_sh : p.kc + hk * p.kc_sh;
+  const int64_t my_sb = loads_v ? p.vc_sb : p.kc_sb;
+  const int my_st = loads_v ? p.vc_st : p.kc_st;
+  const int my_c = tid % (D / 16), my_key = (tid % (NW * 32)) / (D / 16);
+  constexpr int KEYS = NW * 32 * 16 / D;  // keys of one load of all these threads
+  u32x4 raw[LOADS];
   auto load = [&](const Ahead& a, int t) {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int key = i * (NW * 64 * 16 / D) + my_key, c = __builtin_amdgcn_readfirstlane(key >> 4);
-      kr[i] = *reinterpret_cast<const u32x4*>(piece_at(p, k_head, p.kc_sb, p.kc_st, a, t, c) +
-                                              (unsigned)((key & 15) * p.kc_st + 16 * my_c));
-      vr[i] = *reinterpret_cast<const u32x4*>(piece_at(p, v_head, p.vc_sb, p.vc_st, a, t, c) +
-                                              (unsigned)((key & 15) * p.vc_st + 16 * my_c));
+      const int key = i * KEYS + my_key, c = __builtin_amdgcn_readfirstlane(key >> 4);
+      raw[i] = *reinterpret_cast<const u32x4*>(piece_at(p, head_at, my_sb, my_st, a, t, c) +
+                                               (unsigned)((key & 15) * my_st + 16 * my_c));
     }
   };
   // does some row of the workgroup not see some key of the tile?
@@ -641,26 +645,34 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedP
            (p.window >= 0 && t * KT < job.place_hi - p.window);
   };
   auto store = [&](const Ahead& a, int t, int buf) {
+    if (!loads_v) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int key = i * KEYS + my_key;
+        unsigned char* to = smem + buf * 2 * TILE + key * ROWB;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          *reinterpret_cast<bf16x8*>(to + (((2 * my_c + h) ^ k_swz(key)) << 4)) = widen_bf16(raw[i][2 * h], raw[i][2 * h + 1]);
+      }
+      return;
+    }
     if (in_part(t, a.ok)) {
       unsigned any = 0;
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
-        const int key = i * (NW * 64 * 16 / D) + my_key;
-        if (!((a.ok >> (key >> 4)) & 1) || t * KT + key >= job.s.len) vr[i] = u32x4{0, 0, 0, 0};
-        any |= clear_nan(vr[i]);
+        const int key = i * KEYS + my_key;
+        if (!((a.ok >> (key >> 4)) & 1) || t * KT + key >= job.s.len) raw[i] = u32x4{0, 0, 0, 0};
+        any |= clear_nan(raw[i]);
       }
       if (any) nan_values = 1;
     }
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int key = i * (NW * 64 * 16 / D) + my_key;
-      unsigned char* kt = smem + buf * 2 * TILE + key * ROWB;
-      unsigned char* vt = kt + TILE;
+      const int key = i * KEYS + my_key;
+      unsigned char* to = smem + buf * 2 * TILE + TILE + key * ROWB;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        *reinterpret_cast<bf16x8*>(kt + (((2 * my_c + h) ^ k_swz(key)) << 4)) = widen_bf16(kr[i][2 * h], kr[i][2 * h + 1]);
-        *reinterpret_cast<f16x8*>(vt + (((2 * my_c + h) ^ v_swz(key)) << 4)) = widen_f16(vr[i][2 * h], vr[i][2 * h + 1]);
-      }
+      for (int h = 0; h < 2; ++h)
+        *reinterpret_cast<f16x8*>(to + (((2 * my_c + h) ^ v_swz(key)) << 4)) = widen_f16(raw[i][2 * h], raw[i][2 * h + 1]);
     }
   };
 
@@ -697,8 +709,11 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedP
     store(now, job.t0, 0);
   }
   const bool live_wave = job.row0 + 32 * wave < job.rows;
-  auto tile = [&](auto bufc, int t) {
-    constexpr int buf = decltype(bufc)::value;
+  // the queries are here before the loop begins: waited for inside it, they would hold up the loads
+  // of the next tile with them at every turn
+#pragma unroll
+  for (int s = 0; s < KSTEPS; ++s) asm volatile("" : "+v"(qf[s]));
+  for (int t = job.t0, buf = 0; t < job.t1; ++t, buf ^= 1) {
     const int key0 = t * KT;
     __syncthreads();
     const bool more = t + 1 < job.t1;
@@ -732,7 +747,7 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedP
       const bool masked = key0 + KT > job.s.len || now.ok != 15u || (p.causal && key0 + KT - 1 > w_lo) ||
                           (p.window >= 0 && key0 < w_hi - p.window);
       // as in the kernel above: x[c][e] is element e of piece c
-      float x[4][8], pe[4][8], sum[4];
+      float x[4][8], sum[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const float add = sc.v_log[c] - m;
@@ -747,25 +762,12 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedP
             x[c][e] = sees((now.ok >> c) & 1, key0 + 16 * c + (e & 3) + 8 * (e >> 2) + 4 * hh, see_lo, see_hi)
                           ? x[c][e] : -INFINITY;
       }
-      auto exponentials = [&]() {
+      float top = x[0][0];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          sum[c] = 0.f;
+      for (int c = 0; c < 4; ++c)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            pe[c][e] = __builtin_amdgcn_exp2f(x[c][e]);
-            sum[c] += pe[c][e];
-          }
-        }
-        return (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      };
-      const float all = exponentials();
-      if (__builtin_amdgcn_ballot_w64(!(all <= LAZY_SUM) || l == 0.f) != 0) {
-        float top = x[0][0];
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) top = fmaxf(top, x[c][e]);
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, x[c][e]);
+      if (__builtin_amdgcn_ballot_w64(top > LAZY || l == 0.f) != 0) {
         const Move mv = move_reference(fmaxf(top, __shfl_xor(top, 32, 64)), l + __shfl_xor(l, 32, 64));
         m += mv.by;
         l *= mv.shrink;
@@ -777,7 +779,15 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedP
         for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[c][e] -= mv.by;
-        (void)exponentials();
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        sum[c] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[c][e] = __builtin_amdgcn_exp2f(x[c][e]);
+          sum[c] += x[c][e];
+        }
       }
 #pragma unroll
       for (int c = 0; c < 4; ++c) l = fmaf(sum[c], sc.v_inv[c], l);
@@ -787,7 +797,7 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedP
 #pragma unroll
         for (int st = 0; st < 2; ++st)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) pf[kb][st][j] = (_Float16)pe[2 * kb + st][j];
+          for (int j = 0; j < 8; ++j) pf[kb][st][j] = (_Float16)x[2 * kb + st][j];
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -803,16 +813,11 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedP
                                                           pf[kb][st], o[d], 0, 0, 0);
           }
     }
-    if (more) {
-      store(next, t + 1, buf ^ 1);
-      now = next;
-      next = resolve(p, job, t + 2, entry);
-      sc = scales_of(p, ks, vs);
-    }
-  };
-  for (int t = job.t0; t < job.t1; t += 2) {
-    tile(std::integral_constant<int, 0>{}, t);
-    if (t + 1 < job.t1) tile(std::integral_constant<int, 1>{}, t + 1);
+    if (!more) break;  // (so that whatever was loaded has been used before the next turn)
+    store(next, t + 1, buf ^ 1);
+    now = next;
+    next = resolve(p, job, t + 2, entry);
+    sc = scales_of(p, ks, vs);
   }
   __syncthreads();
   if (nan_values) {  // poison, as above
@@ -822,7 +827,7 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedP
       for (int k = 0; k < KT; ++k) {
         const int key = t * KT + k;
         if (!((now.ok >> (k >> 4)) & 1) || key >= job.s.len) continue;
-        const unsigned char* at = piece_at(p, v_head, p.vc_sb, p.vc_st, now, t, k >> 4) + (k & 15) * p.vc_st + 4 * hh;
+        const unsigned char* at = piece_at(p, p.vc + hk * p.vc_sh, p.vc_sb, p.vc_st, now, t, k >> 4) + (k & 15) * p.vc_st + 4 * hh;
         const unsigned seen = (unsigned)sees(true, key, see_lo, see_hi);
 #pragma unroll
         for (int d = 0; d < DVB; ++d)
