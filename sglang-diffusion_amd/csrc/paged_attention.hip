@@ -208,12 +208,17 @@ __device__ __forceinline__ Ahead resolve(const PagedParams& p, const Job& j, int
                   (int)(entry < p.num_blocks);
   return Ahead{ok ? entry : 0, (unsigned)__builtin_amdgcn_ballot_w64(ok) & 15u};
 }
-// the first byte of a piece (wave-uniform)
-__device__ __forceinline__ const unsigned char* piece_at(const PagedParams& p, const unsigned char* head, int64_t sb,
-                                                         int st, const Ahead& a, int t, int c) {
-  const int block = __builtin_amdgcn_readlane(a.block, c);
-  const int off = (a.ok >> c) & 1 ? (t * KT + 16 * c) & ((1 << p.lb) - 1) : 0;
-  return head + (block * sb + (int64_t)off * st);
+// Where the pieces begin, in bytes behind the head's first: lane c holds piece c's, formed for all
+// four at once, and piece_at hands one to the scalar unit.
+__device__ __forceinline__ int64_t piece_offsets(const PagedParams& p, const Ahead& a, int t, int64_t sb, int st) {
+  const int key = t * KT + 16 * (int)(threadIdx.x & 3);
+  const bool ok = (a.ok >> (threadIdx.x & 3)) & 1;
+  return a.block * sb + (int64_t)(ok ? key & ((1 << p.lb) - 1) : 0) * st;
+}
+__device__ __forceinline__ const unsigned char* piece_at(const unsigned char* head, int64_t offsets, int c) {
+  const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)offsets, c);
+  const unsigned hi = (unsigned)__builtin_amdgcn_readlane((int)(offsets >> 32), c);
+  return head + (int64_t)(((uint64_t)hi << 32) | lo);
 }
 // scales of a tile's pieces: factor of the score, addend of the exponent, weight in the row sum
 struct Scales {
@@ -336,18 +341,20 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
   const unsigned k_lane = (unsigned)((lane / CPR) * p.kc_st + (lane % CPR) * 16);
   const unsigned v_lane = (unsigned)((lane / CPR) * p.vc_st + (lane % CPR) * 16);
   auto load_k = [&](const Ahead& a, int t) {
+    const int64_t offsets = piece_offsets(p, a, t, p.kc_sb, p.kc_st);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const unsigned char* at = piece_at(p, k_head, p.kc_sb, p.kc_st, a, t, c);
+      const unsigned char* at = piece_at(k_head, offsets, c);
 #pragma unroll
       for (int i = 0; i < CPR / 4; ++i)
         kr[c * CPR / 4 + i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at + (k_lane + (unsigned)(i * (64 / CPR) * p.kc_st))));
     }
   };
   auto load_v = [&](const Ahead& a, int t) {
+    const int64_t offsets = piece_offsets(p, a, t, p.vc_sb, p.vc_st);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const unsigned char* at = piece_at(p, v_head, p.vc_sb, p.vc_st, a, t, c);
+      const unsigned char* at = piece_at(v_head, offsets, c);
 #pragma unroll
       for (int i = 0; i < CPR / 4; ++i)  // 64 / CPR rows at a time
         vr[c * CPR / 4 + i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at + (v_lane + (unsigned)(i * (64 / CPR) * p.vc_st))));
@@ -508,10 +515,11 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
     for (t = job.t0 + wave; t < job.t1; t += 4) {
       now = resolve(p, job, t, load_entry(p, job, t));
       if (!in_part(t, now.ok)) continue;
+      const int64_t offsets = piece_offsets(p, now, t, p.vc_sb, p.vc_st);
       for (int k = 0; k < KT; ++k) {
         const int key = t * KT + k;
         if (!((now.ok >> (k >> 4)) & 1) || key >= job.s.len) continue;
-        const unsigned char* at = piece_at(p, v_head, p.vc_sb, p.vc_st, now, t, k >> 4) + (k & 15) * p.vc_st;
+        const unsigned char* at = piece_at(v_head, offsets, k >> 4) + (k & 15) * p.vc_st;
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
           const unsigned n = nan_codes(*reinterpret_cast<const unsigned*>(at + 16 * d + 4 * g));
@@ -632,11 +640,11 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedP
   constexpr int KEYS = NW * 32 * 16 / D;  // keys of one load of all these threads
   u32x4 raw[LOADS];
   auto load = [&](const Ahead& a, int t) {
+    const int64_t offsets = piece_offsets(p, a, t, my_sb, my_st);
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       const int key = i * KEYS + my_key, c = __builtin_amdgcn_readfirstlane(key >> 4);
-      raw[i] = *reinterpret_cast<const u32x4*>(piece_at(p, head_at, my_sb, my_st, a, t, c) +
-                                               (unsigned)((key & 15) * my_st + 16 * my_c));
+      raw[i] = *reinterpret_cast<const u32x4*>(piece_at(head_at, offsets, c) + (unsigned)((key & 15) * my_st + 16 * my_c));
     }
   };
   // does some row of the workgroup not see some key of the tile?
@@ -824,10 +832,11 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedP
     for (int t = job.t0; t < job.t1; ++t) {
       now = resolve(p, job, t, load_entry(p, job, t));
       if (!in_part(t, now.ok)) continue;
+      const int64_t offsets = piece_offsets(p, now, t, p.vc_sb, p.vc_st);
       for (int k = 0; k < KT; ++k) {
         const int key = t * KT + k;
         if (!((now.ok >> (k >> 4)) & 1) || key >= job.s.len) continue;
-        const unsigned char* at = piece_at(p, p.vc + hk * p.vc_sh, p.vc_sb, p.vc_st, now, t, k >> 4) + (k & 15) * p.vc_st + 4 * hh;
+        const unsigned char* at = piece_at(p.vc + hk * p.vc_sh, offsets, k >> 4) + (k & 15) * p.vc_st + 4 * hh;
         const unsigned seen = (unsigned)sees(true, key, see_lo, see_hi);
 #pragma unroll
         for (int d = 0; d < DVB; ++d)
