@@ -132,27 +132,37 @@ struct Rope {
   const int64_t* positions;
   const void* inv_freq;  // [half], fp64 or fp32
   int f64, half, neox;
-  float factor;
+  double factor;
 };
 
-// cos and sin of position * frequency, times the factor.  The product is formed in turns and in
-// fp64 (a position of 10^6 leaves fp32 0.06 rad of it), reduced exactly to an eighth of a turn
-// on either side of the nearest quarter, and evaluated by the Taylor sums up to the terms that
-// stay below 2e-9.
-__device__ __forceinline__ float2 rope_cos_sin(const Rope& r, int64_t pos, int i) {
-  const double w = r.f64 ? reinterpret_cast<const double*>(r.inv_freq)[i]
-                         : (double)reinterpret_cast<const float*>(r.inv_freq)[i];
-  const double quarters = (double)pos * (w * 0.63661977236758134308);  // 2 / pi
+// cos and sin of position * frequency, times the factor.  The product is formed in quarter turns
+// and in fp64 (a position of 10^6 leaves fp32 0.06 rad of it), reduced exactly to an eighth of a
+// turn on either side of the nearest quarter, and evaluated there by the Taylor sums, in fp64 up to
+// the terms that stay below 10^-11: rounded to fp32 they are as good as correctly rounded.  That is
+// some twenty fp64 operations for a pair of a token, shared by all its heads (or by a block's rows).
+__device__ __forceinline__ double rope_quarters(const Rope& r, int i) {  // turned for each position, in quarters
+  return (r.f64 ? reinterpret_cast<const double*>(r.inv_freq)[i]
+                : (double)reinterpret_cast<const float*>(r.inv_freq)[i]) * 0.63661977236758134308;  // 2 / pi
+}
+__device__ __forceinline__ float2 rope_cos_sin(const Rope& r, int64_t pos, double each) {
+  const double quarters = (double)pos * each;
   const double whole = rint(quarters);
-  const float a = (float)((quarters - whole) * 1.57079632679489661923);
+  const double a = (quarters - whole) * 1.57079632679489661923, a2 = a * a;
   const int quadrant = (int)(whole - 4.0 * floor(whole * 0.25));
-  const float a2 = a * a;
-  const float s = a + a * a2 * fmaf(a2, fmaf(a2, fmaf(a2, 2.7557319e-6f, -1.9841270e-4f), 8.3333333e-3f), -0.16666667f);
-  const float c = 1.f + a2 * fmaf(a2, fmaf(a2, fmaf(a2, fmaf(a2, -2.7557319e-7f, 2.4801587e-5f), -1.3888889e-3f),
-                                           4.1666667e-2f), -0.5f);
-  const float cq = quadrant & 1 ? s : c, sq = quadrant & 1 ? c : s;
-  return make_float2((quadrant == 1 || quadrant == 2 ? -cq : cq) * r.factor,
-                     (quadrant >= 2 ? -sq : sq) * r.factor);
+  double s = fma(a2, -1.0 / 39916800.0, 1.0 / 362880.0);
+  s = fma(a2, s, -1.0 / 5040.0);
+  s = fma(a2, s, 1.0 / 120.0);
+  s = fma(a2, s, -1.0 / 6.0);
+  s = fma(a2 * a, s, a);
+  double c = fma(a2, 1.0 / 479001600.0, -1.0 / 3628800.0);
+  c = fma(a2, c, 1.0 / 40320.0);
+  c = fma(a2, c, -1.0 / 720.0);
+  c = fma(a2, c, 1.0 / 24.0);
+  c = fma(a2, c, -0.5);
+  c = fma(a2, c, 1.0);
+  const double cq = quadrant & 1 ? s : c, sq = quadrant & 1 ? c : s;
+  return make_float2((float)((quadrant == 1 || quadrant == 2 ? -cq : cq) * r.factor),
+                     (float)((quadrant >= 2 ? -sq : sq) * r.factor));
 }
 
 __device__ __forceinline__ void unpack8(u32x4 v, float (&f)[8]) {
@@ -215,7 +225,7 @@ __device__ __forceinline__ void rope_tokens(const Rope& r, const RopeRows& a, co
                                             int64_t t0, int nt, float2* cs) {
   for (int i = threadIdx.x; i < nt * r.half; i += ROPE_THREADS) {
     const int k = i / r.half;
-    cs[i] = rope_cos_sin(r, r.positions[t0 + k], i - k * r.half);
+    cs[i] = rope_cos_sin(r, r.positions[t0 + k], rope_quarters(r, i - k * r.half));
   }
   __syncthreads();
   const int turned = r.neox ? r.half / 8 : r.half / 4;
@@ -243,10 +253,12 @@ __global__ __launch_bounds__(ROPE_THREADS) void rope_scaled_kernel(Rope r, RopeR
 inline int rope_group(int64_t tokens) { return tokens >= 8192 ? ROPE_MAX_TOKENS : 1; }
 
 // ----------------------------------------------------------------------------------- store --
-// A wave owns one run: the tokens of a call that follow each other into one block, for one head
-// and one of the two caches.  The wave whose token begins a run (the token before it goes to
-// another block) takes it, so no two waves write one block's scale.  A row of D elements is held
-// by D / 8 lanes, 64 / (D / 8) rows at a time.
+// A workgroup owns one run: the tokens of a call that follow each other into one block, for one
+// head and one of the two caches.  The workgroup whose token begins a run (the token before it
+// goes to another block) takes it, so no two of them write one block's scale.  A row of D elements
+// is held by D / 8 lanes, and the 256 threads hold HELD such sets of rows in registers between the
+// maximum and the rounding; longer runs are read a second time.  Cosines and sines of these rows
+// are formed together and handed on through LDS.
 struct StoreParams {
   const unsigned short *k, *v;
   int64_t k_st, k_sh, v_st, v_sh;
@@ -285,101 +297,125 @@ __device__ __forceinline__ u32x2 round_fp8(const float (&f)[8], float inv) {
   return o;
 }
 
-template <int D, bool KEYS>
-__device__ __forceinline__ void load_row(const StoreParams& p, int64_t t, int head, int c, bool live,
-                                         float (&f)[8]) {
-  constexpr int LPR = D / 8;
-  u32x4 raw = u32x4{0, 0, 0, 0};
-  if (live)
-    raw = *reinterpret_cast<const u32x4*>((KEYS ? p.k + t * p.k_st + head * p.k_sh
-                                                : p.v + t * p.v_st + head * p.v_sh) + 8 * c);
-  unpack8(raw, f);
-  if constexpr (KEYS) {
-    if (p.rope.positions) {
-      const Rope& r = p.rope;
-      const bool mine = 8 * c < 2 * r.half;
-      const int64_t pos = live ? p.rope.positions[t] : 0;
+// HELD sets: of 16 rows of 128, or 32 of 64
+template <int D, int HELD>
+struct StoreLds {
+  static constexpr int ROWS = 256 / (D / 8);  // of a set
+  float2 cs[HELD * ROWS][D / 2];
+  float top[4];
+  int first[4];
+};
+
+template <int D, int HELD, bool KEYS>
+__device__ void store_run(const StoreParams& p, int64_t t0, int64_t len, int64_t block, int head,
+                          StoreLds<D, HELD>& lds) {
+  constexpr int LPR = D / 8, ROWS = StoreLds<D, HELD>::ROWS, CHUNK = HELD * ROWS;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = threadIdx.x % LPR, sub = threadIdx.x / LPR;
+  const int bs = 1 << p.lb;
+  const Rope& r = p.rope;
+  const bool turned = KEYS && r.positions;
+  float* scale_at = (KEYS ? p.k_scale : p.v_scale) + block * p.Hk + head;
+  const float old = *scale_at;
+  u32x4 held[HELD];
+  int place[HELD];  // in the block; bs: no row
+  // CHUNK rows of the run, keys rotated.  The rotated key is a bf16 value before it is rounded to 8
+  // bits, as it would be between the rotary operator and the store.
+  auto fetch = [&](int64_t row0) {
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+      const int64_t row = row0 + h * ROWS + sub, t = t0 + row;
+      held[h] = u32x4{0, 0, 0, 0};
+      place[h] = bs;
+      if (row < len) {
+        held[h] = *reinterpret_cast<const u32x4*>((KEYS ? p.k + t * p.k_st + head * p.k_sh
+                                                        : p.v + t * p.v_st + head * p.v_sh) + 8 * c);
+        place[h] = (int)(p.slots[t] & (bs - 1));
+      }
+    }
+    if (!turned) return;
+    const int rows = (int)min((int64_t)CHUNK, len - row0);
+    __syncthreads();  // what was here before has been read
+    // a lane keeps its pair, and goes over the rows
+    const int side = 64 / r.half, pair = lane % r.half, k0 = wave * side + lane / r.half;
+    if (lane < side * r.half) {
+      const double each = rope_quarters(r, pair);
+#pragma unroll 4
+      for (int k = k0; k < rows; k += 4 * side) lds.cs[k][pair] = rope_cos_sin(r, r.positions[t0 + row0 + k], each);
+    }
+    __syncthreads();
+    const bool mine = 8 * c < 2 * r.half;
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+      float f[8];
+      unpack8(held[h], f);
+      const float2* cs = lds.cs[h * ROWS + sub];
       if (r.neox) {
-        // the other element of each pair is `half` away: `half / 8` lanes, in the same row
+        // the other element of each pair is `half` away: half / 8 lanes, in the same row and wave
         const int away = r.half / 8;
         const bool second = c >= away;
-        const int lane = threadIdx.x & 63;
         const int from = mine ? (second ? lane - away : lane + away) : lane;
         u32x4 other;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) other[j] = __shfl(raw[j], from, 64);
+        for (int j = 0; j < 4; ++j) other[j] = __shfl(held[h][j], from, 64);
         float g[8];
         unpack8(other, g);
-        if (mine) {
+        if (mine && place[h] < bs) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const float2 cs = rope_cos_sin(r, pos, (second ? c - away : c) * 8 + j);
-            if (second) turn(g[j], f[j], cs);
-            else turn(f[j], g[j], cs);
+            const float2 w = cs[(second ? c - away : c) * 8 + j];
+            if (second) turn(g[j], f[j], w);
+            else turn(f[j], g[j], w);
           }
         }
-      } else if (mine) {
+      } else if (mine && place[h] < bs) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) turn(f[2 * j], f[2 * j + 1], rope_cos_sin(r, pos, c * 4 + j));
+        for (int j = 0; j < 4; ++j) turn(f[2 * j], f[2 * j + 1], cs[c * 4 + j]);
       }
-      // the rotated key is a bf16 value before it is rounded to 8 bits, as it would be between
-      // the rotary operator and the store
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = rbf(f[j]);
+      held[h] = pack8(f);
     }
-  }
-  static_assert(64 % LPR == 0, "rows of a wave");
-}
-
-template <int D, bool KEYS>
-__device__ void store_run(const StoreParams& p, int64_t t0, int64_t block, int head) {
-  constexpr int LPR = D / 8, RPI = 64 / LPR;
-  const int lane = threadIdx.x & 63, c = lane % LPR, sub = lane / LPR;
-  const int bs = 1 << p.lb;
-  // length of the run, the largest finite magnitude, the smallest place in the block
-  int64_t len = 0;
-  for (;;) {
-    const int64_t t = t0 + len + lane;
-    const int64_t s = t < p.tokens ? p.slots[t] : -1;
-    const unsigned long long out = __ballot(s < 0 || (s >> p.lb) != block);
-    if (out) {
-      len += __ffsll((unsigned long long)out) - 1;
-      break;
-    }
-    len += 64;
-  }
+  };
+  // the largest finite magnitude and the smallest place in the block
   float top = 0.f;
   int first = bs;
-  for (int64_t i = 0; i < len; i += RPI) {
-    const bool live = i + sub < len;
-    const int64_t t = t0 + (live ? i + sub : 0);
-    float f[8];
-    load_row<D, KEYS>(p, t, head, c, live, f);
-    if (live) {
-      first = min(first, (int)(p.slots[t] & (bs - 1)));
+  for (int64_t row0 = 0; row0 < len; row0 += CHUNK) {
+    fetch(row0);
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+      float f[8];
+      unpack8(held[h], f);
+      first = min(first, place[h]);
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (finite(f[j])) top = fmaxf(top, fabsf(f[j]));
+        if (finite(f[j])) top = fmaxf(top, fabsf(f[j]));  // rows behind the run are zeros
     }
   }
   top = group_max<64>(top);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) first = min(first, __shfl_xor(first, o, 64));
+  __syncthreads();  // the run before has been read, and every thread has the old scale
+  if (lane == 0) {
+    lds.top[wave] = top;
+    lds.first[wave] = first;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    top = fmaxf(top, lds.top[w]);
+    first = min(first, lds.first[w]);
+  }
   // the smallest power of two with top <= 448 * 2^e: 448 = 1.75 * 2^8
   const unsigned bits = __float_as_uint(top);
   const int e = max(SCALE_EXP_MIN, (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0));
   float scale = __uint_as_float((unsigned)(e + 127) << 23);
-  float* scale_at = (KEYS ? p.k_scale : p.v_scale) + block * p.Hk + head;
   unsigned char* cache = (KEYS ? p.k_cache : p.v_cache) + block * (KEYS ? p.kc_sb : p.vc_sb) +
                          head * (KEYS ? p.kc_sh : p.vc_sh) + 8 * c;
   const int64_t row_bytes = KEYS ? p.kc_st : p.vc_st;
   if (first > 0) {
-    const float old = *scale_at;
     if (old >= scale) {
       scale = old;
     } else if (old > 0.f) {  // the block's earlier tokens to the larger step
       const float shrink = old / scale;
-      for (int i = sub; i < first; i += RPI) {
+      for (int i = sub; i < first; i += ROWS) {
         u32x2* at = reinterpret_cast<u32x2*>(cache + i * row_bytes);
         const u32x2 w = *at;
         u32x2 n;
@@ -387,62 +423,68 @@ __device__ void store_run(const StoreParams& p, int64_t t0, int64_t block, int h
         for (int h = 0; h < 2; ++h) {
           const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w[h], false);
           const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(w[h], true);
-          unsigned nan = 0;
+          unsigned nan = 0;  // NaN stays NaN
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (((w[h] >> (8 * j)) & 0x7f) == 0x7f) nan |= 0x7fu << (8 * j);
-          n[h] = cvt4_fp8(lo[0] * shrink, lo[1] * shrink, hi[0] * shrink, hi[1] * shrink);
-          unsigned keep = 0;
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if ((nan >> (8 * j)) & 0x7f) keep |= 0xffu << (8 * j);
-          n[h] = (n[h] & ~keep) | nan;
+            if (((w[h] >> (8 * j)) & 0x7f) == 0x7f) nan |= 0xffu << (8 * j);
+          n[h] = (cvt4_fp8(lo[0] * shrink, lo[1] * shrink, hi[0] * shrink, hi[1] * shrink) & ~nan) | (nan & 0x7f7f7f7fu);
         }
         *at = n;
       }
     }
   }
-  if (lane == 0) *scale_at = scale;
+  if (threadIdx.x == 0) *scale_at = scale;
   const float inv = 1.f / scale;  // exact: a power of two (a scale that a caller set may be any)
-  for (int64_t i = 0; i < len; i += RPI) {
-    const bool live = i + sub < len;
-    const int64_t t = t0 + (live ? i + sub : 0);
-    float f[8];
-    load_row<D, KEYS>(p, t, head, c, live, f);
-    if (live)
-      *reinterpret_cast<u32x2*>(cache + (p.slots[t] & (bs - 1)) * row_bytes) = round_fp8(f, inv);
+  for (int64_t row0 = 0; row0 < len; row0 += CHUNK) {
+    if (len > CHUNK) fetch(row0);
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+      float f[8];
+      unpack8(held[h], f);
+      if (place[h] < bs) *reinterpret_cast<u32x2*>(cache + place[h] * row_bytes) = round_fp8(f, inv);
+    }
   }
 }
 
-template <int D>
-__global__ __launch_bounds__(256) void kv_store_kernel(StoreParams p) {
-  __shared__ float2 cs[ROPE_MAX_HALF * ROPE_MAX_TOKENS];
+template <int D, int HELD>
+__global__ __launch_bounds__(256, 4) void kv_store_kernel(StoreParams p) {
+  __shared__ union {
+    float2 q[ROPE_MAX_HALF * ROPE_MAX_TOKENS];
+    StoreLds<D, HELD> kv;
+  } lds;
   if (blockIdx.x >= p.kv_groups) {
     const int64_t t0 = (int64_t)(blockIdx.x - p.kv_groups) * p.q_group;
     rope_tokens(p.rope, p.q, RopeRows{nullptr, nullptr, 0, 0, 0, 0, 0}, D, t0,
-                (int)min((int64_t)p.q_group, p.tokens - t0), cs);
+                (int)min((int64_t)p.q_group, p.tokens - t0), lds.q);
     return;
   }
-  // a wave: (group of tokens, head, keys or values)
-  const int64_t unit = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  const int64_t which = unit % (2 * p.Hk), g = unit / (2 * p.Hk);
+  // a workgroup: (group of tokens, head, keys or values); each wave finds the runs that begin there
+  const unsigned which = blockIdx.x % (2 * p.Hk);
+  const int64_t g = blockIdx.x / (2 * p.Hk);
   const int head = (int)(which >> 1);
-  const int64_t t = g * p.group + lane;
+  const int lane = threadIdx.x & 63;
+  const int64_t w0 = g * p.group, t = w0 + lane;  // 64 slots: the group's and those behind it
   const int64_t limit = p.num_blocks << p.lb;
-  int64_t s = -1, before = -1;
-  if (lane < p.group && t < p.tokens) {
-    s = p.slots[t];
-    if (t > 0) before = p.slots[t - 1];
-  }
-  const bool leads = s >= 0 && s < limit && (before < 0 || (before >> p.lb) != (s >> p.lb));
-  unsigned long long todo = __ballot(leads);
+  const int64_t s = t < p.tokens ? p.slots[t] : -1;
+  const int64_t before = t > 0 && t < p.tokens ? p.slots[t - 1] : -1;
+  const int64_t block = s < 0 ? -1 : s >> p.lb;
+  unsigned long long todo =
+      __ballot(lane < p.group && s >= 0 && s < limit && (before < 0 || (before >> p.lb) != block));
   while (todo) {
     const int l = __ffsll(todo) - 1;
     todo &= todo - 1;
-    const int64_t slot = p.slots[g * p.group + l];
-    if (which & 1) store_run<D, false>(p, g * p.group + l, slot >> p.lb, head);
-    else store_run<D, true>(p, g * p.group + l, slot >> p.lb, head);
+    const int64_t mine = __shfl(block, l, 64);
+    // the length of the run: to the first slot of another block, if need be behind these 64
+    int64_t len = 0;
+    unsigned long long out = __ballot(lane >= l && block != mine);
+    if (out) len = __ffsll(out) - 1 - l;
+    for (int64_t at = w0 + 64; !out; at += 64) {
+      const int64_t s2 = at + lane < p.tokens ? p.slots[at + lane] : -1;
+      out = __ballot(s2 < 0 || (s2 >> p.lb) != mine);
+      len = at - w0 - l + (out ? __ffsll(out) - 1 : 0);
+    }
+    if (which & 1) store_run<D, HELD, false>(p, w0 + l, len, mine, head, lds.kv);
+    else store_run<D, HELD, true>(p, w0 + l, len, mine, head, lds.kv);
   }
 }
 
@@ -565,12 +607,16 @@ extern "C" int mi355_kv_store_fp8(const mi355_kv_store_args* a, void* stream) {
   p.num_blocks = a->num_blocks;
   p.Hk = (int)a->Hk;
   p.lb = log2_of(a->block_size);
-  // Tokens that a wave looks at for the beginning of a run: one while there are few tokens (each
-  // may be a request of its own, and runs that one wave finds are stored one after the other),
-  // sixteen where tokens mostly follow each other and waves without a run would only be launched.
-  p.group = a->tokens <= 2048 ? 1 : 16;
+  // Tokens that a workgroup looks at for the beginning of a run: one while there are few tokens
+  // (each may be a request of its own, and runs that one workgroup finds are stored one after the
+  // other), then as many as keep the launch to about twice the workgroups that the chip holds: most
+  // of them find no run where tokens follow each other, and take a place for the while (4602 tokens
+  // of 12 prompts, 8 heads: %GROUP%).
+  p.group = 1;
+  while (p.group < 64 && (a->tokens + p.group - 1) / p.group * 2 * a->Hk > 2048) p.group *= 2;
   const int64_t units = (a->tokens + p.group - 1) / p.group * 2 * a->Hk;
-  p.kv_groups = (unsigned)((units + 3) / 4);
+  MI355_REQUIRE(units + a->tokens < (1ll << 31), "kv_store_fp8: too many tokens and heads for one call");
+  p.kv_groups = (unsigned)units;
   p.q_group = rope_group(a->tokens);
   const unsigned q_groups = a->Hq ? (unsigned)((a->tokens + p.q_group - 1) / p.q_group) : 0;
   p.rope = Rope{a->positions, a->inv_freq, a->inv_freq_is_f64, (int)(a->rot_dim / 2), a->is_neox != 0,
@@ -578,8 +624,15 @@ extern "C" int mi355_kv_store_fp8(const mi355_kv_store_args* a, void* stream) {
   p.q = RopeRows{(const unsigned short*)a->q, (unsigned short*)a->q_out, a->q_st, a->q_sh, a->qo_st, a->qo_sh,
                  (int)a->Hq};
   const dim3 grid(p.kv_groups + q_groups), block(256);
-  if (a->D == 128) hipLaunchKernelGGL(kv_store_kernel<128>, grid, block, 0, (hipStream_t)stream, p);
-  else hipLaunchKernelGGL(kv_store_kernel<64>, grid, block, 0, (hipStream_t)stream, p);
+  // with one token to look at, runs are likely short: one set of rows, and the registers of one
+  hipStream_t st = (hipStream_t)stream;
+  if (a->D == 128) {
+    if (p.group == 1) hipLaunchKernelGGL((kv_store_kernel<128, 1>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((kv_store_kernel<128, 4>), grid, block, 0, st, p);
+  } else {
+    if (p.group == 1) hipLaunchKernelGGL((kv_store_kernel<64, 1>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((kv_store_kernel<64, 4>), grid, block, 0, st, p);
+  }
   MI355_CHECK_LAUNCH("kv_store_fp8");
   return MI355_OK;
 }

@@ -1002,12 +1002,11 @@ Plan plan_of(const mi355_paged_attn_args* a) {
   w.few = rows <= 16 ? 1 : rows <= 32 ? 2 : 0;
   w.M = w.few ? 16 * w.few : 128;
   const int64_t tiles = all_rows / w.M + a->B;  // row tiles: at most one not full for each sequence
-  // Two workgroups of either kernel fit a CU.  With few rows, twice as many items as that: chunks
-  // end unevenly, and the next one takes the place (4 x 1 token over 128k keys 178 us, with one
-  // round of items 205 us, with three 195 us).  With many rows the parts that are joined are
-  // larger, and one round is better (509 tokens behind 30k, D 64: 112 us either way, the join 8 us
-  // against 14).
-  const int64_t want = (w.few ? 4 : 2) * (int64_t)cu_count();
+  // Items to aim for.  Many rows: as many as the chip holds workgroups (two a CU, with heads of 64
+  // three: 509 tokens behind 30k keys 105 us, with two 115 us); the parts to be joined are large.
+  // Few rows: twice as many, since chunks end unevenly and the next one takes the place (4 x 1
+  // token over 128k keys 178 us, one round 205 us, three 195 us).
+  const int64_t want = (w.few ? 4 : a->D == 64 ? 3 : 2) * (int64_t)cu_count();
   w.target = (want + a->Hk - 1) / a->Hk;
   w.chunk_min = 4;
   const int64_t cap = a->table_width * a->block_size;
