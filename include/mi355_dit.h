@@ -477,7 +477,7 @@ int mi355_merge_attn_states(void* out, float* out_lse, const void* a, const floa
  *   status int32 [3]  blocks that the free list lacks, tokens beyond max_tokens, requests that
  *     outgrow table_width (counts saturate).  If any is not 0 nothing is given to anybody: the table is left as it
  *     was, seq_lens = context_lens, all slots -1, cu_seqlens_q 0, free_end = free_begin.
- * seq_lens and free_end must not be the memory of an input.  B <= 8192. */
+ * seq_lens and free_end must not be the memory of an input.  B <= 4096. */
 int mi355_kv_block_plan(const int32_t* context_lens, const int32_t* new_lens, int64_t B,
                         int32_t* block_table, int64_t table_stride, int64_t table_width,
                         const int32_t* free_blocks, int64_t num_free, const int32_t* free_begin,

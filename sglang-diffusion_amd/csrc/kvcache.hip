@@ -1,6 +1,8 @@
 // What stands around a paged 8-bit key/value cache, for gfx950: block tables and slot maps from
 // request lengths, rotary positions from scaled frequencies, and the store that rounds keys and
 // values into the cache.  The attention that reads the cache is in paged_attention.hip.
+#include <type_traits>
+
 #include "common.h"
 
 namespace {
@@ -20,7 +22,7 @@ inline int log2_of(int64_t bs) { return __builtin_ctzll((unsigned long long)bs);
 // another.  Entries of the table that a workgroup reads (blocks held before the call) and
 // entries that any workgroup writes (fresh blocks) are different ones.
 constexpr int PLAN_THREADS = 256, PLAN_TOKENS = 1024;
-constexpr int64_t PLAN_MAX_REQUESTS = 8192;  // two ints each in LDS: 64 KiB
+constexpr int64_t PLAN_MAX_REQUESTS = 4096;  // three ints each in LDS: 48 KiB
 
 struct PlanParams {
   const int32_t *context_lens, *new_lens, *free_blocks, *free_begin;
@@ -30,43 +32,44 @@ struct PlanParams {
   int B, lb;
 };
 
+// Sum over the lanes up to this one of values below 2^36, in two halves of 32-bit lane operations.
+__device__ __forceinline__ int64_t wave_scan36(int64_t v) {
+  return ((int64_t)wave_scan((int)(v >> 16)) << 16) + wave_scan((int)(v & 0xffff));
+}
+
 __global__ __launch_bounds__(PLAN_THREADS) void kv_block_plan_kernel(PlanParams p) {
   extern __shared__ int32_t lds_plan[];
-  int32_t* cu = lds_plan;             // [B] first token of a request
-  int32_t* fresh_at = lds_plan + p.B; // [B] its first entry among the fresh blocks
-  __shared__ long long wave_tok[4], wave_fresh[4];
+  int32_t* cu = lds_plan;                  // [B] first token of a request
+  int32_t* fresh_at = lds_plan + p.B;      // [B] its first entry among the fresh blocks
+  int32_t* context = lds_plan + 2 * p.B;   // [B]
+  __shared__ int64_t wave_tok[4], wave_fresh[4];
   __shared__ int wave_wide[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t bs = 1ll << p.lb;
-  // a thread owns `per` requests that follow each other: one scan over the threads is enough
+  const int64_t begin = max(p.free_begin[0], 0);
+  // a thread owns `per` requests that follow each other: one scan over the threads is enough.  At
+  // most 16 requests of less than 2^31 tokens each: its sums stay below 2^36.
   const int per = (p.B + PLAN_THREADS - 1) / PLAN_THREADS;
   const int i0 = tid * per, i1 = min(p.B, i0 + per);
-  long long tok = 0, fresh = 0;
+  int64_t tok = 0, fresh = 0;
   int wide = 0;
   for (int i = i0; i < i1; ++i) {
     const int64_t c = max(p.context_lens[i], 0), n = max(p.new_lens[i], 0);
     const int64_t held = (c + bs - 1) >> p.lb, need = (c + n + bs - 1) >> p.lb;
+    context[i] = (int)c;
     tok += n;
     fresh += need - held;
     wide += need > p.table_width;
   }
-  long long tok_in = tok, fresh_in = fresh;  // inclusive over the wave
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const long long a = __shfl_up(tok_in, o, 64), b = __shfl_up(fresh_in, o, 64);
-    if (lane >= o) {
-      tok_in += a;
-      fresh_in += b;
-    }
-    wide += __shfl_xor(wide, o, 64);
-  }
+  const int64_t tok_in = wave_scan36(tok), fresh_in = wave_scan36(fresh);  // inclusive over the wave
+  wide = wave_scan(wide);
   if (lane == 63) {
     wave_tok[wave] = tok_in;
     wave_fresh[wave] = fresh_in;
     wave_wide[wave] = wide;
   }
   __syncthreads();
-  long long tok_all = 0, fresh_all = 0, tok_at = tok_in - tok, fresh_from = fresh_in - fresh;
+  int64_t tok_all = 0, fresh_all = 0, tok_at = tok_in - tok, fresh_from = fresh_in - fresh;
   int wide_all = 0;
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
@@ -78,13 +81,12 @@ __global__ __launch_bounds__(PLAN_THREADS) void kv_block_plan_kernel(PlanParams 
     fresh_all += wave_fresh[w];
     wide_all += wave_wide[w];
   }
-  const int64_t begin = max(p.free_begin[0], 0);
   const int64_t lacking = max((int64_t)0, begin + fresh_all - p.num_free);
-  const int64_t over = max((int64_t)0, (int64_t)tok_all - p.max_tokens);
+  const int64_t over = max((int64_t)0, tok_all - p.max_tokens);
   const bool good = lacking == 0 && over == 0 && wide_all == 0;
   const bool first_group = blockIdx.x == 0;
   for (int i = i0; i < i1; ++i) {
-    const int64_t c = max(p.context_lens[i], 0), n = max(p.new_lens[i], 0);
+    const int64_t c = context[i], n = max(p.new_lens[i], 0);
     if (good) {  // the sums fit: tokens are below max_tokens, blocks below num_free
       cu[i] = (int)tok_at;
       fresh_at[i] = (int)fresh_from;
@@ -104,26 +106,55 @@ __global__ __launch_bounds__(PLAN_THREADS) void kv_block_plan_kernel(PlanParams 
     p.status[2] = wide_all;
   }
   __syncthreads();
-  const int64_t t_end = min(p.max_tokens, ((int64_t)blockIdx.x + 1) * PLAN_TOKENS);
-  for (int64_t t = (int64_t)blockIdx.x * PLAN_TOKENS + tid; t < t_end; t += PLAN_THREADS) {
-    int64_t slot = -1, place = 0;
-    if (good && t < tok_all) {
-      int lo = 0, hi = p.B;  // the last request that begins at or before t is the one that holds it
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (cu[mid] <= (int)t) lo = mid;
-        else hi = mid;
-      }
-      const int64_t c = max(p.context_lens[lo], 0);
-      place = c + (t - cu[lo]);
-      const int64_t j = place >> p.lb, held = (c + bs - 1) >> p.lb;
-      int32_t* entry = p.table + lo * p.table_stride + j;
-      const int id = j < held ? *entry : p.free_blocks[begin + fresh_at[lo] + (j - held)];
-      if ((place & (bs - 1)) == 0) *entry = id;  // a block's first token: never one held before
-      if (id >= 0 && id < p.num_blocks) slot = ((int64_t)id << p.lb) + (place & (bs - 1));
+  // Tokens t0, t0 + 256, ...: four at a time, so that their searches and look-ups go on together.
+  const int64_t t0 = (int64_t)blockIdx.x * PLAN_TOKENS + tid;
+  auto fill = [&](auto count, int64_t from) {
+    constexpr int N = decltype(count)::value;
+    int lo[N], hi[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      lo[k] = 0;
+      hi[k] = p.B;
     }
-    p.slots[t] = slot;
-    p.positions[t] = place;
+    // the last request that begins at or before t is the one that holds it
+    for (int left = good ? p.B : 1; left > 1; left = (left + 1) >> 1) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const int mid = (lo[k] + hi[k]) >> 1;
+        const bool up = cu[mid] <= (int)(from + k * PLAN_THREADS);  // (mid is in [0, B))
+        lo[k] = up ? mid : lo[k];
+        hi[k] = up ? hi[k] : mid;
+      }
+    }
+    int64_t place[N];
+    int id[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int64_t t = from + k * PLAN_THREADS;
+      place[k] = 0;
+      id[k] = -1;
+      if (good && t < tok_all) {
+        const int64_t c = context[lo[k]];
+        place[k] = c + (t - cu[lo[k]]);
+        const int64_t j = place[k] >> p.lb, held = (c + bs - 1) >> p.lb;
+        id[k] = j < held ? p.table[lo[k] * p.table_stride + j] : p.free_blocks[begin + fresh_at[lo[k]] + (j - held)];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int64_t t = from + k * PLAN_THREADS;
+      if (t >= p.max_tokens) continue;
+      // a block's first token: never one held before
+      if (good && t < tok_all && (place[k] & (bs - 1)) == 0)
+        p.table[lo[k] * p.table_stride + (place[k] >> p.lb)] = id[k];
+      p.slots[t] = id[k] >= 0 && id[k] < p.num_blocks ? ((int64_t)id[k] << p.lb) + (place[k] & (bs - 1)) : -1;
+      p.positions[t] = place[k];
+    }
+  };
+  if (p.max_tokens > 2 * PLAN_THREADS) {
+    fill(std::integral_constant<int, 4>{}, t0);
+  } else {
+    for (int64_t t = t0; t - tid < p.max_tokens; t += PLAN_THREADS) fill(std::integral_constant<int, 1>{}, t);
   }
 }
 
@@ -248,9 +279,10 @@ __global__ __launch_bounds__(ROPE_THREADS) void rope_scaled_kernel(Rope r, RopeR
   rope_tokens(r, q, k, D, t0, (int)min((int64_t)per_group, tokens - t0), cs);
 }
 
-// Tokens of one workgroup: one while there are few, for the sake of latency; four where that
-// still leaves eight workgroups to each CU.
-inline int rope_group(int64_t tokens) { return tokens >= 8192 ? ROPE_MAX_TOKENS : 1; }
+// Tokens of one workgroup: one while there are few, for the sake of latency, then four, since very
+// many small workgroups are held up by their own dispatch (8191 tokens, 40 heads of 128, half of a
+// head turned: 36.5 us, with one token 38.0, with eight 46.7).
+inline int rope_group(int64_t tokens) { return tokens >= 1024 ? ROPE_MAX_TOKENS : 1; }
 
 // ----------------------------------------------------------------------------------- store --
 // A workgroup owns one run: the tokens of a call that follow each other into one block, for one
@@ -515,7 +547,7 @@ extern "C" int mi355_kv_block_plan(const int32_t* context_lens, const int32_t* n
                 (long)B, (long)PLAN_MAX_REQUESTS);
   MI355_REQUIRE(block_size_ok(block_size), "kv_block_plan: block size %ld must be a power of two in [16, 1024]",
                 (long)block_size);
-  MI355_REQUIRE(max_tokens >= 0 && max_tokens < (1ll << 31) && num_free >= 0 && num_free < (1ll << 31) &&
+  MI355_REQUIRE(max_tokens >= 0 && max_tokens <= (1ll << 31) - 4096 && num_free >= 0 && num_free < (1ll << 31) &&
                     num_blocks >= 0 && num_blocks < (1ll << 31) && table_width >= 0 &&
                     (B <= 1 || table_stride >= table_width),
                 "kv_block_plan: bad size");
@@ -532,7 +564,7 @@ extern "C" int mi355_kv_block_plan(const int32_t* context_lens, const int32_t* n
                   free_end, status, slot_mapping, positions, table_stride, table_width, num_free, num_blocks,
                   max_tokens, (int)B, log2_of(block_size)};
   const int64_t groups = max_tokens ? (max_tokens + PLAN_TOKENS - 1) / PLAN_TOKENS : 1;
-  const size_t lds = (size_t)(2 * B) * sizeof(int32_t);
+  const size_t lds = (size_t)(3 * B) * sizeof(int32_t);
   hipLaunchKernelGGL(kv_block_plan_kernel, dim3((unsigned)groups), dim3(PLAN_THREADS), lds,
                      (hipStream_t)stream, p);
   MI355_CHECK_LAUNCH("kv_block_plan");
@@ -611,7 +643,7 @@ extern "C" int mi355_kv_store_fp8(const mi355_kv_store_args* a, void* stream) {
   // (each may be a request of its own, and runs that one workgroup finds are stored one after the
   // other), then as many as keep the launch to about twice the workgroups that the chip holds: most
   // of them find no run where tokens follow each other, and take a place for the while (4602 tokens
-  // of 12 prompts, 8 heads: %GROUP%).
+  // of 12 prompts, 8 heads: 43 us, with groups of 32 53 us, of 16 54 us).
   p.group = 1;
   while (p.group < 64 && (a->tokens + p.group - 1) / p.group * 2 * a->Hk > 2048) p.group *= 2;
   const int64_t units = (a->tokens + p.group - 1) / p.group * 2 * a->Hk;
