@@ -341,7 +341,7 @@ def _check_table(what, table, rows, name, like):
 def _check_heads(what, x, tokens, name, like):
     if not (x.dtype == torch.bfloat16 and x.dim() == 3 and x.stride(2) == 1 and x.shape[0] == tokens):
         _fail(f"{what}: {name} must be bfloat16 [tokens, heads, head_size] with a contiguous last dimension")
-    if x.get_device() != like.get_device():
+    if x is not like and x.get_device() != like.get_device():
         _fail(f"{what}: all tensors must be on {like.device}")
 
 
@@ -385,16 +385,19 @@ def _fwd_paged(q, k_cache, v_cache, out, cu_seqlens_q, cache_seqlens, max_seqlen
         _fail("fwd: sliding windows need causal attention, and end at the token itself")
     device = q.device
     if out is None:
-        out = torch.empty(shape, dtype=torch.bfloat16, device=device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif not (out.shape == shape and out.dtype == q.dtype and out.stride(-1) == 1 and out.device == device):
         _fail("fwd: out must match q")
-    lse = torch.empty((H, shape[0]) if packed else (B, H, shape[1]), dtype=torch.float32, device=device)
+    if packed:
+        lse = torch.empty(H, shape[0], dtype=torch.float32, device=device)
+    else:
+        lse = torch.empty(B, H, shape[1], dtype=torch.float32, device=device)
     if softmax_scale is None:
         softmax_scale = shape[-1] ** -0.5
     if q.numel() and B:
         _C.paged_attention_fp8(q, k_cache, v_cache, k_descale, v_descale, page_table, cache_seqlens, cu_seqlens_q,
                                max_seqlen_q, out, lse, softmax_scale, is_causal, window_left)
-    empty = torch.empty(0, dtype=torch.float32, device=device)
+    empty = lse.new_empty(0)
     return out, lse, empty, empty
 
 

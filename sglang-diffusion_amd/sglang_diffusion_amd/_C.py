@@ -227,10 +227,10 @@ def _stream(t: torch.Tensor) -> int:
     if not t.is_cuda:
         raise RuntimeError("mi355 kernels need tensors on a HIP device (got a CPU tensor)")
     index = t.get_device()
-    if index != torch.cuda.current_device():
+    if index != torch._C._cuda_getDevice():
         raise RuntimeError(f"tensor on cuda:{index} but the current device is cuda:"
                            f"{torch.cuda.current_device()}: wrap the call in torch.cuda.device(...)")
-    # (the raw handle: making a Stream object to ask it costs microseconds at every launch)
+    # (the raw calls: a Stream object and the checks of torch.cuda cost microseconds at every launch)
     return torch._C._cuda_getCurrentRawStream(index)
 
 
@@ -804,13 +804,21 @@ def kv_block_plan(context_lens, new_lens, block_table, free_blocks, free_begin, 
 def rope_scaled(positions, q, k, inv_freq, attn_factor, is_neox, q_out, k_out) -> None:
     """q [T, Hq, D], k [T, Hk, D] or None (last dim contiguous), written to q_out / k_out."""
     T, H, D = q.shape
-    ks = (0, 0, 0, 0) if k is None else (k.stride(0), k.stride(1), k_out.stride(0), k_out.stride(1))
+    qt, qh, _ = q.stride()
+    qot, qoh, _ = q_out.stride()
+    if k is None:
+        Hk = kt = kh = kot = koh = 0
+        kp = kop = None
+    else:
+        Hk = k.shape[1]
+        kt, kh, _ = k.stride()
+        kot, koh, _ = k_out.stride()
+        kp, kop = k.data_ptr(), k_out.data_ptr()
     _check(
         load_library().mi355_rope_scaled(
-            positions.data_ptr(), q.data_ptr(), q_out.data_ptr(), _p(k), _p(k_out), T, H,
-            0 if k is None else k.shape[1], D, 2 * inv_freq.numel(), q.stride(0), q.stride(1), q_out.stride(0),
-            q_out.stride(1), *ks, inv_freq.data_ptr(), int(inv_freq.dtype == torch.float64), float(attn_factor),
-            int(bool(is_neox)), _stream(q),
+            positions.data_ptr(), q.data_ptr(), q_out.data_ptr(), kp, kop, T, H, Hk, D, 2 * inv_freq.numel(), qt, qh,
+            qot, qoh, kt, kh, kot, koh, inv_freq.data_ptr(), inv_freq.dtype == torch.float64, attn_factor,
+            bool(is_neox), _stream(q),
         ),
         "rope_scaled",
     )
@@ -821,18 +829,19 @@ def kv_store_fp8(k, v, k_cache, v_cache, k_scale, v_scale, slot_mapping, q=None,
     """k, v [T, Hk, D] bf16 into caches [blocks, block_size, Hk, D] (e4m3) with scales [blocks, Hk];
     positions given: keys, and q [T, Hq, D] into q_out, are rotated."""
     T, Hk, D = k.shape
+    blocks, block_size = k_cache.shape[:2]
     a = KvStoreArgs(
-        k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1), k_cache.data_ptr(),
-        v_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2), v_cache.stride(0),
-        v_cache.stride(1), v_cache.stride(2), k_scale.data_ptr(), v_scale.data_ptr(), slot_mapping.data_ptr(),
-        T, Hk, D, k_cache.shape[1], k_cache.shape[0])
+        k.data_ptr(), v.data_ptr(), *k.stride()[:2], *v.stride()[:2], k_cache.data_ptr(), v_cache.data_ptr(),
+        *k_cache.stride()[:3], *v_cache.stride()[:3], k_scale.data_ptr(), v_scale.data_ptr(),
+        slot_mapping.data_ptr(), T, Hk, D, block_size, blocks)
     if positions is not None:
         a.positions, a.inv_freq = positions.data_ptr(), inv_freq.data_ptr()
         a.rot_dim, a.inv_freq_is_f64 = 2 * inv_freq.numel(), inv_freq.dtype == torch.float64
         a.is_neox, a.attn_factor = bool(is_neox), attn_factor
     if q is not None:
         a.Hq, a.q, a.q_out = q.shape[1], q.data_ptr(), q_out.data_ptr()
-        a.q_st, a.q_sh, a.qo_st, a.qo_sh = q.stride(0), q.stride(1), q_out.stride(0), q_out.stride(1)
+        a.q_st, a.q_sh, _ = q.stride()
+        a.qo_st, a.qo_sh, _ = q_out.stride()
     _check(load_library().mi355_kv_store_fp8(ctypes.byref(a), _stream(k)), "kv_store_fp8")
 
 
@@ -843,14 +852,15 @@ def paged_attention_fp8(q, k_cache, v_cache, k_scale, v_scale, page_table, cache
     current stream, or to the graph that is being captured."""
     packed = q.dim() == 3
     Sq, H, D = q.shape[-3:]
-    B = cache_seqlens.numel()
+    blocks, block_size, Hk, _ = k_cache.shape
+    B, width = page_table.shape
     s, os_ = q.stride(), out.stride()
     a = PagedAttnArgs(
         q.data_ptr(), out.data_ptr(), _p(lse), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
-        v_scale.data_ptr(), _p(cu_seqlens_q), cache_seqlens.data_ptr(), page_table.data_ptr(), B, Sq, H,
-        k_cache.shape[2], D, max_seqlen_q, 0 if packed else s[0], s[-3], s[-2], 0 if packed else os_[0], os_[-3],
-        os_[-2], 0 if packed else H * Sq, Sq, *k_cache.stride()[:3], *v_cache.stride()[:3], page_table.stride(0),
-        page_table.shape[1], k_cache.shape[0], k_cache.shape[1], softmax_scale, causal, window_left)
+        v_scale.data_ptr(), _p(cu_seqlens_q), cache_seqlens.data_ptr(), page_table.data_ptr(), B, Sq, H, Hk, D,
+        max_seqlen_q, 0 if packed else s[0], s[-3], s[-2], 0 if packed else os_[0], os_[-3], os_[-2],
+        0 if packed else H * Sq, Sq, *k_cache.stride()[:3], *v_cache.stride()[:3], page_table.stride(0), width, blocks,
+        block_size, softmax_scale, causal, window_left)
     lib = load_library()
     stream = _stream(q)
     need = lib.mi355_paged_attn_workspace_bytes(ctypes.byref(a))
