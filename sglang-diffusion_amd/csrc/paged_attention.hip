@@ -49,7 +49,7 @@ struct PagedParams {
   int num_blocks, lb, causal, window;
   float scale_log2;
   // items
-  int items, chunk_min, split;
+  int items, chunk_min, split, hw, turns;  // hw: heads of a workgroup, turns: waves of each
   float inv_target;
   float* part;       // [Hk * items][M][D + 2]
   int32_t* info;     // [B][2]: first item of the sequence, chunks of each of its row tiles
@@ -87,7 +87,7 @@ struct Item {
 // The item'th item of a key/value head, for the whole workgroup; false behind the last one.  One
 // wave adds up the sequences, `per` that follow each other to a lane, and hands the item on.
 template <int M>
-__device__ bool find_item(const PagedParams& p, int item, int hk, Item* out) {
+__device__ bool find_item(const PagedParams& p, int item, int group, Item* out) {
   __shared__ Item found;
   if (threadIdx.x < 64) {
     const int lane = threadIdx.x;
@@ -108,7 +108,7 @@ __device__ bool find_item(const PagedParams& p, int item, int hk, Item* out) {
       }
       work = group_sum<64>(work);
       length = (int)fminf(1e9f, fmaxf((float)p.chunk_min, ceilf(work * p.inv_target)));
-      if (M < 64) length = (length + 3) & ~3;  // whole turns of the four waves
+      length = (length + p.turns - 1) / p.turns * p.turns;  // whole turns of the waves of a head
     } else if (b0 < b1) {
       s = seq_of(p, b0);
     }
@@ -136,7 +136,7 @@ __device__ bool find_item(const PagedParams& p, int item, int hk, Item* out) {
         if (k >= 0 && k < (int64_t)tiles * chunks) {
           // causal rows further down see more: they begin first
           found = Item{s, b, tiles - 1 - k / chunks, k % chunks, chunks, length};
-          if (p.split && k == 0 && hk == 0) {  // for the join
+          if (p.split && k == 0 && group == 0) {  // for the join
             p.info[2 * b] = item;
             p.info[2 * b + 1] = chunks;
           }
@@ -292,11 +292,16 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
   constexpr int M = 16 * RT, NH = D / 64, CPR = D / 16, DB = D / 16;
   __shared__ __attribute__((aligned(16))) unsigned char vimg[4][2 * KT * D];
   __shared__ float wave_m[4][M], wave_l[4][M];
-  const int item = (blockIdx.x / (8 * p.Hk)) * 8 + blockIdx.x % 8, hk = (blockIdx.x / 8) % p.Hk;
+  // eight items side by side, so that all heads of an item are on one of the eight XCDs
+  const int groups = p.Hk / p.hw, item = (blockIdx.x / (8 * groups)) * 8 + blockIdx.x % 8;
+  const int group = (blockIdx.x / 8) % groups;
   Item it;
-  if (!find_item<M>(p, item, hk, &it)) return;
-  const Job job = job_of<M>(p, it, hk);
+  if (!find_item<M>(p, item, group, &it)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // `hw` heads, and `turns` waves for each that take the tiles in turn
+  const int hw = p.hw, turns = 4 / hw, in_group = wave % hw, turn = wave / hw;
+  const int hk = group * hw + in_group;
+  const Job job = job_of<M>(p, it, hk);
   const int r = lane & 15, g = lane >> 4;
 
   bf16x8 qf[RT][NH][2];
@@ -361,14 +366,14 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
   };
 
   bool nan_values = false;
-  int t = job.t0 + wave;
+  int t = job.t0 + turn;
   Ahead now{0, 0}, next{0, 0};
   Scales sc{};
   if (t < job.t1) {
     now = resolve(p, job, t, load_entry(p, job, t));
     load_k(now, t);
     load_v(now, t);
-    next = resolve(p, job, t + 4, load_entry(p, job, t + 4));
+    next = resolve(p, job, t + turns, load_entry(p, job, t + turns));
     const int64_t at = (int64_t)now.block * p.Hk + hk;
     sc = scales_of(p, p.ks[at], p.vs[at]);
   }
@@ -380,8 +385,8 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
     for (int h2 = 0; h2 < NH; ++h2)
 #pragma unroll
       for (int u = 0; u < 2; ++u) asm volatile("" : "+v"(qf[rt][h2][u]));
-  for (; t < job.t1; t += 4) {
-    const bool more = t + 4 < job.t1;
+  for (; t < job.t1; t += turns) {
+    const bool more = t + turns < job.t1;
     const int key0 = t * KT;
     const bool masked = in_part(t, now.ok);
     // values into the image
@@ -403,12 +408,12 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    if (more) load_k(next, t + 4);
+    if (more) load_k(next, t + turns);
     // entries of the tile after the next, values and scales of the next
-    const int entry = load_entry(p, job, t + 8);
+    const int entry = load_entry(p, job, t + 2 * turns);
     const int64_t scale_at = (int64_t)next.block * p.Hk + hk;
     const float ks = p.ks[scale_at], vs = p.vs[scale_at];
-    if (more) load_v(next, t + 4);
+    if (more) load_v(next, t + turns);
 
     f32x4 s[RT][4];
 #pragma unroll
@@ -497,11 +502,11 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
     __builtin_amdgcn_wave_barrier();
     if (!more) break;  // (so that whatever was loaded has been used before the next turn)
     now = next;
-    next = resolve(p, job, t + 8, entry);
+    next = resolve(p, job, t + 2 * turns, entry);
     sc = scales_of(p, ks, vs);
   }
   if (nan_values) {  // poison: the NaN among the values of tiles seen in part, for the rows that see them
-    for (t = job.t0 + wave; t < job.t1; t += 4) {
+    for (t = job.t0 + turn; t < job.t1; t += turns) {
       now = resolve(p, job, t, load_entry(p, job, t));
       if (!in_part(t, now.ok)) continue;
       const int64_t offsets = piece_offsets(p, now, t, p.vc_sb, p.vc_st);
@@ -523,7 +528,7 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
     }
   }
 
-  // ---- the four waves' parts of each row, joined ----
+  // ---- the parts of each row that the waves of a head hold, joined ----
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     l[rt] += __shfl_xor(l[rt], 16, 64);
@@ -539,9 +544,8 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     __syncthreads();
-    float top = wave_m[0][16 * rt + r];
-#pragma unroll
-    for (int w = 1; w < 4; ++w) top = fmaxf(top, wave_m[w][16 * rt + r]);
+    float top = M_EMPTY;
+    for (int w = in_group; w < 4; w += hw) top = fmaxf(top, wave_m[w][16 * rt + r]);
     const float weight = __builtin_amdgcn_exp2f(m[rt] - top);
     // [16 rows][D] fp32 in the wave's image (64 D bytes), 16-byte pieces turned by the row
     float* mine = reinterpret_cast<float*>(vimg[wave]);
@@ -549,19 +553,18 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
     for (int d = 0; d < DB; ++d)
       *reinterpret_cast<f32x4*>(mine + r * D + (((4 * d + g) ^ (r & 7)) << 2)) = o[rt][d] * weight;
     __syncthreads();
-    // four channels of a row for each thread
-    for (int i = threadIdx.x; i < 16 * D / 4; i += 256) {
+    // four channels of a row for each thread of the head
+    for (int i = turn * 64 + lane; i < 16 * D / 4; i += turns * 64) {
       const int row = i / (D / 4), c4 = i % (D / 4), at = row * D + ((c4 ^ (row & 7)) << 2);
-      f32x4 sum = *reinterpret_cast<const f32x4*>(reinterpret_cast<float*>(vimg[0]) + at);
-#pragma unroll
-      for (int w = 1; w < 4; ++w)
+      const int in_tile = 16 * rt + row, q_row = job.row0 + in_tile;
+      if (q_row >= job.rows) continue;
+      float rm = M_EMPTY, rl = 0.f;
+      for (int w = in_group; w < 4; w += hw) rm = fmaxf(rm, wave_m[w][in_tile]);
+      f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int w = in_group; w < 4; w += hw) {
         sum = sum + *reinterpret_cast<const f32x4*>(reinterpret_cast<float*>(vimg[w]) + at);
-      const int in_tile = 16 * rt + row;
-      float rm = wave_m[0][in_tile], rl = 0.f;
-#pragma unroll
-      for (int w = 1; w < 4; ++w) rm = fmaxf(rm, wave_m[w][in_tile]);
-#pragma unroll
-      for (int w = 0; w < 4; ++w) rl = fmaf(wave_l[w][in_tile], __builtin_amdgcn_exp2f(wave_m[w][in_tile] - rm), rl);
+        rl = fmaf(wave_l[w][in_tile], __builtin_amdgcn_exp2f(wave_m[w][in_tile] - rm), rl);
+      }
       if (part) {
         *reinterpret_cast<f32x4*>(part + in_tile * D + 4 * c4) = sum;
         if (c4 == 0) {
@@ -570,8 +573,6 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
         }
         continue;
       }
-      const int q_row = job.row0 + in_tile;
-      if (q_row >= job.rows) continue;
       const int tok = q_row / p.G, head = hk * p.G + q_row - tok * p.G;
       const float inv = rl == 0.f ? 0.f : 1.f / rl;
       *reinterpret_cast<u32x2*>(p.o + job.b * p.o_sb + (int64_t)(job.s.first + tok) * p.o_ss + head * p.o_sh +
@@ -884,12 +885,13 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedP
 }
 
 // ------------------------------------------------------------------------------------- joint --
-// The chunks of a row: a wave for each row of q.  Lane c weighs chunk c; the sums run over eight
+// The chunks of a row of q: WAVES waves for each.  Lane c weighs chunk c; the sums run over a few
 // chunks at a time, so that their loads are in flight together.
-template <int D>
+template <int D, int WAVES>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p, int M, int64_t rows) {
-  const int lane = threadIdx.x & 63;
-  const int64_t row_of_q = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  __shared__ f32x4 others[3][D / 4];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t row_of_q = WAVES == 4 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
   if (row_of_q >= rows) return;
   const int H = p.Hk * p.G;
   const int64_t t = row_of_q / H;
@@ -933,7 +935,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p, int M, i
     const float w = c0 + lane < chunks ? __builtin_amdgcn_exp2f(ml[0] - top) : 0.f;
     l = fmaf(w != 0.f ? ml[1] : 0.f, w, l);
     const int here = min(64, chunks - c0);
-    for (int k = 0; k < here; k += 4 * SIDE) {
+    for (int k = WAVES == 4 ? wave * 4 * SIDE : 0; k < here; k += WAVES * 4 * SIDE) {
       f32x4 v[4];
       float wv[4];
 #pragma unroll
@@ -954,6 +956,13 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p, int M, i
   for (int w = LANES; w < 64; w <<= 1)
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[j] += __shfl_xor(acc[j], w, 64);
+  if constexpr (WAVES == 4) {
+    if (wave && mine == 0) others[wave - 1][ch] = acc;
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int w = 0; w < 3; ++w) acc = acc + others[w][ch];
+  }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   if (mine == 0)
     *reinterpret_cast<u32x2*>(p.o + b * p.o_sb + (p.cu ? t : tok) * p.o_ss + head * p.o_sh + 4 * ch) =
@@ -977,7 +986,7 @@ int cu_count() {
 }
 
 struct Plan {
-  int M, few;          // rows of a tile; which kernel
+  int M, few, hw;      // rows of a tile; which kernel; heads of a workgroup
   int64_t items, target;
   int chunk_min, split;
   int64_t part_bytes, info_bytes;
@@ -990,16 +999,21 @@ Plan plan_of(const mi355_paged_attn_args* a) {
   const int64_t all_rows = (a->cu_seqlens_q ? a->Sq : a->Sq * a->B) * G;
   w.few = rows <= 16 ? 1 : rows <= 32 ? 2 : 0;
   w.M = w.few ? 16 * w.few : 128;
+  // as many heads to a workgroup as share its four waves: what they read lies side by side
+  w.hw = !w.few ? 1 : a->Hk % 4 == 0 ? 4 : a->Hk % 2 == 0 ? 2 : 1;
   const int64_t tiles = all_rows / w.M + a->B;  // row tiles: at most one not full for each sequence
-  // Items to aim for.  Many rows: as many as the chip holds workgroups (two a CU, with heads of 64
-  // three: 509 tokens behind 30k keys 105 us, with two 115 us); the parts to be joined are large.
-  // Few rows: twice as many, since chunks end unevenly and the next one takes the place (4 x 1
-  // token over 128k keys 178 us, one round 205 us, three 195 us).
-  const int64_t want = (w.few ? 4 : a->D == 64 ? 3 : 2) * (int64_t)cu_count();
-  w.target = (want + a->Hk - 1) / a->Hk;
-  w.chunk_min = 4;
+  // Items to aim for: as many as the chip holds workgroups, two a CU (many rows with heads of 64:
+  // three; 509 tokens behind 30k keys 105 us, with two 115 us).  With few rows the last chunk of
+  // each row tile is about half a chunk, and what is over one round of workgroups waits for it:
+  // half the row tiles are taken off (32 x 1 token, ragged: 44 us, without 53 us, with two rounds
+  // of half the length 50 us).
+  const int64_t want = (w.few ? 2 : a->D == 64 ? 3 : 2) * (int64_t)cu_count();
+  const int64_t groups = a->Hk / w.hw;
+  w.target = (want + groups - 1) / groups;
+  if (w.few) w.target -= tiles < w.target ? tiles / 2 : w.target / 2;
+  w.chunk_min = w.few ? (w.hw == 4 ? 1 : 4) : 4;
   const int64_t cap = a->table_width * a->block_size;
-  w.split = cap > (int64_t)w.chunk_min * KT && (all_rows / w.M) * a->Hk < 2 * want;
+  w.split = cap > (int64_t)w.chunk_min * KT && (all_rows / w.M) * groups < 2 * want;
   w.items = tiles + (w.split ? w.target : 0);
   w.part_bytes = w.split ? a->Hk * w.items * w.M * (a->D + 2) * (int64_t)sizeof(float) : 0;
   w.info_bytes = w.split ? a->B * 2 * (int64_t)sizeof(int32_t) : 0;
@@ -1026,7 +1040,7 @@ int check(const mi355_paged_attn_args* a) {
 
 template <int D>
 int launch(const PagedParams& p, const Plan& w, hipStream_t st) {
-  const dim3 grid((unsigned)((w.few ? (w.items + 7) / 8 * 8 : w.items) * p.Hk));
+  const dim3 grid((unsigned)(w.few ? (w.items + 7) / 8 * 8 * (p.Hk / w.hw) : w.items * p.Hk));
   if (w.few == 1) {
     hipLaunchKernelGGL((paged_few_rows_kernel<D, 1>), grid, dim3(256), 0, st, p);
   } else if (w.few == 2) {
@@ -1052,7 +1066,11 @@ int launch(const PagedParams& p, const Plan& w, hipStream_t st) {
   MI355_CHECK_LAUNCH("paged_attn_fp8");
   if (w.split) {
     const int64_t rows = (int64_t)p.Sq * (p.cu ? 1 : p.B) * p.Hk * p.G;
-    hipLaunchKernelGGL(paged_join_kernel<D>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, p, w.M, rows);
+    // four waves for a row while there are few rows (4 x 1 token over 128k keys: 6.3 us, with one 9)
+    if (rows <= 2048)
+      hipLaunchKernelGGL((paged_join_kernel<D, 4>), dim3((unsigned)rows), dim3(256), 0, st, p, w.M, rows);
+    else
+      hipLaunchKernelGGL((paged_join_kernel<D, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, p, w.M, rows);
     MI355_CHECK_LAUNCH("paged_attn_fp8 (join)");
   }
   return MI355_OK;
@@ -1121,6 +1139,8 @@ extern "C" int mi355_paged_attn_fp8(const mi355_paged_attn_args* a, void* stream
   p.inv_target = 1.f / (float)w.target;
   p.chunk_min = w.chunk_min;
   p.split = w.split;
+  p.hw = w.hw;
+  p.turns = w.few ? 4 / w.hw : 1;
   p.part = (float*)a->workspace;
   p.info = (int32_t*)((char*)a->workspace + w.part_bytes);
   return a->D == 128 ? launch<128>(p, w, (hipStream_t)stream) : launch<64>(p, w, (hipStream_t)stream);
