@@ -278,19 +278,22 @@ __device__ __forceinline__ unsigned clear_nan(u32x4& v) {
   return any;
 }
 
-// ----------------------------------------------------------------- few rows: 16 or 32 of them --
-// Four waves share the rows and take turns at the tiles of the chunk; each keeps its own m, l and
-// O, joined through LDS at the end.  A wave's tile: keys straight to registers (lane: key l & 15,
-// 16 bytes of the head at (l >> 4) * 16: two k-steps of the 16x16x32 product), values through its
-// own 64-row image in LDS, from which ds_read_b64_tr_b8 reads eight keys of one channel.  Both
-// are loaded one tile ahead into the registers that the current tile has just left.
+// ----------------------------------------------------------------------- few rows: up to sixteen --
+// What a decoding step has: it is bound by reading the cache, and built to read it in whole lines,
+// early, once.  A wave owns a head and takes tiles of its chunk; the four waves of a workgroup have
+// as many neighbouring heads as there are (what they read lies side by side: 4 x 1 token over 128k
+// keys in 135 us, 6.1 TB/s of the 6.3 that a plain read of that memory reaches; with the waves side
+// by side in the keys of one head 158 us) and take turns at the tiles where heads are fewer; their
+// parts are joined through LDS.  Keys and values of the next tile are loaded into registers, past
+// the caches, as soon as the current ones are in the wave's images in LDS: keys are read from there
+// in rows, values by ds_read_b64_tr_b8, eight keys of one channel to a lane.
 //   S^T[key][row] = K . Q^T: a lane holds row l & 15, keys 4 (l >> 4) + i of each piece;
 //   O^T[channel][row] += V^T . P^T: the same registers are the second operand, if the k index
 //   8 g + j counts keys 4 g + j of the first piece, then of the second one.
-template <int D, int RT>
-__global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
-  constexpr int M = 16 * RT, NH = D / 64, CPR = D / 16, DB = D / 16;
-  __shared__ __attribute__((aligned(16))) unsigned char vimg[4][2 * KT * D];
+template <int D>
+__global__ __launch_bounds__(256, D == 64 ? 4 : 2) void paged_few_rows_kernel(PagedParams p) {
+  constexpr int M = 16, NH = D / 64, CPR = D / 16, DB = D / 16;
+  __shared__ __attribute__((aligned(16))) unsigned char images[4][2 * KT * D];
   __shared__ float wave_m[4][M], wave_l[4][M];
   // eight items side by side, so that all heads of an item are on one of the eight XCDs
   const int groups = p.Hk / p.hw, item = (blockIdx.x / (8 * groups)) * 8 + blockIdx.x % 8;
@@ -304,36 +307,29 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
   const Job job = job_of<M>(p, it, hk);
   const int r = lane & 15, g = lane >> 4;
 
-  bf16x8 qf[RT][NH][2];
-  int see_lo[RT], see_hi[RT];
+  bf16x8 qf[NH][2];
+  int see_lo, see_hi;
+  const int row = min(job.row0 + r, job.rows - 1), tok = row / p.G, h = row - tok * p.G;
+  const unsigned short* qp = p.q + job.b * p.q_sb + (int64_t)(job.s.first + tok) * p.q_ss +
+                             (int64_t)(hk * p.G + h) * p.q_sh + 16 * g;
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const int row = min(job.row0 + 16 * rt + r, job.rows - 1), tok = row / p.G, h = row - tok * p.G;
-    const unsigned short* qp = p.q + job.b * p.q_sb + (int64_t)(job.s.first + tok) * p.q_ss +
-                               (int64_t)(hk * p.G + h) * p.q_sh + 16 * g;
+  for (int h2 = 0; h2 < NH; ++h2)
 #pragma unroll
-    for (int h2 = 0; h2 < NH; ++h2)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) qf[rt][h2][u] = *reinterpret_cast<const bf16x8*>(qp + 64 * h2 + 8 * u);
-    const int place = job.s.len - job.s.n + tok;
-    see_hi[rt] = min(p.causal ? place : job.s.len - 1, job.s.len - 1);
-    see_lo[rt] = p.window >= 0 ? place - p.window : 0;
-  }
+    for (int u = 0; u < 2; ++u) qf[h2][u] = *reinterpret_cast<const bf16x8*>(qp + 64 * h2 + 8 * u);
+  const int place = job.s.len - job.s.n + tok;
+  see_hi = min(p.causal ? place : job.s.len - 1, job.s.len - 1);
+  see_lo = p.window >= 0 ? place - p.window : 0;
 
-  f32x4 o[RT][DB];
-  float m[RT], l[RT];
+  f32x4 o[DB];
+  float m = 0.f, l = 0.f;
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    m[rt] = 0.f;
-    l[rt] = 0.f;
-#pragma unroll
-    for (int d = 0; d < DB; ++d) o[rt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
+  for (int d = 0; d < DB; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   u32x4 kr[CPR], vr[CPR];
   const unsigned char *k_head = p.kc + hk * p.kc_sh, *v_head = p.vc + hk * p.vc_sh;
   const unsigned k_lane = (unsigned)((lane / CPR) * p.kc_st + (lane % CPR) * 16);
   const unsigned v_lane = (unsigned)((lane / CPR) * p.vc_st + (lane % CPR) * 16);
+  auto once = [](const unsigned char* at) { return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at)); };
   auto load_k = [&](const Ahead& a, int t) {
     const int64_t offsets = piece_offsets(p, a, t, p.kc_sb, p.kc_st);
 #pragma unroll
@@ -341,7 +337,7 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
       const unsigned char* at = piece_at(k_head, offsets, c);
 #pragma unroll
       for (int i = 0; i < CPR / 4; ++i)
-        kr[c * CPR / 4 + i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at + (k_lane + (unsigned)(i * (64 / CPR) * p.kc_st))));
+        kr[c * CPR / 4 + i] = once(at + (k_lane + (unsigned)(i * (64 / CPR) * p.kc_st)));
     }
   };
   auto load_v = [&](const Ahead& a, int t) {
@@ -351,11 +347,11 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
       const unsigned char* at = piece_at(v_head, offsets, c);
 #pragma unroll
       for (int i = 0; i < CPR / 4; ++i)  // 64 / CPR rows at a time
-        vr[c * CPR / 4 + i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at + (v_lane + (unsigned)(i * (64 / CPR) * p.vc_st))));
+        vr[c * CPR / 4 + i] = once(at + (v_lane + (unsigned)(i * (64 / CPR) * p.vc_st)));
     }
   };
   auto swz = [](int row) { return D == 128 ? (row >> 1) & 7 : (row >> 2) & 3; };
-  unsigned char* img = vimg[wave];
+  unsigned char *img = images[wave], *k_img = img + KT * D;
   const int tr_row = (r >> 1) < 4 ? 4 * g + (r >> 1) : 12 + 4 * g + (r >> 1);
   const int tr_swz = swz(tr_row);
   const unsigned char* tr_at = img + tr_row * D + (r & 1) * 8;
@@ -380,16 +376,14 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
   // the queries are here before the loop begins: waited for inside it, they would hold up the loads
   // of the next tile with them at every turn
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt)
+  for (int h2 = 0; h2 < NH; ++h2)
 #pragma unroll
-    for (int h2 = 0; h2 < NH; ++h2)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) asm volatile("" : "+v"(qf[rt][h2][u]));
+    for (int u = 0; u < 2; ++u) asm volatile("" : "+v"(qf[h2][u]));
   for (; t < job.t1; t += turns) {
     const bool more = t + turns < job.t1;
     const int key0 = t * KT;
     const bool masked = in_part(t, now.ok);
-    // values into the image
+    // keys and values into the images; what is no key of the sequence as zeros (0 * NaN is NaN)
     if (masked) {
       unsigned any = 0;
 #pragma unroll
@@ -404,9 +398,9 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
     for (int i = 0; i < CPR; ++i) {
       const int row = (i * 64 + lane) / CPR;
       *reinterpret_cast<u32x4*>(img + row * D + (((lane % CPR) ^ swz(row)) << 4)) = vr[i];
-      *reinterpret_cast<u32x4*>(img + KT * D + row * D + (((lane % CPR) ^ swz(row)) << 4)) = kr[i];
+      *reinterpret_cast<u32x4*>(k_img + row * D + (((lane % CPR) ^ swz(row)) << 4)) = kr[i];
     }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
     if (more) load_k(next, t + turns);
     // entries of the tile after the next, values and scales of the next
@@ -415,78 +409,72 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
     const float ks = p.ks[scale_at], vs = p.vs[scale_at];
     if (more) load_v(next, t + turns);
 
-    f32x4 s[RT][4];
+    f32x4 s[4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) s[rt][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+      s[c] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int h = 0; h < NH; ++h) {
-        const u32x4 kk = *reinterpret_cast<const u32x4*>(img + KT * D + (16 * c + r) * D + (((4 * h + g) ^ swz(16 * c + r)) << 4));
+        const u32x4 kk = *reinterpret_cast<const u32x4*>(k_img + (16 * c + r) * D + (((4 * h + g) ^ swz(16 * c + r)) << 4));
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const bf16x8 kf = widen_bf16(kk[2 * u], kk[2 * u + 1]);
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt)
-            s[rt][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[rt][h][u], s[rt][c], 0, 0, 0);
+          s[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[h][u], s[c], 0, 0, 0);
         }
       }
     }
 
-    f16x8 pf[RT][2];
+    f16x8 pf[2];
+    // exponents against the reference as it stands; it moves (move_reference), and O and l with
+    // it, only where one of them is too large for a half, or a row has had no weight yet
+    float x[4][4], sum[4];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      // exponents against the reference as it stands; it moves (move_reference), and O and l with
-      // it, only where one of them is too large for a half, or a row has had no weight yet
-      float x[4][4], sum[4];
+    for (int c = 0; c < 4; ++c) {
+      const float add = sc.v_log[c] - m;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const float add = sc.v_log[c] - m[rt];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[c][i] = fmaf(s[rt][c][i], sc.k[c], add);
-      }
-      if (masked) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            x[c][i] = sees((now.ok >> c) & 1, key0 + 16 * c + 4 * g + i, see_lo[rt], see_hi[rt]) ? x[c][i] : -INFINITY;
-      }
-      float top = x[0][0];
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top = fmaxf(top, x[c][i]);
-      if (__builtin_amdgcn_ballot_w64(top > LAZY || l[rt] == 0.f) != 0) {
-        float mass = l[rt];
-#pragma unroll
-        for (int w = 16; w < 64; w <<= 1) {
-          top = fmaxf(top, __shfl_xor(top, w, 64));
-          mass += __shfl_xor(mass, w, 64);
-        }
-        const Move mv = move_reference(top, mass);
-        m[rt] += mv.by;
-        l[rt] *= mv.shrink;
-#pragma unroll
-        for (int d = 0; d < DB; ++d) o[rt][d] *= mv.shrink;
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[c][i] -= mv.by;
-      }
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[c][i] = __builtin_amdgcn_exp2f(x[c][i]);
-        sum[c] = (x[c][0] + x[c][1]) + (x[c][2] + x[c][3]);
-      }
-#pragma unroll
-      for (int c = 0; c < 4; ++c) l[rt] = fmaf(sum[c], sc.v_inv[c], l[rt]);
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) pf[rt][c >> 1][4 * (c & 1) + i] = (_Float16)x[c][i];
+      for (int i = 0; i < 4; ++i) x[c][i] = fmaf(s[c][i], sc.k[c], add);
     }
+    if (masked) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          x[c][i] = sees((now.ok >> c) & 1, key0 + 16 * c + 4 * g + i, see_lo, see_hi) ? x[c][i] : -INFINITY;
+    }
+    float top = x[0][0];
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = fmaxf(top, x[c][i]);
+    if (__builtin_amdgcn_ballot_w64(top > LAZY || l == 0.f) != 0) {
+      float mass = l;
+#pragma unroll
+      for (int w = 16; w < 64; w <<= 1) {
+        top = fmaxf(top, __shfl_xor(top, w, 64));
+        mass += __shfl_xor(mass, w, 64);
+      }
+      const Move mv = move_reference(top, mass);
+      m += mv.by;
+      l *= mv.shrink;
+#pragma unroll
+      for (int d = 0; d < DB; ++d) o[d] *= mv.shrink;
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[c][i] -= mv.by;
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[c][i] = __builtin_amdgcn_exp2f(x[c][i]);
+      sum[c] = (x[c][0] + x[c][1]) + (x[c][2] + x[c][3]);
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) l = fmaf(sum[c], sc.v_inv[c], l);
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pf[c >> 1][4 * (c & 1) + i] = (_Float16)x[c][i];
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -494,11 +482,9 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
         const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
             (__attribute__((address_space(3))) i32x2*)(tr_at + st * 32 * D + ((d ^ tr_swz) << 4)));
         const f16x8 vf = widen_f16((unsigned)w[0], (unsigned)w[1]);
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-          o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[rt][st], o[rt][d], 0, 0, 0);
+        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[st], o[d], 0, 0, 0);
       }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
     if (!more) break;  // (so that whatever was loaded has been used before the next turn)
     now = next;
@@ -514,73 +500,64 @@ __global__ __launch_bounds__(256, 2) void paged_few_rows_kernel(PagedParams p) {
         const int key = t * KT + k;
         if (!((now.ok >> (k >> 4)) & 1) || key >= job.s.len) continue;
         const unsigned char* at = piece_at(v_head, offsets, k >> 4) + (k & 15) * p.vc_st;
+        const unsigned seen = (unsigned)sees(true, key, see_lo, see_hi);
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
           const unsigned n = nan_codes(*reinterpret_cast<const unsigned*>(at + 16 * d + 4 * g));
 #pragma unroll
-          for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              o[rt][d][i] = ((n >> (8 * i + 7)) & (unsigned)sees(true, key, see_lo[rt], see_hi[rt])) ? __builtin_nanf("")
-                                                                                                  : o[rt][d][i];
+          for (int i = 0; i < 4; ++i) o[d][i] = ((n >> (8 * i + 7)) & seen) ? __builtin_nanf("") : o[d][i];
         }
       }
     }
   }
 
   // ---- the parts of each row that the waves of a head hold, joined ----
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    l[rt] += __shfl_xor(l[rt], 16, 64);
-    l[rt] += __shfl_xor(l[rt], 32, 64);
-    if (l[rt] == 0.f) m[rt] = M_EMPTY;
-    if (g == 0) {
-      wave_m[wave][16 * rt + r] = m[rt];
-      wave_l[wave][16 * rt + r] = l[rt];
-    }
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  if (l == 0.f) m = M_EMPTY;
+  if (g == 0) {
+    wave_m[wave][r] = m;
+    wave_l[wave][r] = l;
   }
   float* part = nullptr;
   if (it.chunks > 1) part = p.part + ((int64_t)hk * p.items + item) * (M * (D + 2));
+  __syncthreads();
+  float top = M_EMPTY;
+  for (int w = in_group; w < 4; w += hw) top = fmaxf(top, wave_m[w][r]);
+  const float weight = __builtin_amdgcn_exp2f(m - top);
+  // [16 rows][D] fp32 in the wave's image (64 D bytes), 16-byte pieces turned by the row
+  float* mine = reinterpret_cast<float*>(images[wave]);
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    __syncthreads();
-    float top = M_EMPTY;
-    for (int w = in_group; w < 4; w += hw) top = fmaxf(top, wave_m[w][16 * rt + r]);
-    const float weight = __builtin_amdgcn_exp2f(m[rt] - top);
-    // [16 rows][D] fp32 in the wave's image (64 D bytes), 16-byte pieces turned by the row
-    float* mine = reinterpret_cast<float*>(vimg[wave]);
-#pragma unroll
-    for (int d = 0; d < DB; ++d)
-      *reinterpret_cast<f32x4*>(mine + r * D + (((4 * d + g) ^ (r & 7)) << 2)) = o[rt][d] * weight;
-    __syncthreads();
-    // four channels of a row for each thread of the head
-    for (int i = turn * 64 + lane; i < 16 * D / 4; i += turns * 64) {
-      const int row = i / (D / 4), c4 = i % (D / 4), at = row * D + ((c4 ^ (row & 7)) << 2);
-      const int in_tile = 16 * rt + row, q_row = job.row0 + in_tile;
-      if (q_row >= job.rows) continue;
-      float rm = M_EMPTY, rl = 0.f;
-      for (int w = in_group; w < 4; w += hw) rm = fmaxf(rm, wave_m[w][in_tile]);
-      f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
-      for (int w = in_group; w < 4; w += hw) {
-        sum = sum + *reinterpret_cast<const f32x4*>(reinterpret_cast<float*>(vimg[w]) + at);
-        rl = fmaf(wave_l[w][in_tile], __builtin_amdgcn_exp2f(wave_m[w][in_tile] - rm), rl);
-      }
-      if (part) {
-        *reinterpret_cast<f32x4*>(part + in_tile * D + 4 * c4) = sum;
-        if (c4 == 0) {
-          part[M * D + 2 * in_tile] = rm;
-          part[M * D + 2 * in_tile + 1] = rl;
-        }
-        continue;
-      }
-      const int tok = q_row / p.G, head = hk * p.G + q_row - tok * p.G;
-      const float inv = rl == 0.f ? 0.f : 1.f / rl;
-      *reinterpret_cast<u32x2*>(p.o + job.b * p.o_sb + (int64_t)(job.s.first + tok) * p.o_ss + head * p.o_sh +
-                                4 * c4) = u32x2{pack_bf2(sum[0] * inv, sum[1] * inv), pack_bf2(sum[2] * inv, sum[3] * inv)};
-      if (p.lse && c4 == 0)
-        p.lse[job.b * p.lse_sb + head * p.lse_sh + job.s.first + tok] =
-            rl == 0.f ? -INFINITY : (rm + __builtin_amdgcn_logf(rl)) * 0.6931471805599453f;
+  for (int d = 0; d < DB; ++d)
+    *reinterpret_cast<f32x4*>(mine + r * D + (((4 * d + g) ^ (r & 7)) << 2)) = o[d] * weight;
+  __syncthreads();
+  // four channels of a row for each thread of the head
+  for (int i = turn * 64 + lane; i < 16 * D / 4; i += turns * 64) {
+    const int row = i / (D / 4), c4 = i % (D / 4), at = row * D + ((c4 ^ (row & 7)) << 2);
+    const int q_row = job.row0 + row;
+    if (q_row >= job.rows) continue;
+    float rm = M_EMPTY, rl = 0.f;
+    for (int w = in_group; w < 4; w += hw) rm = fmaxf(rm, wave_m[w][row]);
+    f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int w = in_group; w < 4; w += hw) {
+      sum = sum + *reinterpret_cast<const f32x4*>(reinterpret_cast<float*>(images[w]) + at);
+      rl = fmaf(wave_l[w][row], __builtin_amdgcn_exp2f(wave_m[w][row] - rm), rl);
     }
+    if (part) {
+      *reinterpret_cast<f32x4*>(part + row * D + 4 * c4) = sum;
+      if (c4 == 0) {
+        part[M * D + 2 * row] = rm;
+        part[M * D + 2 * row + 1] = rl;
+      }
+      continue;
+    }
+    const int tok = q_row / p.G, head = hk * p.G + q_row - tok * p.G;
+    const float inv = rl == 0.f ? 0.f : 1.f / rl;
+    *reinterpret_cast<u32x2*>(p.o + job.b * p.o_sb + (int64_t)(job.s.first + tok) * p.o_ss + head * p.o_sh +
+                              4 * c4) = u32x2{pack_bf2(sum[0] * inv, sum[1] * inv), pack_bf2(sum[2] * inv, sum[3] * inv)};
+    if (p.lse && c4 == 0)
+      p.lse[job.b * p.lse_sb + head * p.lse_sh + job.s.first + tok] =
+          rl == 0.f ? -INFINITY : (rm + __builtin_amdgcn_logf(rl)) * 0.6931471805599453f;
   }
 }
 
@@ -997,8 +974,10 @@ Plan plan_of(const mi355_paged_attn_args* a) {
   Plan w;
   const int64_t G = a->H / a->Hk, rows = a->max_seqlen_q * G;
   const int64_t all_rows = (a->cu_seqlens_q ? a->Sq : a->Sq * a->B) * G;
-  w.few = rows <= 16 ? 1 : rows <= 32 ? 2 : 0;
-  w.M = w.few ? 16 * w.few : 128;
+  // (two tiles of sixteen rows in the first kernel gain nothing: 32 rows over 8 to 60 thousand keys
+  // take 33 and 116 us there, 23 and 117 us in the second)
+  w.few = rows <= 16;
+  w.M = w.few ? 16 : 128;
   // as many heads to a workgroup as share its four waves: what they read lies side by side
   w.hw = !w.few ? 1 : a->Hk % 4 == 0 ? 4 : a->Hk % 2 == 0 ? 2 : 1;
   const int64_t tiles = all_rows / w.M + a->B;  // row tiles: at most one not full for each sequence
@@ -1041,10 +1020,8 @@ int check(const mi355_paged_attn_args* a) {
 template <int D>
 int launch(const PagedParams& p, const Plan& w, hipStream_t st) {
   const dim3 grid((unsigned)(w.few ? (w.items + 7) / 8 * 8 * (p.Hk / w.hw) : w.items * p.Hk));
-  if (w.few == 1) {
-    hipLaunchKernelGGL((paged_few_rows_kernel<D, 1>), grid, dim3(256), 0, st, p);
-  } else if (w.few == 2) {
-    hipLaunchKernelGGL((paged_few_rows_kernel<D, 2>), grid, dim3(256), 0, st, p);
+  if (w.few) {
+    hipLaunchKernelGGL(paged_few_rows_kernel<D>, grid, dim3(256), 0, st, p);
   } else {
     constexpr int LDS = 4 * KT * D * 2;  // two stages of keys and values
     // the limit of dynamic LDS is an attribute of the function on each device
