@@ -329,7 +329,12 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void paged_few_rows_kernel(Pa
   const unsigned char *k_head = p.kc + hk * p.kc_sh, *v_head = p.vc + hk * p.vc_sh;
   const unsigned k_lane = (unsigned)((lane / CPR) * p.kc_st + (lane % CPR) * 16);
   const unsigned v_lane = (unsigned)((lane / CPR) * p.vc_st + (lane % CPR) * 16);
-  auto once = [](const unsigned char* at) { return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at)); };
+  // past the caches where a head's row is a whole line; two heads of 64 share one, and the second wave
+  // finds it in the cache (8 sequences of 16000, 16 heads of 64: 63 us, past the cache 73)
+  auto once = [](const unsigned char* at) {
+    if constexpr (D == 64) return *reinterpret_cast<const u32x4*>(at);
+    else return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at));
+  };
   auto load_k = [&](const Ahead& a, int t) {
     const int64_t offsets = piece_offsets(p, a, t, p.kc_sb, p.kc_st);
 #pragma unroll
