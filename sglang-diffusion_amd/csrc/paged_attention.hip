@@ -1016,7 +1016,7 @@ int check(const mi355_paged_attn_args* a) {
   MI355_REQUIRE(a->block_size >= 16 && a->block_size <= 1024 && (a->block_size & (a->block_size - 1)) == 0,
                 "paged_attn_fp8: block size %ld must be a power of two in [16, 1024]", (long)a->block_size);
   MI355_REQUIRE(a->num_blocks >= 0 && a->num_blocks < (1ll << 31) && a->table_width >= 0 &&
-                    a->table_width * a->block_size <= (1ll << 31) - 4096 && (a->B <= 1 || a->table_stride >= a->table_width),
+                    a->table_width * a->block_size <= (1ll << 31) - 4096 && a->table_stride >= 0,
                 "paged_attn_fp8: bad page table");
   MI355_REQUIRE(a->window_left < 0 || a->causal, "paged_attn_fp8: a window needs causal masking");
   return MI355_OK;
