@@ -50,6 +50,7 @@ struct PagedParams {
   float scale_log2;
   // items
   int items, chunk_min, split, hw, turns;  // hw: heads of a workgroup, turns: waves of each
+  int by_length;     // items longest first
   float inv_target;
   float* part;       // [Hk * items][M][D + 2]
   int32_t* info;     // [B][2]: first item of the sequence, chunks of each of its row tiles
@@ -84,12 +85,65 @@ struct Item {
   int length;                  // tiles of a chunk
 };
 
+// Items of whole rows (no chunks) of a few sequences with causal rows, longest first: what is left
+// for the last round of workgroups is short then, whatever the sequences' order (prompts of 4096,
+// 1115 and 1341 tokens, 32 heads over 8: 215 us, one sequence after the other 224).  Row tiles are put in order by
+// the place of their last row, in levels of `unit` tiles of keys.  Lanes count the tiles at and above
+// 64 levels at a time: two rounds find the level of the item, a walk over the sequences its tile.
+constexpr int SORTED_SEQS = 16;
+template <int M>
+__device__ __forceinline__ void find_longest(const PagedParams& p, int item, Item* found) {
+  const int lane = threadIdx.x;
+  const Seq s = seq_of(p, min(lane, p.B - 1));
+  const int base = s.len - s.n, tiles = (s.n * p.G + M - 1) / M;
+  // levels there are, at most, in tiles of keys; step <= 33
+  const int most = __builtin_amdgcn_readfirstlane((int)group_max<64>((float)(s.len >> 6))) + 2;
+  const int unit = (most >> 11) + 1, step = (most / unit + 64) >> 6;
+  // tiles of sequence b whose last row is at level x or above: the last tile if x begins before the
+  // end, and those from row (x's place - base) G on
+  auto upper = [&](int b, int x) {
+    const int rb = __builtin_amdgcn_readlane(base, b), rt = __builtin_amdgcn_readlane(tiles, b);
+    const unsigned at = (unsigned)x * unit * KT;
+    if (x == 0) return rt;
+    if (at >= (unsigned)__builtin_amdgcn_readlane(s.len, b)) return 0;
+    const int first = (int)at > rb ? ((int)at - rb) * p.G / M : 0;
+    return rt - min(max(rt - 1, 0), first);
+  };
+  auto above = [&](int x) {
+    int n = 0;
+    for (int b = 0; b < p.B; ++b) n += upper(b, x);
+    return n;
+  };
+  int level = 0;
+#pragma unroll 1
+  for (int s2 = step; s2; s2 = s2 > 1 ? 1 : 0) {
+    const int n = __popcll(__builtin_amdgcn_ballot_w64(above(level + lane * s2) > item));
+    if (n == 0) {  // behind the last item
+      if (lane == 0) found->b = -1;
+      return;
+    }
+    level += (n - 1) * s2;
+  }
+  int k = item - above(level + 1);
+  for (int b = 0; b < p.B; ++b) {
+    const int from = upper(b, level), n = from - upper(b, level + 1);
+    if (k < n) {
+      const int rt = __builtin_amdgcn_readlane(tiles, b);
+      if (lane == b) *found = Item{s, b, rt - from + k, 0, 1, 1 << 30};
+      return;
+    }
+    k -= n;
+  }
+}
+
 // The item'th item of a key/value head, for the whole workgroup; false behind the last one.  One
 // wave adds up the sequences, `per` that follow each other to a lane, and hands the item on.
 template <int M>
 __device__ bool find_item(const PagedParams& p, int item, int group, Item* out) {
   __shared__ Item found;
-  if (threadIdx.x < 64) {
+  if (p.by_length) {
+    if (threadIdx.x < 64) find_longest<M>(p, item, &found);
+  } else if (threadIdx.x < 64) {
     const int lane = threadIdx.x;
     const int per = (p.B + 63) >> 6;
     const int b0 = lane * per, b1 = min(p.B, b0 + per);
@@ -1121,6 +1175,7 @@ extern "C" int mi355_paged_attn_fp8(const mi355_paged_attn_args* a, void* stream
   p.inv_target = 1.f / (float)w.target;
   p.chunk_min = w.chunk_min;
   p.split = w.split;
+  p.by_length = !w.few && !w.split && a->causal && a->B > 1 && a->B <= SORTED_SEQS;
   p.hw = w.hw;
   p.turns = w.few ? 4 / w.hw : 1;
   p.part = (float*)a->workspace;

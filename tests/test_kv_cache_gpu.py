@@ -442,6 +442,17 @@ def test_attend_prompts(device, new, lens, H, Hk, block, D):
     c.check(causal=False)
 
 
+@pytest.mark.parametrize("new,lens,H,Hk", [
+    ([1500, 100, 0, 2000, 700, 1], [1500, 900, 5, 2100, 700, 3], 64, 32),     # longest first
+    ([130] * 3 + [260] * 14, [130] * 3 + list(range(260, 1660, 100)), 64, 32),  # more than are put in order
+    ([1500, 1900, 40], [1300, 1900, 0], 64, 64),                               # rows before the first key
+])
+def test_attend_enough_prompts_to_leave_keys_whole(device, new, lens, H, Hk):
+    c = Case(new, lens, H, Hk, 64, 64, 16)
+    c.check()
+    c.check(window=333)
+
+
 def test_attend_rows_that_see_nothing(device):
     """No keys at all, and more new tokens than the cache holds: the first stand before its start."""
     for new, lens in (([1, 1, 1], [0, -4, 5]), ([6, 2], [3, 0]), ([90, 40], [70, 0])):
