@@ -475,9 +475,11 @@ int mi355_merge_attn_states(void* out, float* out_lse, const void* a, const floa
  *   positions int64 [max_tokens]  place of the token in its sequence; 0 behind the last one
  *   free_end int32 [1]  free_begin + blocks taken
  *   status int32 [3]  blocks that the free list lacks, tokens beyond max_tokens, requests that
- *     outgrow table_width (counts saturate).  If any is not 0 nothing is given to anybody: the table is left as it
- *     was, seq_lens = context_lens, all slots -1, cu_seqlens_q 0, free_end = free_begin.
- * seq_lens and free_end must not be the memory of an input.  B <= 4096. */
+ *     outgrow table_width (counts saturate).  If any is not 0 nothing is given to anybody: the
+ *     table is left as it was, seq_lens = context_lens, all slots -1, cu_seqlens_q 0,
+ *     free_end = free_begin.
+ * Outputs must not share memory with inputs or with each other.  B <= 4096, and rows of the table
+ * hold at most 2^31 - 4096 tokens. */
 int mi355_kv_block_plan(const int32_t* context_lens, const int32_t* new_lens, int64_t B,
                         int32_t* block_table, int64_t table_stride, int64_t table_width,
                         const int32_t* free_blocks, int64_t num_free, const int32_t* free_begin,
@@ -509,7 +511,8 @@ int mi355_rope_scaled(const int64_t* positions, const void* q, void* q_out, cons
  * in the block; a slot is given once.
  * positions != NULL: keys are first rotated as by mi355_rope_scaled (and rounded to bf16), and
  * the queries q (Hq heads, or 0) are rotated into q_out in the same launch.
- * k, v [tokens, Hk, D] bf16, D 64 or 128; strides in elements (of the cache: bytes). */
+ * k, v [tokens, Hk, D] bf16, D 64 or 128; strides in elements (of the cache: bytes), multiples of
+ * 8; k, v, q, q_out 16-byte aligned, the caches 8-byte. */
 typedef struct {
   const void* k;
   const void* v;
@@ -541,11 +544,13 @@ int mi355_kv_store_fp8(const mi355_kv_store_args* args, void* stream);
  * nothing gives 0 and a log-sum-exp of -infinity.
  * q, out bf16: [Sq, H, D] packed with cu_seqlens_q int32 [B + 1] (rows behind the last sequence
  * are left as they are), or [B, Sq, H, D] with cu_seqlens_q == NULL.  lse fp32 or NULL, element
- * (row, head) at b * lse_sb + head * lse_sh + row.  max_seqlen_q chooses the kernel; any value is
+ * (row, head) at b * lse_sb + head * lse_sh + row.  out may be q.  max_seqlen_q chooses the kernel; any value is
  * right.  Lengths beyond the table count as its length; entries of the table that are not in
  * [0, num_blocks) are skipped as if their tokens were masked; entries behind a sequence's end are
  * not read.  Scales are positive, value scales between 2^-64 and 2^120.
- * D 64 or 128.  workspace: mi355_paged_attn_workspace_bytes(args) of device memory (16-byte
+ * D 64 or 128; strides of q and out multiples of 8 elements, those of the caches multiples of 16
+ * bytes (the token's below 2^24), q, out and the caches 16-byte aligned; a table row holds at most
+ * 2^31 - 4096 tokens, rows of the table may be one row.  workspace: mi355_paged_attn_workspace_bytes(args) of device memory (16-byte
  * aligned, no initial contents) that no other call in flight uses. */
 typedef struct {
   const void* q;

@@ -520,6 +520,11 @@ __global__ __launch_bounds__(256, 4) void kv_store_kernel(StoreParams p) {
   }
 }
 
+// rows that are written must not be the same ones (an expanded tensor's are)
+bool rows_apart(int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t D) {
+  return (n0 <= 1 || s0 >= D) && (n1 <= 1 || s1 >= D);
+}
+
 bool rope_args_ok(const char* what, int64_t head_size, int64_t rot_dim, const void* inv_freq,
                   const int64_t* positions, int64_t tokens) {
   if (tokens && (!positions || !inv_freq)) {
@@ -548,7 +553,8 @@ extern "C" int mi355_kv_block_plan(const int32_t* context_lens, const int32_t* n
   MI355_REQUIRE(block_size_ok(block_size), "kv_block_plan: block size %ld must be a power of two in [16, 1024]",
                 (long)block_size);
   MI355_REQUIRE(max_tokens >= 0 && max_tokens <= (1ll << 31) - 4096 && num_free >= 0 && num_free < (1ll << 31) &&
-                    num_blocks >= 0 && num_blocks < (1ll << 31) && table_width >= 0 &&
+                    num_blocks >= 0 && num_blocks < (1ll << 31) && table_width >= 0 && table_width < (1ll << 31) &&
+                    table_width * block_size <= (1ll << 31) - 4096 && table_stride < (1ll << 40) &&
                     (B <= 1 || table_stride >= table_width),
                 "kv_block_plan: bad size");
   MI355_REQUIRE(free_begin && cu_seqlens_q && free_end && status, "kv_block_plan: null pointer");
@@ -556,10 +562,25 @@ extern "C" int mi355_kv_block_plan(const int32_t* context_lens, const int32_t* n
                 "kv_block_plan: null pointer");
   MI355_REQUIRE(max_tokens == 0 || (slot_mapping && positions), "kv_block_plan: null pointer");
   MI355_REQUIRE(num_free == 0 || free_blocks, "kv_block_plan: null pointer");
-  // every workgroup reads these while the first one writes those
-  MI355_REQUIRE((const void*)free_end != free_begin && (B == 0 || ((const void*)seq_lens != context_lens &&
-                (const void*)seq_lens != new_lens)),
-                "kv_block_plan: seq_lens and free_end must not share memory with the inputs");
+  // every workgroup reads the inputs, some while others write already
+  struct Span {
+    const void* at;
+    int64_t bytes;
+  };
+  const Span in[] = {{context_lens, 4 * B}, {new_lens, 4 * B}, {free_blocks, 4 * num_free}, {free_begin, 4},
+                     {block_table, B ? 4 * ((B - 1) * table_stride + table_width) : 0}};
+  const Span out[] = {{cu_seqlens_q, 4 * (B + 1)}, {seq_lens, 4 * B}, {free_end, 4}, {status, 12},
+                      {slot_mapping, 8 * max_tokens}, {positions, 8 * max_tokens}};
+  auto apart = [](const Span& a, const Span& b) {
+    return a.bytes == 0 || b.bytes == 0 || (uintptr_t)a.at + a.bytes <= (uintptr_t)b.at ||
+           (uintptr_t)b.at + b.bytes <= (uintptr_t)a.at;
+  };
+  bool clear = apart(in[2], in[4]);  // the table is written as well
+  for (const Span& o : out) {
+    for (const Span& i : in) clear = clear && apart(o, i);
+    for (const Span& o2 : out) clear = clear && (&o == &o2 || apart(o, o2));
+  }
+  MI355_REQUIRE(clear, "kv_block_plan: outputs must not share memory with inputs or with each other");
   PlanParams p = {context_lens, new_lens, free_blocks, free_begin, block_table, cu_seqlens_q, seq_lens,
                   free_end, status, slot_mapping, positions, table_stride, table_width, num_free, num_blocks,
                   max_tokens, (int)B, log2_of(block_size)};
@@ -589,6 +610,9 @@ extern "C" int mi355_rope_scaled(const int64_t* positions, const void* q, void* 
     MI355_REQUIRE(s % 8 == 0, "rope_scaled: strides must be multiples of 8 elements");
   MI355_REQUIRE(((uintptr_t)q | (uintptr_t)q_out | (uintptr_t)k | (uintptr_t)k_out) % 16 == 0,
                 "rope_scaled: rows must be 16-byte aligned");
+  MI355_REQUIRE((Hq == 0 || rows_apart(tokens, qo_st, Hq, qo_sh, head_size)) &&
+                    (Hk == 0 || rows_apart(tokens, ko_st, Hk, ko_sh, head_size)),
+                "rope_scaled: rows of an output overlap each other");
   Rope r = {positions, inv_freq, inv_freq_is_f64, (int)(rot_dim / 2), is_neox != 0, attn_factor};
   RopeRows a = {(const unsigned short*)q, (unsigned short*)q_out, q_st, q_sh, qo_st, qo_sh, (int)Hq};
   RopeRows b = {(const unsigned short*)k, (unsigned short*)k_out, k_st, k_sh, ko_st, ko_sh, (int)Hk};
@@ -624,6 +648,11 @@ extern "C" int mi355_kv_store_fp8(const mi355_kv_store_args* a, void* stream) {
     return MI355_EINVAL;
   MI355_REQUIRE(a->Hq == 0 || (turn_keys && a->q && a->q_out),
                 "kv_store_fp8: queries need positions and both their pointers");
+  MI355_REQUIRE((a->Hq == 0 || rows_apart(a->tokens, a->qo_st, a->Hq, a->qo_sh, a->D)) &&
+                    rows_apart(a->block_size, a->kc_st, a->Hk, a->kc_sh, a->D) &&
+                    rows_apart(a->block_size, a->vc_st, a->Hk, a->vc_sh, a->D) &&
+                    rows_apart(a->num_blocks, a->kc_sb, a->num_blocks, a->vc_sb, a->D),
+                "kv_store_fp8: rows of an output overlap each other");
   StoreParams p;
   p.k = (const unsigned short*)a->k;
   p.v = (const unsigned short*)a->v;

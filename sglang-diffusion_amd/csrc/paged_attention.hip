@@ -1131,6 +1131,10 @@ extern "C" int mi355_paged_attn_fp8(const mi355_paged_attn_args* a, void* stream
   const int64_t strides[] = {a->q_sb, a->q_ss, a->q_sh, a->o_sb, a->o_ss, a->o_sh};
   for (int64_t s : strides)
     MI355_REQUIRE(s % 8 == 0, "paged_attn_fp8: strides of q and out must be multiples of 8 elements");
+  const bool batched = a->cu_seqlens_q == nullptr;
+  MI355_REQUIRE((!batched || a->B <= 1 || a->o_sb >= a->D) && (a->Sq <= 1 || a->o_ss >= a->D) &&
+                    (a->H <= 1 || a->o_sh >= a->D),
+                "paged_attn_fp8: rows of out overlap each other");
   const int64_t cache_strides[] = {a->kc_sb, a->kc_st, a->kc_sh, a->vc_sb, a->vc_st, a->vc_sh};
   for (int64_t s : cache_strides)
     MI355_REQUIRE(s % 16 == 0, "paged_attn_fp8: strides of the caches must be multiples of 16 bytes");

@@ -23,7 +23,8 @@ def kv_block_plan(context_lens: torch.Tensor, new_lens: torch.Tensor, block_tabl
     are lacking, tokens that `slot_mapping` has no room for, requests that outgrow their row.  If any
     of them is not 0, nothing is given to anybody: the table stays, every slot is -1,
     `seq_lens` = `context_lens` and `free_end` = `free_begin`.
-    `seq_lens` and `free_end` are other memory than the inputs; copy them back for the next step."""
+    Outputs are other memory than the inputs; copy `seq_lens` and `free_end` back for the next step.
+    At most 4096 requests in one call."""
     torch.ops.sgl_kernel.kv_block_plan.default(
         context_lens, new_lens, block_table, free_blocks, free_begin, block_size, num_blocks, slot_mapping,
         positions, cu_seqlens_q, seq_lens, free_end, status)

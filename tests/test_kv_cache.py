@@ -214,6 +214,8 @@ def test_c_abi_refuses_before_any_launch():
     assert "aligned" in attn(k_cache=24)
     assert "page table" in attn(table_width=1 << 28)
     assert "too large" in attn(kc_st=1 << 24)
+    assert "overlap" in attn(o_ss=0) and "overlap" in attn(o_sh=0)
+    assert "overlap" in attn(cu_seqlens_q=None, o_sb=0)
     assert "workspace" in attn(table_width=1 << 16, table_stride=1 << 16)
     assert "null args" in (lib.mi355_paged_attn_fp8(None, None), last_error())[1]
     b = _C.PagedAttnArgs()
@@ -238,6 +240,9 @@ def test_c_abi_refuses_before_any_launch():
     assert "null" in store(k=None)
     assert "null" in store(k_scale=None)
     assert "multiples of 8" in store(kc_st=100)
+    for name in ("kc_sb", "kc_st", "kc_sh", "vc_sb", "vc_st", "vc_sh"):
+        assert "overlap" in store(**{name: 0})
+    assert "overlap" in store(Hq=3, q=16, q_out=16, positions=16, inv_freq=16, rot_dim=64, qo_sh=64)
     assert "aligned" in store(v=24)
     assert "queries need" in store(Hq=3, q=16, q_out=16)
     assert "rot_dim" in store(positions=16, inv_freq=16, rot_dim=24)
@@ -245,26 +250,36 @@ def test_c_abi_refuses_before_any_launch():
     s.tokens = 0
     assert lib.mi355_kv_store_fp8(ctypes.byref(s), None) == 0
 
-    def rope(D=64, rot=64, st=256, ptr=16):
-        rc = lib.mi355_rope_scaled(16, ptr, 16, None, None, 5, 4, 0, D, rot, st, 64, 256, 64, 0, 0, 0, 0, 16, 1, 1.0, 1,
-                                   None)
+    def rope(D=64, rot=64, st=256, ptr=16, out_st=256):
+        rc = lib.mi355_rope_scaled(16, ptr, 16, None, None, 5, 4, 0, D, rot, st, 64, out_st, 64, 0, 0, 0, 0, 16, 1, 1.0,
+                                   1, None)
         assert rc == -1
         return last_error()
 
     assert "rot_dim" in rope(rot=128) and "rot_dim" in rope(rot=40) and "rot_dim" in rope(rot=0)
     assert "head size" in rope(D=264, rot=64) and "head size" in rope(D=60, rot=16)
-    assert "multiples of 8" in rope(st=255) and "aligned" in rope(ptr=8)
+    assert "multiples of 8" in rope(st=255) and "aligned" in rope(ptr=8) and "overlap" in rope(out_st=0)
 
-    def plan(B=2, block=16, width=4, stride=4, seq_lens=48, free_end=64, room=6):
-        rc = lib.mi355_kv_block_plan(16, 32, B, 80, stride, width, 96, 9, 112, block, 20, 128, 144, room, 160, seq_lens,
-                                     free_end, 176, None)
+    # inputs and outputs 4096 bytes apart, except those named
+    names = ["context", "new", "table", "free", "begin", "slots", "positions", "cu", "seq_lens", "free_end", "status"]
+
+    def plan(B=2, block=16, width=4, stride=4, room=6, **at):
+        p = {n: at.get(n, 4096 * (i + 1)) for i, n in enumerate(names)}
+        rc = lib.mi355_kv_block_plan(p["context"], p["new"], B, p["table"], stride, width, p["free"], 9, p["begin"], block,
+                                     20, p["slots"], p["positions"], room, p["cu"], p["seq_lens"], p["free_end"],
+                                     p["status"], None)
         assert rc == -1
         return last_error()
 
     assert "at most" in plan(B=4097) and "power of two" in plan(block=48)
-    assert "bad size" in plan(stride=3) and "bad size" in plan(room=1 << 31)
-    assert "share memory" in plan(seq_lens=16) and "share memory" in plan(seq_lens=32)
-    assert "share memory" in plan(free_end=112)
+    assert "bad size" in plan(stride=3) and "bad size" in plan(room=1 << 31) and "bad size" in plan(width=1 << 27)
+    assert "null" in plan(cu=None) and "null" in plan(slots=None) and "null" in plan(table=None)
+    for out, size in (("slots", 48), ("positions", 48), ("cu", 12), ("seq_lens", 8), ("free_end", 4), ("status", 12)):
+        for n in names:
+            if n != out:
+                assert "share memory" in plan(**{out: 4096 * (names.index(n) + 1)})
+        assert "share memory" in plan(**{out: 4096 - size + 4})       # the context's first length
+    assert "share memory" in plan(free=4096 * 3 + 28)                 # the table's last entry
 
 
 def test_shapes_under_tracing():

@@ -65,7 +65,8 @@ def make_plan(B, block, new_hi, ctx_hi, seed, room=7, spare=3, begin=2):
 
 
 @pytest.mark.parametrize("B,block,new_hi,ctx_hi", [(1, 16, 1, 40), (5, 16, 1, 100), (64, 32, 3, 500), (3, 64, 900, 0),
-                                                   (257, 16, 20, 60), (700, 128, 9, 300), (1500, 16, 2, 5)])
+                                                   (257, 16, 20, 60), (700, 128, 9, 300), (1500, 16, 2, 5),
+                                                   (4096, 16, 3, 40)])
 def test_plan(device, B, block, new_hi, ctx_hi):
     got = run_plan(*make_plan(B, block, new_hi, ctx_hi, B))
     assert got[-1] == [0, 0, 0]
@@ -451,6 +452,76 @@ def test_attend_enough_prompts_to_leave_keys_whole(device, new, lens, H, Hk):
     c = Case(new, lens, H, Hk, 64, 64, 16)
     c.check()
     c.check(window=333)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("H,Hk", [(8, 1), (9, 3), (4, 4), (32, 8), (6, 6)])
+def test_attend_long_cache_for_each_number_of_heads(device, H, Hk, D):
+    """Heads side by side in a workgroup and waves that take turns, over keys that are split."""
+    c = Case([1, 2, 1], [2500, 700, 4000], H, Hk, D, 32, 17)
+    c.check()
+    c.check(window=1000)
+
+
+@pytest.mark.parametrize("B,new,block", [(300, 1, 16), (300, 4, 64), (130, 40, 16)])
+def test_attend_many_sequences(device, B, new, block):
+    """More sequences than lanes, short and long."""
+    g = torch.Generator().manual_seed(B)
+    lens = torch.exp(torch.rand(B, generator=g) * 6.5).int().tolist()
+    lens[7], lens[-1] = 3000, 0
+    Case([new] * B, lens, 4, 2, 64, block, 18).check()
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [5, 1, 40], [130, 7, 1]])
+def test_attend_whatever_the_largest_length_is_said_to_be(device, new):
+    c = Case(new, [600, 90, 333], 4, 2, 128, 16, 19)
+    want = c.want()
+    for said in (1, 5, 5000, None):
+        c.compare(*c.call(max_seqlen_q=said), want)
+
+
+@pytest.mark.parametrize("new", [[1] * 4, [30] * 4])
+def test_attend_shared_blocks_and_one_length(device, new):
+    """Sequences that begin with the same blocks (a prompt in common), a table of one row for all,
+    and cache_seqlens as one int."""
+    c = Case(new, [200] * 4, 4, 2, 64, 16, 20)
+    c.table[:, :9] = c.table[0, :9]
+    c.check()
+    c.table = c.table[:1].expand(4, -1)
+    table = c.table[:1].to(DEV).expand(4, -1)
+    assert table.stride(0) == 0
+    c.compare(*c.call(page_table=table, cache_seqlens=200), c.want())
+
+
+def test_attend_nothing(device):
+    """No sequences, no tokens, a table without columns, a pool without blocks."""
+    c = Case([1, 3], [40, 70], 4, 2, 64, 16, 21)
+    got, lse = c.call(q=torch.empty(0, 4, 64, dtype=torch.bfloat16, device=DEV), cu_seqlens_q=i32([0, 0, 0]))
+    assert got.shape == (0, 4, 64) and lse.shape == (4, 0)
+    got, lse = c.call(q=torch.empty(0, 3, 4, 64, dtype=torch.bfloat16, device=DEV), cache_seqlens=i32([]),
+                      page_table=torch.empty(0, 5, dtype=torch.int32, device=DEV))
+    assert got.shape == (0, 3, 4, 64) and lse.shape == (0, 4, 3)
+    empty = torch.empty(2, 0, dtype=torch.int32, device=DEV)
+    got, lse = c.call(page_table=empty)
+    assert (got == 0).all() and (lse == -math.inf).all()
+    c.dev = [x[:0] for x in c.dev]
+    got, lse = c.call(page_table=empty, k_descale=torch.empty(0, 2, device=DEV), v_descale=torch.empty(0, 2, device=DEV))
+    assert (got == 0).all() and (lse == -math.inf).all()
+
+
+def test_attend_into_the_memory_of_q(device):
+    """`out` may be q itself: a row is read before it is written."""
+    import sgl_kernel  # noqa: F401
+
+    for new in ([1, 1], [3, 2], [100, 60]):
+        c = Case(new, [3000, 400], 8, 2, 128, 32, 22)
+        want, lse = c.check()
+        q = c.q.to(DEV)
+        got, lse2, *_ = torch.ops.sgl_kernel.fwd.default(
+            q, *c.dev, None, None, None, q, i32(c.cu), None, None, None, i32(c.lens), max(new), None, c.table.to(DEV),
+            None, None, None, None, None, None, c.scales[0].to(DEV), c.scales[1].to(DEV), None, True, -1, -1, 0, 0.0,
+            False, None, 0, None, 0, None)
+        assert got.data_ptr() == q.data_ptr() and torch.equal(q, want) and torch.equal(lse, lse2)
 
 
 def test_attend_rows_that_see_nothing(device):
