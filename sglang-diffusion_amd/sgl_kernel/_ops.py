@@ -62,6 +62,9 @@ SCHEMAS = {
            "Tensor? sinks) -> (Tensor, Tensor, Tensor, Tensor)",
     # the paged 8-bit cache that `fwd` reads through page_table: ops of this package, in the
     # conventions of the ones above
+    "fwd_paged_fp8": "(Tensor q, Tensor k_cache, Tensor v_cache, Tensor? k_descale, Tensor? v_descale, "
+                     "Tensor page_table, Tensor? cache_seqlens, Tensor? cu_seqlens_q, int? max_seqlen_q, "
+                     "float? softmax_scale, bool causal, int window_left, int window_right) -> (Tensor, Tensor)",
     "kv_block_plan": "(Tensor context_lens, Tensor new_lens, Tensor! block_table, Tensor free_blocks, "
                      "Tensor free_begin, int block_size, int num_blocks, Tensor! slot_mapping, "
                      "Tensor! positions, Tensor! cu_seqlens_q, Tensor! seq_lens, Tensor! free_end, "
@@ -237,7 +240,7 @@ def _fwd(q, k, v, k_new, v_new, q_v, out, cu_seqlens_q, cu_seqlens_k, cu_seqlens
          rotary_sin, seqlens_rotary, q_descale, k_descale, v_descale, softmax_scale, is_causal,
          window_left, window_right, attention_chunk, softcap, is_rotary_interleaved,
          scheduler_metadata, num_splits, pack_gqa, sm_margin, sinks):
-    """With page_table and e4m3 caches: attention over a paged 8-bit cache (_fwd_paged).  Otherwise
+    """With page_table and e4m3 caches: attention over a paged 8-bit cache (fwd_paged_fp8).  Otherwise
     dense non-causal attention, the only form the diffusion path issues
     (python/sglang/multimodal_gen/runtime/layers/attention/backends/flash_attn.py:517-563).
     Batched [B,S,H,d] inputs, or packed [T,H,d] inputs whose sequences all have the maximum
@@ -251,8 +254,10 @@ def _fwd(q, k, v, k_new, v_new, q_v, out, cu_seqlens_q, cu_seqlens_k, cu_seqlens
             _fail("fwd: arguments not supported with a paged 8-bit cache: "
                   f"{[n for n, t in other.items() if t is not None]}")
         _require(attention_chunk == 0 and softcap == 0.0, "fwd: attention_chunk / softcap are not implemented")
-        return _fwd_paged(q, k, v, out, cu_seqlens_q, seqused_k, max_seqlen_q, page_table, k_descale, v_descale,
-                          softmax_scale, is_causal, window_left, window_right)
+        out, lse = _fwd_paged_fp8(q, k, v, k_descale, v_descale, page_table, seqused_k, cu_seqlens_q, max_seqlen_q,
+                                  softmax_scale, is_causal, window_left, window_right, out)
+        empty = lse.new_empty(0)
+        return out, lse, empty, empty
     unsupported = dict(k_new=k_new, v_new=v_new, q_v=q_v, cu_seqlens_k_new=cu_seqlens_k_new,
                        seqused_q=seqused_q, seqused_k=seqused_k, page_table=page_table,
                        kv_batch_idx=kv_batch_idx, leftpad_k=leftpad_k, rotary_cos=rotary_cos,
@@ -312,6 +317,13 @@ def _fail(msg):
     raise RuntimeError(msg)
 
 
+_ONE = (1,)
+
+
+def _dense(t, dtype, shape, device):
+    return t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == device
+
+
 def _check_cache(what, cache, scale, name, like):
     if not (cache.dtype == FP8 and cache.dim() == 4 and cache.stride(3) == 1):
         _fail(f"{what}: {name}_cache must be [blocks, block_size, heads, head_size] float8_e4m3fn with a "
@@ -351,15 +363,14 @@ def _check_inv_freq(what, inv_freq, like):
         _fail(f"{what}: inv_freq must be a contiguous 1-D float64 or float32 tensor on {like.device}")
 
 
-def _fwd_paged(q, k_cache, v_cache, out, cu_seqlens_q, cache_seqlens, max_seqlen_q, page_table, k_descale, v_descale,
-               softmax_scale, is_causal, window_left, window_right):
-    shape = q.shape
-    packed = len(shape) == 3
-    if not (q.dtype == torch.bfloat16 and (packed or len(shape) == 4) and q.stride(-1) == 1):
+def _check_fwd_paged(q, k_cache, v_cache, k_descale, v_descale, page_table, cache_seqlens, cu_seqlens_q, is_causal,
+                     window_left, window_right):
+    packed = q.dim() == 3
+    if not (q.dtype == torch.bfloat16 and (packed or q.dim() == 4) and q.stride(-1) == 1):
         _fail("fwd: q must be bfloat16 [T,H,d] or [B,S,H,d] with a contiguous last dimension")
     _check_cache("fwd", k_cache, k_descale, "k", q)
     _check_cache("fwd", v_cache, v_descale, "v", q)
-    if not (v_cache.shape == k_cache.shape and k_cache.shape[3] == shape[-1]):
+    if not (v_cache.shape == k_cache.shape and k_cache.shape[3] == q.shape[-1]):
         _fail("fwd: k_cache and v_cache must have one shape, with the head size of q")
     if cache_seqlens is None:
         _fail("fwd: a paged cache needs the sequences' lengths (cache_seqlens)")
@@ -371,34 +382,53 @@ def _fwd_paged(q, k_cache, v_cache, out, cu_seqlens_q, cache_seqlens, max_seqlen
         _check_ints("fwd", q, torch.int32, cache_seqlens=cache_seqlens, cu_seqlens_q=cu_seqlens_q)
         if cu_seqlens_q.numel() != B + 1:
             _fail("fwd: cu_seqlens_q and cache_seqlens disagree")
-        if max_seqlen_q is None:
-            max_seqlen_q = shape[0]
     else:
         _check_ints("fwd", q, torch.int32, cache_seqlens=cache_seqlens)
-        if cu_seqlens_q is not None or shape[0] != B:
+        if cu_seqlens_q is not None or q.shape[0] != B:
             _fail("fwd: batched q needs one sequence for each length and no cu_seqlens_q")
-        max_seqlen_q = shape[1]
-    H, Hk = shape[-2], k_cache.shape[2]
+    H, Hk = q.shape[-2], k_cache.shape[2]
     if not (Hk > 0 and H > 0 and H % Hk == 0):
         _fail("fwd: the heads of q must be a multiple of the cache's")
     if not (window_left < 0 and window_right < 0 or is_causal and window_right in (-1, 0)):
         _fail("fwd: sliding windows need causal attention, and end at the token itself")
+
+
+def _fwd_paged_fp8(q, k_cache, v_cache, k_descale, v_descale, page_table, cache_seqlens, cu_seqlens_q, max_seqlen_q,
+                   softmax_scale, is_causal, window_left, window_right, out=None):
+    shape, cache, dev = q.shape, k_cache.shape, q.get_device()
+    packed = len(shape) == 3
+    # the usual call in few steps; whatever is not that is looked at one by one
+    scales = cache[0::2]
+    if not (q.dtype is torch.bfloat16 and k_cache.dtype is FP8 and v_cache.dtype is FP8 and packed and len(cache) == 4
+            and v_cache.shape == cache and cache[3] == shape[2] and shape[1] % max(cache[2], 1) == 0 and shape[1] > 0
+            and q.stride(2) == 1 and k_cache.stride(3) == 1 and v_cache.stride(3) == 1
+            and (window_left < 0 and window_right < 0 or is_causal and -1 <= window_right <= 0) and k_descale is not None and v_descale is not None and cu_seqlens_q is not None
+            and cache_seqlens is not None and _dense(k_descale, torch.float32, scales, dev) and _dense(v_descale, torch.float32, scales, dev)
+            and page_table.dtype is torch.int32 and page_table.stride()[1:] == _ONE
+            and _dense(cache_seqlens, torch.int32, page_table.shape[:1], dev)
+            and _dense(cu_seqlens_q, torch.int32, (page_table.shape[0] + 1,), dev)
+            and k_cache.get_device() == v_cache.get_device() == page_table.get_device() == dev):
+        _check_fwd_paged(q, k_cache, v_cache, k_descale, v_descale, page_table, cache_seqlens, cu_seqlens_q, is_causal,
+                         window_left, window_right)
+    B = page_table.shape[0]
     device = q.device
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif not (out.shape == shape and out.dtype == q.dtype and out.stride(-1) == 1 and out.device == device):
         _fail("fwd: out must match q")
     if packed:
-        lse = torch.empty(H, shape[0], dtype=torch.float32, device=device)
+        lse = torch.empty(shape[1], shape[0], dtype=torch.float32, device=device)
+        if max_seqlen_q is None:
+            max_seqlen_q = shape[0]
     else:
-        lse = torch.empty(B, H, shape[1], dtype=torch.float32, device=device)
+        lse = torch.empty(B, shape[2], shape[1], dtype=torch.float32, device=device)
+        max_seqlen_q = shape[1]
     if softmax_scale is None:
         softmax_scale = shape[-1] ** -0.5
     if q.numel() and B:
         _C.paged_attention_fp8(q, k_cache, v_cache, k_descale, v_descale, page_table, cache_seqlens, cu_seqlens_q,
                                max_seqlen_q, out, lse, softmax_scale, is_causal, window_left)
-    empty = lse.new_empty(0)
-    return out, lse, empty, empty
+    return out, lse
 
 
 # --------------------------------------------------------------------- paged 8-bit KV cache --
@@ -502,6 +532,7 @@ _IMPLS = {
     "rotary_embedding": _rotary_embedding,
     "apply_rope_pos_ids_cos_sin_cache": _apply_rope_pos_ids_cos_sin_cache,
     "fwd": _fwd,
+    "fwd_paged_fp8": _fwd_paged_fp8,
 }
 for _name, _fn in _IMPLS.items():
     _lib.impl(_name, _fn, "CUDA")
@@ -526,6 +557,11 @@ for _name in ("sgl_per_token_quant_fp8", "sgl_per_token_group_quant_8bit", "sgl_
               "rmsnorm", "fused_add_rmsnorm", "rotary_embedding", "apply_rope_pos_ids_cos_sin_cache",
               "merge_state_v2", "kv_block_plan", "rotary_embedding_scaled", "store_kv_cache_fp8"):
     torch.library.register_fake("sgl_kernel::" + _name)(_fake_none)
+
+
+@torch.library.register_fake("sgl_kernel::fwd_paged_fp8")
+def _fake_fwd_paged_fp8(q, *rest, **kw):
+    return _fake_fwd(q, None, None, None, None, None, None, None, None)[:2]
 
 
 @torch.library.register_fake("sgl_kernel::fwd")

@@ -1,6 +1,6 @@
 """`flash_attn_varlen_func` with the reference's signature
 (sgl-kernel/python/sgl_kernel/flash_attn.py:228-311), and `flash_attn_with_kvcache` beside it, issuing
-`torch.ops.sgl_kernel.fwd`."""
+`torch.ops.sgl_kernel.fwd` and `fwd_paged_fp8`."""
 from __future__ import annotations
 
 import torch
@@ -59,13 +59,19 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, qv=None, rotary
         raise RuntimeError("flash_attn_with_kvcache: only paged caches are implemented (page_table)")
     if k_cache.dtype != torch.float8_e4m3fn:
         raise RuntimeError("flash_attn_with_kvcache: only float8_e4m3fn caches are implemented")
+    if not (k is None and v is None and qv is None and rotary_cos is None and rotary_sin is None
+            and cache_batch_idx is None and cache_leftpad is None and cu_seqlens_k_new is None
+            and rotary_seqlens is None and q_descale is None and sinks is None and attention_chunk in (None, 0)
+            and softcap == 0.0):
+        raise RuntimeError("flash_attn_with_kvcache: k / v / qv / rotary_* / cache_batch_idx / cache_leftpad / "
+                           "cu_seqlens_k_new / q_descale / sinks / attention_chunk / softcap are not implemented for "
+                           "an 8-bit cache")
     if isinstance(cache_seqlens, int):
         cache_seqlens = torch.full((page_table.shape[0],), cache_seqlens, dtype=torch.int32, device=q.device)
-    out, softmax_lse, *rest = torch.ops.sgl_kernel.fwd.default(
-        q, k_cache, v_cache, k, v, qv, None, cu_seqlens_q, None, cu_seqlens_k_new, None, cache_seqlens,
-        max_seqlen_q, None, page_table, cache_batch_idx, cache_leftpad, rotary_cos, rotary_sin, rotary_seqlens,
-        q_descale, k_descale, v_descale, softmax_scale, causal, window_size[0], window_size[1],
-        0 if attention_chunk is None else int(attention_chunk), softcap,
-        is_rotary_interleaved=rotary_interleaved, scheduler_metadata=scheduler_metadata, num_splits=num_splits,
-        pack_gqa=pack_gqa, sm_margin=sm_margin, sinks=sinks)
-    return (out, softmax_lse, *rest) if return_softmax_lse else out
+    out, softmax_lse = torch.ops.sgl_kernel.fwd_paged_fp8.default(
+        q, k_cache, v_cache, k_descale, v_descale, page_table, cache_seqlens, cu_seqlens_q, max_seqlen_q, softmax_scale,
+        causal, window_size[0], window_size[1])
+    if not return_softmax_lse:
+        return out
+    empty = softmax_lse.new_empty(0)
+    return out, softmax_lse, empty, empty

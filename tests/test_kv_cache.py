@@ -106,6 +106,12 @@ def test_a_16_bit_paged_cache_is_still_refused():
         sgl_kernel.flash_attn_with_kvcache(q, codes.to(FP8), codes.to(FP8), cache_seqlens=i32(2))
     with pytest.raises(NotImplementedError):
         sgl_kernel.flash_attn_with_kvcache(q, codes, codes, score_mod=lambda s: s)
+    for other in (dict(k=q), dict(v=q), dict(qv=q), dict(rotary_cos=q), dict(rotary_sin=q), dict(cache_batch_idx=i32(2)),
+                  dict(cache_leftpad=i32(2)), dict(cu_seqlens_k_new=i32(3)), dict(rotary_seqlens=i32(2)),
+                  dict(q_descale=q), dict(sinks=q), dict(attention_chunk=8), dict(softcap=1.0)):
+        with pytest.raises(RuntimeError, match="not implemented"):
+            sgl_kernel.flash_attn_with_kvcache(q, codes.to(FP8), codes.to(FP8), cache_seqlens=i32(2),
+                                               page_table=i32(2, 3), **other)
 
 
 def plan_args(**change):
@@ -287,6 +293,9 @@ def test_shapes_under_tracing():
     meta = {k: v.to("meta") if isinstance(v, torch.Tensor) else v for k, v in a.items()}
     out, lse, *_ = torch.ops.sgl_kernel.fwd(**meta)
     assert out.shape == (5, 4, 64) and lse.shape == (4, 5) and lse.dtype == torch.float32
+    same = [meta[n] for n in ("q", "k", "v", "k_descale", "v_descale", "page_table", "seqused_k", "cu_seqlens_q")]
+    out, lse = torch.ops.sgl_kernel.fwd_paged_fp8(*same, 3, None, True, -1, -1)
+    assert out.shape == (5, 4, 64) and lse.shape == (4, 5)
     meta["q"] = torch.empty(2, 3, 4, 64, dtype=BF, device="meta")
     out, lse, *_ = torch.ops.sgl_kernel.fwd(**meta)
     assert out.shape == (2, 3, 4, 64) and lse.shape == (2, 4, 3)
