@@ -402,8 +402,10 @@ def _fwd_paged_fp8(q, k_cache, v_cache, k_descale, v_descale, page_table, cache_
     if not (q.dtype is torch.bfloat16 and k_cache.dtype is FP8 and v_cache.dtype is FP8 and packed and len(cache) == 4
             and v_cache.shape == cache and cache[3] == shape[2] and shape[1] % max(cache[2], 1) == 0 and shape[1] > 0
             and q.stride(2) == 1 and k_cache.stride(3) == 1 and v_cache.stride(3) == 1
-            and (window_left < 0 and window_right < 0 or is_causal and -1 <= window_right <= 0) and k_descale is not None and v_descale is not None and cu_seqlens_q is not None
-            and cache_seqlens is not None and _dense(k_descale, torch.float32, scales, dev) and _dense(v_descale, torch.float32, scales, dev)
+            and (window_left < 0 and window_right < 0 or is_causal and -1 <= window_right <= 0)
+            and k_descale is not None and v_descale is not None and cu_seqlens_q is not None
+            and cache_seqlens is not None
+            and _dense(k_descale, torch.float32, scales, dev) and _dense(v_descale, torch.float32, scales, dev)
             and page_table.dtype is torch.int32 and page_table.stride()[1:] == _ONE
             and _dense(cache_seqlens, torch.int32, page_table.shape[:1], dev)
             and _dense(cu_seqlens_q, torch.int32, (page_table.shape[0] + 1,), dev)
