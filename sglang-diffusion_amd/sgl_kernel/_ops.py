@@ -6,7 +6,8 @@ Python layers call them as `torch.ops.sgl_kernel.<name>.default(...)`.  Here the
 are defined from Python and each one is implemented for the `CUDA` dispatch key (= HIP devices
 under PyTorch-ROCm) by a call through the C ABI of include/mi355_dit.h.  There is no CPU
 implementation: CPU tensors hit the dispatcher's "no kernel for backend CPU" error, and a
-missing shared object raises on first use.  `torch.library.register_fake` shims give the
+missing shared object raises on first use.  (The ops around the paged 8-bit cache are
+implemented in csrc/ops.cpp, which checks the arguments before it refuses CPU tensors.)  `torch.library.register_fake` shims give the
 shape/dtype rules for tracing, as the reference does in
 python/sglang/srt/layers/quantization/fp8_utils.py:69-81 and fp8_kernel.py:2057-2076.
 
@@ -65,6 +66,10 @@ SCHEMAS = {
     "fwd_paged_fp8": "(Tensor q, Tensor k_cache, Tensor v_cache, Tensor? k_descale, Tensor? v_descale, "
                      "Tensor page_table, Tensor? cache_seqlens, Tensor? cu_seqlens_q, int? max_seqlen_q, "
                      "float? softmax_scale, bool causal, int window_left, int window_right) -> (Tensor, Tensor)",
+    "fwd_paged_fp8_out": "(Tensor q, Tensor k_cache, Tensor v_cache, Tensor? k_descale, Tensor? v_descale, "
+                         "Tensor page_table, Tensor? cache_seqlens, Tensor? cu_seqlens_q, int? max_seqlen_q, "
+                         "float? softmax_scale, bool causal, int window_left, int window_right, Tensor! out) "
+                         "-> Tensor",
     "kv_block_plan": "(Tensor context_lens, Tensor new_lens, Tensor! block_table, Tensor free_blocks, "
                      "Tensor free_begin, int block_size, int num_blocks, Tensor! slot_mapping, "
                      "Tensor! positions, Tensor! cu_seqlens_q, Tensor! seq_lens, Tensor! free_end, "
@@ -250,12 +255,15 @@ def _fwd(q, k, v, k_new, v_new, q_v, out, cu_seqlens_q, cu_seqlens_k, cu_seqlens
                      cu_seqlens_k_new=cu_seqlens_k_new, seqused_q=seqused_q, kv_batch_idx=kv_batch_idx,
                      leftpad_k=leftpad_k, rotary_cos=rotary_cos, rotary_sin=rotary_sin,
                      seqlens_rotary=seqlens_rotary, q_descale=q_descale, sinks=sinks)
-        if any(t is not None for t in other.values()):
-            _fail("fwd: arguments not supported with a paged 8-bit cache: "
-                  f"{[n for n, t in other.items() if t is not None]}")
+        bad = [n for n, t in other.items() if t is not None]
+        _require(not bad, f"fwd: arguments not supported with a paged 8-bit cache: {bad}")
         _require(attention_chunk == 0 and softcap == 0.0, "fwd: attention_chunk / softcap are not implemented")
-        out, lse = _fwd_paged_fp8(q, k, v, k_descale, v_descale, page_table, seqused_k, cu_seqlens_q, max_seqlen_q,
-                                  softmax_scale, is_causal, window_left, window_right, out)
+        paged = (q, k, v, k_descale, v_descale, page_table, seqused_k, cu_seqlens_q, max_seqlen_q, softmax_scale,
+                 is_causal, window_left, window_right)
+        if out is None:
+            out, lse = torch.ops.sgl_kernel.fwd_paged_fp8.default(*paged)
+        else:
+            lse = torch.ops.sgl_kernel.fwd_paged_fp8_out.default(*paged, out)
         empty = lse.new_empty(0)
         return out, lse, empty, empty
     unsupported = dict(k_new=k_new, v_new=v_new, q_v=q_v, cu_seqlens_k_new=cu_seqlens_k_new,
@@ -311,198 +319,6 @@ def _fwd(q, k, v, k_new, v_new, q_v, out, cu_seqlens_q, cu_seqlens_k, cu_seqlens
     return out, lse, empty, empty
 
 
-# The checks of the operators around the paged cache run at every step of a serving loop, whose
-# kernels take a few microseconds: messages are only formed when something is wrong.
-def _fail(msg):
-    raise RuntimeError(msg)
-
-
-_ONE = (1,)
-
-
-def _dense(t, dtype, shape, device):
-    return t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == device
-
-
-def _check_cache(what, cache, scale, name, like):
-    if not (cache.dtype == FP8 and cache.dim() == 4 and cache.stride(3) == 1):
-        _fail(f"{what}: {name}_cache must be [blocks, block_size, heads, head_size] float8_e4m3fn with a "
-              "contiguous last dimension")
-    if not (scale is not None and scale.dtype == torch.float32 and scale.is_contiguous()
-            and scale.shape == (cache.shape[0], cache.shape[2])):
-        _fail(f"{what}: the scales of {name}_cache must be contiguous float32 [blocks, heads]")
-    if not cache.get_device() == scale.get_device() == like.get_device():
-        _fail(f"{what}: all tensors must be on {like.device}")
-
-
-def _check_ints(what, like, dtype, **tensors):
-    device = like.get_device()
-    for name, t in tensors.items():
-        if not (t.dtype == dtype and t.dim() == 1 and t.is_contiguous()):
-            _fail(f"{what}: {name} must be a contiguous 1-D {str(dtype)[6:]} tensor")
-        if t.get_device() != device:
-            _fail(f"{what}: all tensors must be on {like.device}")
-
-
-def _check_table(what, table, rows, name, like):
-    if not (table.dtype == torch.int32 and table.dim() == 2 and table.shape[0] == rows
-            and (table.shape[1] <= 1 or table.stride(1) == 1) and table.get_device() == like.get_device()):
-        _fail(f"{what}: {name} must be int32 [sequences, blocks] with contiguous rows, on {like.device}")
-
-
-def _check_heads(what, x, tokens, name, like):
-    if not (x.dtype == torch.bfloat16 and x.dim() == 3 and x.stride(2) == 1 and x.shape[0] == tokens):
-        _fail(f"{what}: {name} must be bfloat16 [tokens, heads, head_size] with a contiguous last dimension")
-    if x is not like and x.get_device() != like.get_device():
-        _fail(f"{what}: all tensors must be on {like.device}")
-
-
-def _check_inv_freq(what, inv_freq, like):
-    if not (inv_freq.dtype in (torch.float64, torch.float32) and inv_freq.dim() == 1 and inv_freq.is_contiguous()
-            and inv_freq.get_device() == like.get_device()):
-        _fail(f"{what}: inv_freq must be a contiguous 1-D float64 or float32 tensor on {like.device}")
-
-
-def _check_fwd_paged(q, k_cache, v_cache, k_descale, v_descale, page_table, cache_seqlens, cu_seqlens_q, is_causal,
-                     window_left, window_right):
-    packed = q.dim() == 3
-    if not (q.dtype == torch.bfloat16 and (packed or q.dim() == 4) and q.stride(-1) == 1):
-        _fail("fwd: q must be bfloat16 [T,H,d] or [B,S,H,d] with a contiguous last dimension")
-    _check_cache("fwd", k_cache, k_descale, "k", q)
-    _check_cache("fwd", v_cache, v_descale, "v", q)
-    if not (v_cache.shape == k_cache.shape and k_cache.shape[3] == q.shape[-1]):
-        _fail("fwd: k_cache and v_cache must have one shape, with the head size of q")
-    if cache_seqlens is None:
-        _fail("fwd: a paged cache needs the sequences' lengths (cache_seqlens)")
-    B = cache_seqlens.numel()
-    _check_table("fwd", page_table, B, "page_table", q)
-    if packed:
-        if cu_seqlens_q is None:
-            _fail("fwd: packed q needs cu_seqlens_q")
-        _check_ints("fwd", q, torch.int32, cache_seqlens=cache_seqlens, cu_seqlens_q=cu_seqlens_q)
-        if cu_seqlens_q.numel() != B + 1:
-            _fail("fwd: cu_seqlens_q and cache_seqlens disagree")
-    else:
-        _check_ints("fwd", q, torch.int32, cache_seqlens=cache_seqlens)
-        if cu_seqlens_q is not None or q.shape[0] != B:
-            _fail("fwd: batched q needs one sequence for each length and no cu_seqlens_q")
-    H, Hk = q.shape[-2], k_cache.shape[2]
-    if not (Hk > 0 and H > 0 and H % Hk == 0):
-        _fail("fwd: the heads of q must be a multiple of the cache's")
-    if not (window_left < 0 and window_right < 0 or is_causal and window_right in (-1, 0)):
-        _fail("fwd: sliding windows need causal attention, and end at the token itself")
-
-
-def _fwd_paged_fp8(q, k_cache, v_cache, k_descale, v_descale, page_table, cache_seqlens, cu_seqlens_q, max_seqlen_q,
-                   softmax_scale, is_causal, window_left, window_right, out=None):
-    shape, cache, dev = q.shape, k_cache.shape, q.get_device()
-    packed = len(shape) == 3
-    # the usual call in few steps; whatever is not that is looked at one by one
-    scales = cache[0::2]
-    if not (q.dtype is torch.bfloat16 and k_cache.dtype is FP8 and v_cache.dtype is FP8 and packed and len(cache) == 4
-            and v_cache.shape == cache and cache[3] == shape[2] and shape[1] % max(cache[2], 1) == 0 and shape[1] > 0
-            and q.stride(2) == 1 and k_cache.stride(3) == 1 and v_cache.stride(3) == 1
-            and (window_left < 0 and window_right < 0 or is_causal and -1 <= window_right <= 0)
-            and k_descale is not None and v_descale is not None and cu_seqlens_q is not None
-            and cache_seqlens is not None
-            and _dense(k_descale, torch.float32, scales, dev) and _dense(v_descale, torch.float32, scales, dev)
-            and page_table.dtype is torch.int32 and page_table.stride()[1:] == _ONE
-            and _dense(cache_seqlens, torch.int32, page_table.shape[:1], dev)
-            and _dense(cu_seqlens_q, torch.int32, (page_table.shape[0] + 1,), dev)
-            and k_cache.get_device() == v_cache.get_device() == page_table.get_device() == dev):
-        _check_fwd_paged(q, k_cache, v_cache, k_descale, v_descale, page_table, cache_seqlens, cu_seqlens_q, is_causal,
-                         window_left, window_right)
-    B = page_table.shape[0]
-    device = q.device
-    if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    elif not (out.shape == shape and out.dtype == q.dtype and out.stride(-1) == 1 and out.device == device):
-        _fail("fwd: out must match q")
-    if packed:
-        lse = torch.empty(shape[1], shape[0], dtype=torch.float32, device=device)
-        if max_seqlen_q is None:
-            max_seqlen_q = shape[0]
-    else:
-        lse = torch.empty(B, shape[2], shape[1], dtype=torch.float32, device=device)
-        max_seqlen_q = shape[1]
-    if softmax_scale is None:
-        softmax_scale = shape[-1] ** -0.5
-    if q.numel() and B:
-        _C.paged_attention_fp8(q, k_cache, v_cache, k_descale, v_descale, page_table, cache_seqlens, cu_seqlens_q,
-                               max_seqlen_q, out, lse, softmax_scale, is_causal, window_left)
-    return out, lse
-
-
-# --------------------------------------------------------------------- paged 8-bit KV cache --
-def _kv_block_plan(context_lens, new_lens, block_table, free_blocks, free_begin, block_size, num_blocks,
-                   slot_mapping, positions, cu_seqlens_q, seq_lens, free_end, status):
-    what = "kv_block_plan"
-    _check_ints(what, slot_mapping, torch.int32, context_lens=context_lens, new_lens=new_lens,
-                free_blocks=free_blocks, free_begin=free_begin, cu_seqlens_q=cu_seqlens_q, seq_lens=seq_lens,
-                free_end=free_end, status=status)
-    _check_ints(what, slot_mapping, torch.int64, slot_mapping=slot_mapping, positions=positions)
-    B = context_lens.numel()
-    if not (new_lens.numel() == B and seq_lens.numel() == B and cu_seqlens_q.numel() == B + 1):
-        _fail("kv_block_plan: new_lens and seq_lens must have one entry for each request, cu_seqlens_q one more")
-    _check_table(what, block_table, B, "block_table", slot_mapping)
-    if positions.numel() != slot_mapping.numel():
-        _fail("kv_block_plan: positions and slot_mapping differ in length")
-    if not (free_begin.numel() == 1 and free_end.numel() == 1 and status.numel() == 3):
-        _fail("kv_block_plan: free_begin and free_end must have 1 entry, status 3")
-    _C.kv_block_plan(context_lens, new_lens, block_table, free_blocks, free_begin, block_size, num_blocks,
-                     slot_mapping, positions, cu_seqlens_q, seq_lens, free_end, status)
-
-
-def _rotary_embedding_scaled(positions, query, key, inv_freq, attn_factor, is_neox, query_out, key_out):
-    what = "rotary_embedding_scaled"
-    _check_ints(what, query, torch.int64, positions=positions)
-    _check_inv_freq(what, inv_freq, query)
-    T = positions.numel()
-    _check_heads(what, query, T, "query", query)
-    _check_heads(what, query_out, T, "query_out", query)
-    if query_out.shape != query.shape:
-        _fail("rotary_embedding_scaled: query_out must have the shape of query")
-    if (key is None) != (key_out is None):
-        _fail("rotary_embedding_scaled: key and key_out come together")
-    if key is not None:
-        _check_heads(what, key, T, "key", query)
-        _check_heads(what, key_out, T, "key_out", query)
-        if not (key_out.shape == key.shape and key.shape[2] == query.shape[2]):
-            _fail("rotary_embedding_scaled: key_out must have the shape of key, and both the head size of query")
-    _C.rope_scaled(positions, query, key, inv_freq, attn_factor, is_neox, query_out, key_out)
-
-
-def _store_kv_cache_fp8(key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping, query, positions, inv_freq,
-                        attn_factor, is_neox, query_out):
-    what = "store_kv_cache_fp8"
-    _check_ints(what, key, torch.int64, slot_mapping=slot_mapping)
-    T = slot_mapping.numel()
-    _check_heads(what, key, T, "key", key)
-    _check_heads(what, value, T, "value", key)
-    _check_cache(what, k_cache, k_scale, "k", key)
-    _check_cache(what, v_cache, v_scale, "v", key)
-    if not (value.shape == key.shape and v_cache.shape == k_cache.shape and k_cache.shape[2:] == key.shape[1:]):
-        _fail("store_kv_cache_fp8: key and value must have one shape, the caches too, with the same heads")
-    if (positions is None) != (inv_freq is None):
-        _fail("store_kv_cache_fp8: positions and inv_freq come together")
-    if (query is None) != (query_out is None):
-        _fail("store_kv_cache_fp8: query and query_out come together")
-    if positions is not None:
-        _check_ints(what, key, torch.int64, positions=positions)
-        _check_inv_freq(what, inv_freq, key)
-        if positions.numel() != T:
-            _fail("store_kv_cache_fp8: positions and slot_mapping differ in length")
-    if query is not None:
-        if positions is None:
-            _fail("store_kv_cache_fp8: a query is given to be rotated, and needs positions")
-        _check_heads(what, query, T, "query", key)
-        _check_heads(what, query_out, T, "query_out", key)
-        if not (query_out.shape == query.shape and query.shape[2] == key.shape[2]):
-            _fail("store_kv_cache_fp8: query_out must have the shape of query, with the head size of key")
-    _C.kv_store_fp8(key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping, query, positions, inv_freq,
-                    attn_factor, is_neox, query_out)
-
-
 def _merge_state_v2(v_a, s_a, v_b, s_b, v_merged, s_merged):
     """sgl-kernel/csrc/attention/merge_attn_states.cu:180-204: contiguous [tokens, heads, D] /
     [tokens, heads] operands on one device."""
@@ -520,9 +336,6 @@ def _merge_state_v2(v_a, s_a, v_b, s_b, v_merged, s_merged):
 
 
 _IMPLS = {
-    "kv_block_plan": _kv_block_plan,
-    "rotary_embedding_scaled": _rotary_embedding_scaled,
-    "store_kv_cache_fp8": _store_kv_cache_fp8,
     "merge_state_v2": _merge_state_v2,
     "fp8_scaled_mm": _fp8_scaled_mm,
     "fp8_blockwise_scaled_mm": _fp8_blockwise_scaled_mm,
@@ -534,10 +347,22 @@ _IMPLS = {
     "rotary_embedding": _rotary_embedding,
     "apply_rope_pos_ids_cos_sin_cache": _apply_rope_pos_ids_cos_sin_cache,
     "fwd": _fwd,
-    "fwd_paged_fp8": _fwd_paged_fp8,
 }
 for _name, _fn in _IMPLS.items():
     _lib.impl(_name, _fn, "CUDA")
+
+# implemented by csrc/ops.cpp; without its library a call says what is missing
+_NATIVE = ("kv_block_plan", "rotary_embedding_scaled", "store_kv_cache_fp8", "fwd_paged_fp8", "fwd_paged_fp8_out")
+try:
+    _C.load_library()
+    torch.ops.load_library(_C.OPS_PATH)
+except (OSError, RuntimeError) as _error:
+    def _missing(*args, _why=str(_error)):
+        raise RuntimeError(f"{_C.OPS_PATH}: {_why}; build it with `make -C sglang-diffusion_amd/csrc` "
+                           "(or __graft_entry__.build()); there is no other implementation")
+
+    for _name in _NATIVE:
+        _lib.impl(_name, _missing, "CUDA")
 
 
 # --------------------------------------------------------------- fake (meta) implementations --
@@ -564,6 +389,11 @@ for _name in ("sgl_per_token_quant_fp8", "sgl_per_token_group_quant_8bit", "sgl_
 @torch.library.register_fake("sgl_kernel::fwd_paged_fp8")
 def _fake_fwd_paged_fp8(q, *rest, **kw):
     return _fake_fwd(q, None, None, None, None, None, None, None, None)[:2]
+
+
+@torch.library.register_fake("sgl_kernel::fwd_paged_fp8_out")
+def _fake_fwd_paged_fp8_out(q, *rest, **kw):
+    return _fake_fwd(q, None, None, None, None, None, None, None, None)[1]
 
 
 @torch.library.register_fake("sgl_kernel::fwd")

@@ -18,6 +18,8 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # MI355_DIT_LIB points at another build of the library (A/B timing of kernel variants)
 LIB_PATH = os.environ.get("MI355_DIT_LIB") or os.path.join(_HERE, "libmi355dit.so")
+# torch ops in C++ on top of it (csrc/ops.cpp), loaded by sgl_kernel
+OPS_PATH = os.path.join(_HERE, "libmi355ops.so")
 
 _i64 = ctypes.c_int64
 _f32 = ctypes.c_float
@@ -195,7 +197,7 @@ def load_library() -> ctypes.CDLL:
             f"{LIB_PATH} not found: build it with `make -C sglang-diffusion_amd/csrc` "
             "(or __graft_entry__.build()); there is no non-HIP fallback"
         )
-    lib = ctypes.CDLL(LIB_PATH)
+    lib = ctypes.CDLL(LIB_PATH, mode=ctypes.RTLD_GLOBAL)  # csrc/ops.cpp finds the entry points there
     # MI355_DIT_ABI_ANY=1 (A/B timing of an OLDER build through entry points it already had):
     # symbols the build lacks are skipped and the revision check is waived
     lenient = os.environ.get("MI355_DIT_ABI_ANY") == "1"
@@ -784,89 +786,3 @@ def guidance_rescale_static(noise, cond, rescale: float) -> None:
             ),
             "guidance_rescale_static",
         )
-
-
-# ------------------------------------------------------------------- paged 8-bit KV cache --
-def kv_block_plan(context_lens, new_lens, block_table, free_blocks, free_begin, block_size, num_blocks,
-                  slot_mapping, positions, cu_seqlens_q, seq_lens, free_end, status) -> None:
-    B, width = block_table.shape
-    _check(
-        load_library().mi355_kv_block_plan(
-            context_lens.data_ptr(), new_lens.data_ptr(), B, block_table.data_ptr(), block_table.stride(0), width,
-            free_blocks.data_ptr(), free_blocks.numel(), free_begin.data_ptr(), block_size, num_blocks,
-            slot_mapping.data_ptr(), positions.data_ptr(), slot_mapping.numel(), cu_seqlens_q.data_ptr(),
-            seq_lens.data_ptr(), free_end.data_ptr(), status.data_ptr(), _stream(slot_mapping),
-        ),
-        "kv_block_plan",
-    )
-
-
-def rope_scaled(positions, q, k, inv_freq, attn_factor, is_neox, q_out, k_out) -> None:
-    """q [T, Hq, D], k [T, Hk, D] or None (last dim contiguous), written to q_out / k_out."""
-    T, H, D = q.shape
-    qt, qh, _ = q.stride()
-    qot, qoh, _ = q_out.stride()
-    if k is None:
-        Hk = kt = kh = kot = koh = 0
-        kp = kop = None
-    else:
-        Hk = k.shape[1]
-        kt, kh, _ = k.stride()
-        kot, koh, _ = k_out.stride()
-        kp, kop = k.data_ptr(), k_out.data_ptr()
-    _check(
-        load_library().mi355_rope_scaled(
-            positions.data_ptr(), q.data_ptr(), q_out.data_ptr(), kp, kop, T, H, Hk, D, 2 * inv_freq.numel(), qt, qh,
-            qot, qoh, kt, kh, kot, koh, inv_freq.data_ptr(), inv_freq.dtype == torch.float64, attn_factor,
-            bool(is_neox), _stream(q),
-        ),
-        "rope_scaled",
-    )
-
-
-def kv_store_fp8(k, v, k_cache, v_cache, k_scale, v_scale, slot_mapping, q=None, positions=None, inv_freq=None,
-                 attn_factor=1.0, is_neox=True, q_out=None) -> None:
-    """k, v [T, Hk, D] bf16 into caches [blocks, block_size, Hk, D] (e4m3) with scales [blocks, Hk];
-    positions given: keys, and q [T, Hq, D] into q_out, are rotated."""
-    T, Hk, D = k.shape
-    blocks, block_size = k_cache.shape[:2]
-    a = KvStoreArgs(
-        k.data_ptr(), v.data_ptr(), *k.stride()[:2], *v.stride()[:2], k_cache.data_ptr(), v_cache.data_ptr(),
-        *k_cache.stride()[:3], *v_cache.stride()[:3], k_scale.data_ptr(), v_scale.data_ptr(),
-        slot_mapping.data_ptr(), T, Hk, D, block_size, blocks)
-    if positions is not None:
-        a.positions, a.inv_freq = positions.data_ptr(), inv_freq.data_ptr()
-        a.rot_dim, a.inv_freq_is_f64 = 2 * inv_freq.numel(), inv_freq.dtype == torch.float64
-        a.is_neox, a.attn_factor = bool(is_neox), attn_factor
-    if q is not None:
-        a.Hq, a.q, a.q_out = q.shape[1], q.data_ptr(), q_out.data_ptr()
-        a.q_st, a.q_sh, _ = q.stride()
-        a.qo_st, a.qo_sh, _ = q_out.stride()
-    _check(load_library().mi355_kv_store_fp8(ctypes.byref(a), _stream(k)), "kv_store_fp8")
-
-
-def paged_attention_fp8(q, k_cache, v_cache, k_scale, v_scale, page_table, cache_seqlens, cu_seqlens_q,
-                        max_seqlen_q, out, lse, softmax_scale, causal, window_left) -> None:
-    """q, out [T, H, D] with cu_seqlens_q, or [B, Sq, H, D] without; lse [H, T] or [B, H, Sq]
-    (dense fp32) or None.  The workspace comes from the caching allocator, so it belongs to the
-    current stream, or to the graph that is being captured."""
-    packed = q.dim() == 3
-    Sq, H, D = q.shape[-3:]
-    blocks, block_size, Hk, _ = k_cache.shape
-    B, width = page_table.shape
-    s, os_ = q.stride(), out.stride()
-    a = PagedAttnArgs(
-        q.data_ptr(), out.data_ptr(), _p(lse), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
-        v_scale.data_ptr(), _p(cu_seqlens_q), cache_seqlens.data_ptr(), page_table.data_ptr(), B, Sq, H, Hk, D,
-        max_seqlen_q, 0 if packed else s[0], s[-3], s[-2], 0 if packed else os_[0], os_[-3], os_[-2],
-        0 if packed else H * Sq, Sq, *k_cache.stride()[:3], *v_cache.stride()[:3], page_table.stride(0), width, blocks,
-        block_size, softmax_scale, causal, window_left)
-    lib = load_library()
-    stream = _stream(q)
-    need = lib.mi355_paged_attn_workspace_bytes(ctypes.byref(a))
-    if need < 0:
-        _check(need, "paged_attn_fp8")
-    if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), need
-    _check(lib.mi355_paged_attn_fp8(ctypes.byref(a), stream), "paged_attn_fp8")

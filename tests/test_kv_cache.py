@@ -24,11 +24,10 @@ def i64(*shape):
 
 
 def call(name, **kw):
-    """The implementation behind the registry, on CPU tensors: its checks run, the library then
-    refuses the device."""
+    """The op on CPU tensors: its checks run, then the device is refused."""
     from sgl_kernel import _ops
 
-    return _ops._IMPLS[name](**kw)
+    return _ops._IMPLS[name](**kw) if name in _ops._IMPLS else getattr(torch.ops.sgl_kernel, name).default(**kw)
 
 
 def fwd_args(**change):
@@ -55,7 +54,7 @@ def test_attend_reaches_the_library_and_no_cpu_form():
     import sgl_kernel
 
     a = fwd_args()
-    with pytest.raises(NotImplementedError):
+    with pytest.raises(RuntimeError, match="HIP device"):
         sgl_kernel.flash_attn_with_kvcache(a["q"], a["k"], a["v"], cache_seqlens=a["seqused_k"], page_table=a["page_table"],
                                            cu_seqlens_q=a["cu_seqlens_q"], max_seqlen_q=3, k_descale=a["k_descale"],
                                            v_descale=a["v_descale"], causal=True)
@@ -89,6 +88,7 @@ def test_attend_reaches_the_library_and_no_cpu_form():
     (dict(k_new=torch.zeros(1)), "k_new"),
     (dict(cu_seqlens_k=i32(3)), "cu_seqlens_k"),
     (dict(out=torch.zeros(5, 4, 64)), "out must match"),
+    (dict(out=torch.zeros(5, 4, 64, dtype=BF)), "HIP device"),
 ])
 def test_attend_refuses(change, match):
     refused("fwd", fwd_args(**change), match)
@@ -296,6 +296,7 @@ def test_shapes_under_tracing():
     same = [meta[n] for n in ("q", "k", "v", "k_descale", "v_descale", "page_table", "seqused_k", "cu_seqlens_q")]
     out, lse = torch.ops.sgl_kernel.fwd_paged_fp8(*same, 3, None, True, -1, -1)
     assert out.shape == (5, 4, 64) and lse.shape == (4, 5)
+    assert torch.ops.sgl_kernel.fwd_paged_fp8_out(*same, 3, None, True, -1, -1, torch.empty_like(same[0])).shape == (4, 5)
     meta["q"] = torch.empty(2, 3, 4, 64, dtype=BF, device="meta")
     out, lse, *_ = torch.ops.sgl_kernel.fwd(**meta)
     assert out.shape == (2, 3, 4, 64) and lse.shape == (2, 4, 3)
