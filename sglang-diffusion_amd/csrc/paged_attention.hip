@@ -16,6 +16,7 @@
 // its keys.  Lengths are known on the device only, so each workgroup adds up the work of all
 // sequences, from that takes the length of a chunk that makes about as many items as the chip
 // holds workgroups, and finds its own item.  Chunks of one row tile are joined by a second kernel.
+#include <algorithm>
 #include <atomic>
 
 #include "common.h"
@@ -51,7 +52,7 @@ struct PagedParams {
   // items
   int items, chunk_min, split, hw, turns;  // hw: heads of a workgroup, turns: waves of each
   int by_length;     // items longest first
-  float inv_target;
+  float slots;       // workgroups of one round, for each group of heads
   float* part;       // [Hk * items][M][D + 2]
   int32_t* info;     // [B][2]: first item of the sequence, chunks of each of its row tiles
 };
@@ -78,6 +79,9 @@ __device__ __forceinline__ void seq_tiles(const PagedParams& p, const Seq& s, in
   hi = (s.len + KT - 1) / KT;
   if (hi < lo) hi = lo;
 }
+
+// the value of a wave's last lane: of a scan the sum
+__device__ __forceinline__ int wave_last(int v) { return __builtin_amdgcn_readlane(v, 63); }
 
 struct Item {
   Seq s;
@@ -147,37 +151,70 @@ __device__ bool find_item(const PagedParams& p, int item, int group, Item* out) 
     const int lane = threadIdx.x;
     const int per = (p.B + 63) >> 6;
     const int b0 = lane * per, b1 = min(p.B, b0 + per);
-    int length = 1 << 30;
+    int length = 1 << 30;  // tiles of the longest chunk
     Seq s{0, 0, 0};
+    if (b0 < b1) s = seq_of(p, b0);
     auto tiles_of = [&](const Seq& q) { return (q.n * p.G + M - 1) / M; };
-    if (p.split) {
-      // tiles of keys of all items, as a float: only the length of a chunk hangs on it, and every
-      // workgroup adds the same numbers in the same order
-      float work = 0.f;
-      for (int b = b0; b < b1; ++b) {
-        s = seq_of(p, b);
-        int lo, hi;
-        seq_tiles(p, s, lo, hi);
-        work += (float)tiles_of(s) * (float)(hi - lo);
-      }
-      work = group_sum<64>(work);
-      length = (int)fminf(1e9f, fmaxf((float)p.chunk_min, ceilf(work * p.inv_target)));
-      length = (length + p.turns - 1) / p.turns * p.turns;  // whole turns of the waves of a head
-    } else if (b0 < b1) {
-      s = seq_of(p, b0);
-    }
-    auto chunks_of = [&](const Seq& q) {
+    auto keys_of = [&](const Seq& q) {
       int lo, hi;
       seq_tiles(p, q, lo, hi);
-      return max(1, (hi - lo + length - 1) / length);
+      return hi - lo;
     };
-    int mine = 0;
+    // (every workgroup adds the same numbers in the same order)
+    auto whole = [&](float tiles) {  // chunks are at least chunk_min long, and whole turns of a head's waves
+      const int t = (int)fminf(1e9f, fmaxf((float)p.chunk_min, ceilf(tiles)));
+      return (t + p.turns - 1) & -p.turns;
+    };
+    if (p.split && per == 1) {
+      const int tiles = b0 < b1 ? tiles_of(s) : 0, keys = b0 < b1 ? keys_of(s) : 0;
+      const int64_t mine = (int64_t)tiles * keys;  // below 2^49: summed in halves, lane to lane
+      const float work = 0x1p24f * (float)wave_last(wave_scan((int)(mine >> 24))) +
+                         (float)wave_last(wave_scan((int)(mine & 0xffffff)));
+      const float rows = (float)wave_last(wave_scan(tiles));
+      // one round of workgroups, or two where tiles of rows alone take more than 0.6 of one
+      const float slots = rows > 0.6f * p.slots ? 2.f * p.slots : p.slots;
+      auto fits = [&](unsigned l) { return (float)wave_last(wave_scan(tiles * max(1u, (keys + l - 1u) / l))) <= slots; };
+      // between as many chunks as there are slots and as many as fit whatever the last ones' lengths
+      float less = work / slots, most = work / fmaxf(slots - rows, 0.125f * slots);
+      length = whole(less);
+      if (!fits(length)) {
+        for (int i = 0; i < 4; ++i) {
+          const float mid = 0.5f * (less + most);
+          if (fits(whole(mid))) most = mid;
+          else less = mid;
+        }
+        length = whole(most);
+      }
+    } else if (p.split) {
+      // (more sequences than lanes: half the tiles of rows are taken off instead, about what the
+      // last chunks are short of)
+      float work = 0.f, rows = 0.f;
+      for (int b = b0; b < b1; ++b) {
+        s = seq_of(p, b);
+        rows += (float)tiles_of(s);
+        work += (float)tiles_of(s) * (float)keys_of(s);
+      }
+      rows = group_sum<64>(rows);
+      length = whole(group_sum<64>(work) / (p.slots - 0.5f * fminf(rows, p.slots)));
+    }
+    // chunks of a sequence, of one length
+    auto chunks_of = [&](const Seq& q, int& l) {
+      const unsigned keys = keys_of(q), n = max(1u, (keys + length - 1) / (unsigned)length);
+      l = length;
+      if (n == 1) return 1;
+      l = ((keys + n - 1) / n + p.turns - 1) & -p.turns;
+      return (int)((keys + l - 1) / (unsigned)l);
+    };
+    int mine = 0, chunks = 1, own = length;
     if (per == 1) {
-      if (b0 < b1) mine = tiles_of(s) * chunks_of(s);
+      if (b0 < b1) {
+        chunks = chunks_of(s, own);
+        mine = tiles_of(s) * chunks;
+      }
     } else {
       for (int b = b0; b < b1; ++b) {
         s = seq_of(p, b);
-        mine += tiles_of(s) * chunks_of(s);
+        mine += tiles_of(s) * chunks_of(s, own);
       }
     }
     const int upto = wave_scan(mine);
@@ -185,11 +222,14 @@ __device__ bool find_item(const PagedParams& p, int item, int group, Item* out) 
     int at = upto - mine;
     if (item >= at && item < upto) {
       for (int b = b0; b < b1; ++b) {
-        if (per > 1) s = seq_of(p, b);
-        const int tiles = tiles_of(s), chunks = chunks_of(s), k = item - at;
+        if (per > 1) {
+          s = seq_of(p, b);
+          chunks = chunks_of(s, own);
+        }
+        const int tiles = tiles_of(s), k = item - at;
         if (k >= 0 && k < (int64_t)tiles * chunks) {
           // causal rows further down see more: they begin first
-          found = Item{s, b, tiles - 1 - k / chunks, k % chunks, chunks, length};
+          found = Item{s, b, tiles - 1 - k / chunks, k % chunks, chunks, own};
           if (p.split && k == 0 && group == 0) {  // for the join
             p.info[2 * b] = item;
             p.info[2 * b + 1] = chunks;
@@ -1023,7 +1063,7 @@ int cu_count() {
 
 struct Plan {
   int M, few, hw;      // rows of a tile; which kernel; heads of a workgroup
-  int64_t items, target;
+  int64_t items, slots;
   int chunk_min, split;
   int64_t part_bytes, info_bytes;
 };
@@ -1040,19 +1080,20 @@ Plan plan_of(const mi355_paged_attn_args* a) {
   // as many heads to a workgroup as share its four waves: what they read lies side by side
   w.hw = !w.few ? 1 : a->Hk % 4 == 0 ? 4 : a->Hk % 2 == 0 ? 2 : 1;
   const int64_t tiles = all_rows / w.M + a->B;  // row tiles: at most one not full for each sequence
-  // Items to aim for: as many as the chip holds workgroups, two a CU (many rows with heads of 64:
-  // three; 509 tokens behind 30k keys 105 us, with two 115 us).  With few rows the last chunk of
-  // each row tile is about half a chunk, and what is over one round of workgroups waits for it:
-  // half the row tiles are taken off (32 x 1 token, ragged: 44 us, without 53 us, with two rounds
-  // of half the length 50 us).
+  // Workgroups of one round: two a CU (many rows with heads of 64: three; 509 tokens behind 30k keys
+  // 105 us, with two 115 us).  What is over one round waits for it: with few rows two rounds of half
+  // the length take 50 us where one takes 44 (32 x 1 token, ragged).
   const int64_t want = (w.few ? 2 : a->D == 64 ? 3 : 2) * (int64_t)cu_count();
   const int64_t groups = a->Hk / w.hw;
-  w.target = (want + groups - 1) / groups;
-  if (w.few) w.target -= tiles < w.target ? tiles / 2 : w.target / 2;
+  w.slots = (want + groups - 1) / groups;
   w.chunk_min = w.few ? (w.hw == 4 ? 1 : 4) : 4;
   const int64_t cap = a->table_width * a->block_size;
   w.split = cap > (int64_t)w.chunk_min * KT && (all_rows / w.M) * groups < 2 * want;
-  w.items = tiles + (w.split ? w.target : 0);
+  // (find_item makes no more: with one lane for a sequence the chunks fit one or two rounds, else
+  // there is at most one more than the work takes for each tile of rows)
+  const int64_t chunks = a->B > 64 ? tiles + w.slots
+                         : 5 * tiles <= 3 * w.slots ? w.slots : std::max(2 * w.slots, tiles + w.slots / 4);
+  w.items = w.split ? chunks : tiles;
   w.part_bytes = w.split ? a->Hk * w.items * w.M * (a->D + 2) * (int64_t)sizeof(float) : 0;
   w.info_bytes = w.split ? a->B * 2 * (int64_t)sizeof(int32_t) : 0;
   return w;
@@ -1176,7 +1217,7 @@ extern "C" int mi355_paged_attn_fp8(const mi355_paged_attn_args* a, void* stream
   p.window = a->window_left < 0 ? -1 : (int)(a->window_left < (1 << 30) ? a->window_left : (1 << 30));
   p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
   p.items = (int)w.items;
-  p.inv_target = 1.f / (float)w.target;
+  p.slots = (float)w.slots;
   p.chunk_min = w.chunk_min;
   p.split = w.split;
   p.by_length = !w.few && !w.split && a->causal && a->B > 1 && a->B <= SORTED_SEQS;
