@@ -51,6 +51,7 @@ struct PagedParams {
   float scale_log2;
   // items
   int items, chunk_min, split, hw, turns;  // hw: heads of a workgroup, turns: waves of each
+  float join_cost;   // of an item, in tiles
   int by_length;     // items longest first
   float slots;       // workgroups of one round, for each group of heads
   float* part;       // [Hk * items][M][D + 2]
@@ -173,18 +174,23 @@ __device__ bool find_item(const PagedParams& p, int item, int group, Item* out) 
       const float rows = (float)wave_last(wave_scan(tiles));
       // one round of workgroups, or two where tiles of rows alone take more than 0.6 of one
       const float slots = rows > 0.6f * p.slots ? 2.f * p.slots : p.slots;
-      auto fits = [&](unsigned l) { return (float)wave_last(wave_scan(tiles * max(1u, (keys + l - 1u) / l))) <= slots; };
+      auto items = [&](unsigned l) { return (float)wave_last(wave_scan(tiles * max(1u, (keys + l - 1u) / l))); };
       // between as many chunks as there are slots and as many as fit whatever the last ones' lengths
       float less = work / slots, most = work / fmaxf(slots - rows, 0.125f * slots);
       length = whole(less);
-      if (!fits(length)) {
+      if (items(length) > slots) {
         for (int i = 0; i < 4; ++i) {
           const float mid = 0.5f * (less + most);
-          if (fits(whole(mid))) most = mid;
-          else less = mid;
+          if (items(whole(mid)) > slots) less = mid;
+          else most = mid;
         }
         length = whole(most);
       }
+      // What the parts cost is weighed: where the longest keys take no more in one piece than a chunk
+      // and the writing and joining of all of them, they stay in one (one prompt of 1000 tokens, 32
+      // heads over 8: 38 us, in two pieces 54)
+      const float split = slots / p.slots * (float)length + p.join_cost * items(length);
+      if (__builtin_amdgcn_ballot_w64((float)keys * fmaxf(1.f, rows / p.slots) > split) == 0) length = 1 << 30;
     } else if (p.split) {
       // (more sequences than lanes: half the tiles of rows are taken off instead, about what the
       // last chunks are short of)
@@ -961,42 +967,54 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedP
 }
 
 // ------------------------------------------------------------------------------------- joint --
-// The chunks of a row of q: WAVES waves for each.  Lane c weighs chunk c; the sums run over a few
-// chunks at a time, so that their loads are in flight together.
-template <int D, int WAVES>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p, int M, int64_t rows) {
-  __shared__ f32x4 others[3][D / 4];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t row_of_q = WAVES == 4 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
-  if (row_of_q >= rows) return;
-  const int H = p.Hk * p.G;
-  const int64_t t = row_of_q / H;
-  const int head = (int)(row_of_q - t * H);
-  int b, tok;
+// The sequence and token of row t of q, for a whole wave; false where there is nothing to join: a
+// row behind the last sequence, or one whose keys were not split.
+struct JoinRow {
+  int b, tok, base, chunks, tiles;
+};
+__device__ __forceinline__ bool join_row(const PagedParams& p, int M, int64_t t, JoinRow* j) {
+  const int lane = threadIdx.x & 63;
   if (p.cu) {  // the sequence whose rows t is among: those that end at or before t come before it
-    b = 0;
+    j->b = 0;
     for (int i0 = 0; i0 < p.B; i0 += 64) {
       const int i = i0 + lane;
       const unsigned long long before = __builtin_amdgcn_ballot_w64(i < p.B && p.cu[min(i, p.B - 1) + 1] <= (int)t);
-      b += __popcll(before);
+      j->b += __popcll(before);
       if (before != ~0ull) break;
     }
-    if (b >= p.B) return;  // a row behind the last sequence
-    tok = (int)t - seq_of(p, b).first;
+    if (j->b >= p.B) return false;  // a row behind the last sequence
+    j->tok = (int)t - seq_of(p, j->b).first;
   } else {
-    b = (int)(t / p.Sq);
-    tok = (int)(t - (int64_t)b * p.Sq);
+    j->b = (int)(t / p.Sq);
+    j->tok = (int)(t - (int64_t)j->b * p.Sq);
   }
-  const int hk = head / p.G, row = tok * p.G + head - hk * p.G;
-  const int n = seq_of(p, b).n;
-  if (tok < 0 || tok >= n) return;
-  const int base = p.info[2 * b], chunks = p.info[2 * b + 1];
-  const int tiles = (n * p.G + M - 1) / M;
+  const int n = seq_of(p, j->b).n;
+  j->base = p.info[2 * j->b];
+  j->chunks = p.info[2 * j->b + 1];
+  j->tiles = (n * p.G + M - 1) / M;
   // one chunk: written by the kernel itself.  (Running sums that are none would leave this unset.)
-  if (chunks <= 1 || base < 0 || base + (int64_t)tiles * chunks > p.items) return;
+  return j->tok >= 0 && j->tok < n && j->chunks > 1 && j->base >= 0 &&
+         j->base + (int64_t)j->tiles * j->chunks <= p.items;
+}
+__device__ __forceinline__ const float* parts_of(const PagedParams& p, int M, int64_t step, const JoinRow& j, int hk, int row) {
+  return p.part + ((int64_t)hk * p.items + j.base + (int64_t)(j.tiles - 1 - row / M) * j.chunks) * step;
+}
+
+// Few rows of q: four waves for each.  Lane c weighs chunk c; the sums run over a few chunks at a
+// time, so that their loads are in flight together.
+template <int D>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p, int M) {
+  __shared__ f32x4 others[3][D / 4];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int H = p.Hk * p.G;
+  const int64_t t = blockIdx.x / H;
+  const int head = (int)(blockIdx.x - t * H);
+  JoinRow j;
+  if (!join_row(p, M, t, &j)) return;
+  const int hk = head / p.G, row = j.tok * p.G + head - hk * p.G;
+  const int chunks = j.chunks, in_tile = row % M;
   const int64_t step = (int64_t)M * (D + 2);
-  const int in_tile = row % M;
-  const float* part = p.part + ((int64_t)hk * p.items + base + (int64_t)(tiles - 1 - row / M) * chunks) * step;
+  const float* part = parts_of(p, M, step, j, hk, row);
   float top = M_EMPTY;
   for (int c = lane; c < chunks; c += 64) top = fmaxf(top, part[c * step + M * D + 2 * in_tile]);
   top = group_max<64>(top);
@@ -1011,7 +1029,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p, int M, i
     const float w = c0 + lane < chunks ? __builtin_amdgcn_exp2f(ml[0] - top) : 0.f;
     l = fmaf(w != 0.f ? ml[1] : 0.f, w, l);
     const int here = min(64, chunks - c0);
-    for (int k = WAVES == 4 ? wave * 4 * SIDE : 0; k < here; k += WAVES * 4 * SIDE) {
+    for (int k = wave * 4 * SIDE; k < here; k += 16 * SIDE) {
       f32x4 v[4];
       float wv[4];
 #pragma unroll
@@ -1024,27 +1042,88 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p, int M, i
 #pragma unroll
       for (int u = 0; u < 4; ++u)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[j] = wv[u] == 0.f ? acc[j] : fmaf(v[u][j], wv[u], acc[j]);
+        for (int i = 0; i < 4; ++i) acc[i] = wv[u] == 0.f ? acc[i] : fmaf(v[u][i], wv[u], acc[i]);
     }
   }
   l = group_sum<64>(l);
 #pragma unroll
   for (int w = LANES; w < 64; w <<= 1)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[j] += __shfl_xor(acc[j], w, 64);
-  if constexpr (WAVES == 4) {
-    if (wave && mine == 0) others[wave - 1][ch] = acc;
-    __syncthreads();
-    if (wave) return;
+    for (int i = 0; i < 4; ++i) acc[i] += __shfl_xor(acc[i], w, 64);
+  if (wave && mine == 0) others[wave - 1][ch] = acc;
+  __syncthreads();
+  if (wave) return;
 #pragma unroll
-    for (int w = 0; w < 3; ++w) acc = acc + others[w][ch];
-  }
+  for (int w = 0; w < 3; ++w) acc = acc + others[w][ch];
   const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int64_t q_row = p.cu ? t : j.tok;
   if (mine == 0)
-    *reinterpret_cast<u32x2*>(p.o + b * p.o_sb + (p.cu ? t : tok) * p.o_ss + head * p.o_sh + 4 * ch) =
+    *reinterpret_cast<u32x2*>(p.o + j.b * p.o_sb + q_row * p.o_ss + head * p.o_sh + 4 * ch) =
         u32x2{pack_bf2(acc[0] * inv, acc[1] * inv), pack_bf2(acc[2] * inv, acc[3] * inv)};
   if (p.lse && lane == 0)
-    p.lse[b * p.lse_sb + head * p.lse_sh + (p.cu ? t : tok)] =
+    p.lse[j.b * p.lse_sb + head * p.lse_sh + q_row] =
+        l == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+}
+
+// Many rows: a wave for four heads of a token, sixteen lanes for each, all chunks in one pass with
+// a running maximum, four of them in flight.
+template <int D>
+__global__ __launch_bounds__(256) void paged_join_rows_kernel(PagedParams p, int M, int64_t waves, int head_groups) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t id = (int64_t)blockIdx.x * 4 + wave;
+  if (id >= waves) return;
+  const int64_t t = id / head_groups;
+  JoinRow j;
+  if (!join_row(p, M, t, &j)) return;
+  const int H = p.Hk * p.G, ch = lane & 15;
+  const int mine = (int)(id - t * head_groups) * 4 + (lane >> 4), head = min(mine, H - 1);
+  const int hk = head / p.G, row = j.tok * p.G + head - hk * p.G;
+  const int chunks = j.chunks, in_tile = row % M;
+  const int64_t step = (int64_t)M * (D + 2);
+  const float* part = parts_of(p, M, step, j, hk, row);
+  constexpr int NV = D / 64;  // lanes hold channels 4 (ch + 16 n) and on
+  f32x4 acc[NV];
+#pragma unroll
+  for (int n = 0; n < NV; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float top = M_EMPTY, l = 0.f;
+  for (int c0 = 0; c0 < chunks; c0 += 4) {
+    float m[4], lc[4];
+    f32x4 v[4][NV];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float* at = part + min(c0 + u, chunks - 1) * step;
+      m[u] = at[M * D + 2 * in_tile];
+      lc[u] = at[M * D + 2 * in_tile + 1];
+#pragma unroll
+      for (int n = 0; n < NV; ++n) v[u][n] = *reinterpret_cast<const f32x4*>(at + in_tile * D + 4 * (ch + 16 * n));
+    }
+    const float was = top;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) top = fmaxf(top, m[u]);
+    const float shrink = __builtin_amdgcn_exp2f(was - top);
+    l *= shrink;
+#pragma unroll
+    for (int n = 0; n < NV; ++n) acc[n] *= shrink;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float w = c0 + u < chunks ? __builtin_amdgcn_exp2f(m[u] - top) : 0.f;
+      l = w == 0.f ? l : fmaf(lc[u], w, l);
+#pragma unroll
+      for (int n = 0; n < NV; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[n][i] = w == 0.f ? acc[n][i] : fmaf(v[u][n][i], w, acc[n][i]);
+    }
+  }
+  if (mine >= H) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int64_t q_row = p.cu ? t : j.tok;
+  unsigned short* out = p.o + j.b * p.o_sb + q_row * p.o_ss + head * p.o_sh;
+#pragma unroll
+  for (int n = 0; n < NV; ++n)
+    *reinterpret_cast<u32x2*>(out + 4 * (ch + 16 * n)) =
+        u32x2{pack_bf2(acc[n][0] * inv, acc[n][1] * inv), pack_bf2(acc[n][2] * inv, acc[n][3] * inv)};
+  if (p.lse && ch == 0)
+    p.lse[j.b * p.lse_sb + head * p.lse_sh + q_row] =
         l == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
 }
 
@@ -1088,7 +1167,9 @@ Plan plan_of(const mi355_paged_attn_args* a) {
   w.slots = (want + groups - 1) / groups;
   w.chunk_min = w.few ? (w.hw == 4 ? 1 : 4) : 4;
   const int64_t cap = a->table_width * a->block_size;
-  w.split = cap > (int64_t)w.chunk_min * KT && (all_rows / w.M) * groups < 2 * want;
+  // (below that a piece costs less than the join's launch: 1 token over 100 keys 9.5 us, split 13; one
+  // prompt of 500 tokens 19 us, split 30)
+  w.split = cap > (w.few ? 4 * (4 / w.hw) : 8) * KT && (all_rows / w.M) * groups < 2 * want;
   // (find_item makes no more: with one lane for a sequence the chunks fit one or two rounds, else
   // there is at most one more than the work takes for each tile of rows)
   const int64_t chunks = a->B > 64 ? tiles + w.slots
@@ -1142,12 +1223,13 @@ int launch(const PagedParams& p, const Plan& w, hipStream_t st) {
   }
   MI355_CHECK_LAUNCH("paged_attn_fp8");
   if (w.split) {
-    const int64_t rows = (int64_t)p.Sq * (p.cu ? 1 : p.B) * p.Hk * p.G;
+    const int64_t tokens = (int64_t)p.Sq * (p.cu ? 1 : p.B), heads = p.Hk * p.G, head_groups = (heads + 3) / 4;
     // four waves for a row while there are few rows (4 x 1 token over 128k keys: 6.3 us, with one 9)
-    if (rows <= 2048)
-      hipLaunchKernelGGL((paged_join_kernel<D, 4>), dim3((unsigned)rows), dim3(256), 0, st, p, w.M, rows);
+    if (tokens * heads <= 2048)
+      hipLaunchKernelGGL(paged_join_kernel<D>, dim3((unsigned)(tokens * heads)), dim3(256), 0, st, p, w.M);
     else
-      hipLaunchKernelGGL((paged_join_kernel<D, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, p, w.M, rows);
+      hipLaunchKernelGGL(paged_join_rows_kernel<D>, dim3((unsigned)((tokens * head_groups + 3) / 4)), dim3(256), 0, st, p,
+                         w.M, tokens * head_groups, (int)head_groups);
     MI355_CHECK_LAUNCH("paged_attn_fp8 (join)");
   }
   return MI355_OK;
@@ -1218,6 +1300,8 @@ extern "C" int mi355_paged_attn_fp8(const mi355_paged_attn_args* a, void* stream
   p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
   p.items = (int)w.items;
   p.slots = (float)w.slots;
+  // written and read, against what the chip moves while a workgroup does a tile of keys (2 us)
+  p.join_cost = (float)(a->Hk * w.M * (a->D + 2) * 8) / 7e6f;
   p.chunk_min = w.chunk_min;
   p.split = w.split;
   p.by_length = !w.few && !w.split && a->causal && a->B > 1 && a->B <= SORTED_SEQS;
