@@ -14,8 +14,9 @@
 //
 // Work is cut into items: a tile of rows of one sequence and key/value head against a chunk of
 // its keys.  Lengths are known on the device only, so each workgroup adds up the work of all
-// sequences, from that takes the length of a chunk that makes about as many items as the chip
-// holds workgroups, and finds its own item.  Chunks of one row tile are joined by a second kernel.
+// sequences, from that takes the length of a chunk with which the items fill one round of
+// workgroups, and finds its own item.  Chunks of one row tile are joined by a second kernel; keys
+// that are not worth it stay in one piece.
 #include <algorithm>
 #include <atomic>
 
@@ -668,10 +669,16 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void paged_few_rows_kernel(Pa
 
 // --------------------------------------------------------------------------------- many rows --
 // 32 rows for each of four waves, which share the tiles of keys in LDS, widened to 16 bits once
-// for all of them while they are stored there: loaded to registers a tile ahead, converted, two
-// stages, one barrier for each tile.  Products and layouts are those of the dense kernel
-// (attention.hip): S^T = K . Q^T with 32x32x16 instructions, the row on the lane; P^T is the
-// second operand of O^T += V^T . P^T as it stands; values through the transposing LDS read.
+// for all of them while they are stored there: half the waves load keys, half values, to registers a
+// tile ahead, and convert; two stages, one barrier for each tile.  Products and layouts are those of
+// the dense kernel (attention.hip): S^T = K . Q^T with 32x32x16 instructions, the row on the lane;
+// P^T is the second operand of O^T += V^T . P^T as it stands; values through the transposing LDS
+// read.
+// Prompts of 4096, 1115 and 1341 tokens, 32 heads over 8, in 187-204 us: 0.80-0.87 PF/s, where a large
+// bf16 library product reaches 1.19.  Matrix instructions are busy 0.38 of the time and the vector unit
+// (32 exponentials a lane and tile, and the widening) 0.50; the two hardly overlap, neither
+// across waves nor when the second half's exponentials are put between the first half's products
+// (223 us where this order takes 211).  256 rows with eight waves halve the widening and take as long.
 template <int D, int NW>
 __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedParams p) {
   constexpr int M = 32 * NW, ROWB = 2 * D, CPR = ROWB / 16, KSTEPS = D / 16, DVB = D / 32;
@@ -1001,7 +1008,8 @@ __device__ __forceinline__ const float* parts_of(const PagedParams& p, int M, in
 }
 
 // Few rows of q: four waves for each.  Lane c weighs chunk c; the sums run over a few chunks at a
-// time, so that their loads are in flight together.
+// time, so that their loads are in flight together.  Bound by three loads that hang on each other
+// and by the launch: 4 us for 32 rows, 5 for 1024.
 template <int D>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p, int M) {
   __shared__ f32x4 others[3][D / 4];
@@ -1066,7 +1074,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p, int M) {
 }
 
 // Many rows: a wave for four heads of a token, sixteen lanes for each, all chunks in one pass with
-// a running maximum, four of them in flight.
+// a running maximum, four of them in flight (19200 rows of 3 chunks, 30 MB: 8.8 us, with a wave for
+// each row 16).
 template <int D>
 __global__ __launch_bounds__(256) void paged_join_rows_kernel(PagedParams p, int M, int64_t waves, int head_groups) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
