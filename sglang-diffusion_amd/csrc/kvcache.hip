@@ -1,6 +1,7 @@
 // What stands around a paged 8-bit key/value cache, for gfx950: block tables and slot maps from
 // request lengths, rotary positions from scaled frequencies, and the store that rounds keys and
 // values into the cache.  The attention that reads the cache is in paged_attention.hip.
+#include <algorithm>
 #include <type_traits>
 
 #include "common.h"
@@ -255,9 +256,10 @@ constexpr int ROPE_THREADS = 256, ROPE_MAX_HALF = 128, ROPE_MAX_TOKENS = 4;
 // sine of a token are formed once for all its heads and kept in LDS: with 40 heads of 128 that
 // is 1/40 of the fp64 products that forming them at each pair would take.  Bound by memory from some
 // hundred tokens on: 8191 of 40 heads of 128, 168 MB in 35.8 us = 4.7 TB/s (a large copy: 4.9).
+template <int THREADS>
 __device__ __forceinline__ void rope_tokens(const Rope& r, const RopeRows& a, const RopeRows& b, int D,
                                             int64_t t0, int nt, float2* cs) {
-  for (int i = threadIdx.x; i < nt * r.half; i += ROPE_THREADS) {
+  for (int i = threadIdx.x; i < nt * r.half; i += THREADS) {
     const int k = i / r.half;
     cs[i] = rope_cos_sin(r, r.positions[t0 + k], rope_quarters(r, i - k * r.half));
   }
@@ -265,7 +267,7 @@ __device__ __forceinline__ void rope_tokens(const Rope& r, const RopeRows& a, co
   const int turned = r.neox ? r.half / 8 : r.half / 4;
   const int copied = (D - 2 * r.half) / 8;
   const int pieces = turned + copied, heads = a.heads + b.heads;
-  for (int i = threadIdx.x; i < nt * heads * pieces; i += ROPE_THREADS) {
+  for (int i = threadIdx.x; i < nt * heads * pieces; i += THREADS) {
     const int piece = i % pieces, row = i / pieces, head = row % heads, k = row / heads;
     const RopeRows& m = head < a.heads ? a : b;
     const int h = head < a.heads ? head : head - a.heads;
@@ -279,7 +281,7 @@ __global__ __launch_bounds__(ROPE_THREADS) void rope_scaled_kernel(Rope r, RopeR
                                                                    int64_t tokens, int per_group) {
   __shared__ float2 cs[ROPE_MAX_TOKENS * ROPE_MAX_HALF];
   const int64_t t0 = (int64_t)blockIdx.x * per_group;
-  rope_tokens(r, q, k, D, t0, (int)min((int64_t)per_group, tokens - t0), cs);
+  rope_tokens<ROPE_THREADS>(r, q, k, D, t0, (int)min((int64_t)per_group, tokens - t0), cs);
 }
 
 // Tokens of one workgroup: one while there are few, for the sake of latency, then four, since very
@@ -288,18 +290,24 @@ __global__ __launch_bounds__(ROPE_THREADS) void rope_scaled_kernel(Rope r, RopeR
 inline int rope_group(int64_t tokens) { return tokens >= 1024 ? ROPE_MAX_TOKENS : 1; }
 
 // ----------------------------------------------------------------------------------- store --
-// A workgroup owns one run: the tokens of a call that follow each other into one block, for one
-// head and one of the two caches.  The workgroup whose token begins a run (the token before it
-// goes to another block) takes it, so no two of them write one block's scale.  A row of D elements
-// is held by D / 8 lanes, and the 256 threads hold HELD such sets of rows in registers between the
+// A run is the tokens of a call that follow each other into one block, for one head and one of the
+// two caches.  The workgroup among whose tokens a run begins (the token before it goes to another
+// block) takes it, so no two of them write one block's scale.  A team holds it: one wave up to 16 rows
+// of 128, the whole workgroup beyond that, with as many threads as a block's rows ask for.  A row of
+// D elements is held by D / 8 lanes, and the team holds HELD sets of rows in registers between the
 // maximum and the rounding; longer runs are read a second time.  Cosines and sines of these rows
 // are formed together and handed on through LDS.
-// 48 runs of one token take 6 us, bound by the chain slot, row and scale, maximum, code.  4602 tokens of
-// 12 prompts (104 MB with 32 heads of queries) take 41 us = 2.5 TB/s: 15 for the queries, and for keys
-// and values 19 without the rotation and 31 with it, since each head forms the cosines of its
-// rows itself and two runs at most are in flight on a SIMD's registers.  Measured and slower: queries'
-// workgroups in turn with the others (52 us), 128 threads with eight rows each (53-62), 512 with two
-// (45), five or more waves a SIMD, which spill (52-80), two heads to a workgroup (45).
+// Keys come first in the grid, then values, then the queries' rotation: what takes longest begins
+// first.
+//
+// 48 runs of one token take 6 us, bound by the chain slot, row and scale, maximum, code; 1200 of them
+// 30 (run after run by whole workgroups: 106).  4602 tokens of 12 prompts (104 MB with 32 heads of
+// queries) take 37.6 us = 2.8 TB/s: 15 for the queries alone, and for keys and values the chain again
+// and the cosines, which each head forms for itself.  Blocks of 256: 1842 tokens 25 us (with 256
+// threads 70).  Measured and slower: keys and values in turn (44), queries in turn with both (52), 128
+// threads with eight rows each (53-62), 512 with two (45), five or more waves a SIMD, which spill
+// (52-80).
+constexpr int HELD = 4;
 struct StoreParams {
   const unsigned short *k, *v;
   int64_t k_st, k_sh, v_st, v_sh;
@@ -309,7 +317,7 @@ struct StoreParams {
   const int64_t* slots;
   int64_t tokens, num_blocks;
   int Hk, lb, group;
-  unsigned kv_groups;  // workgroups before those that turn the queries
+  unsigned kv_groups;  // workgroups before those that turn the queries; half of them keys'
   int q_group;
   Rope rope;           // positions == nullptr: keys are stored as they are
   RopeRows q;
@@ -338,87 +346,110 @@ __device__ __forceinline__ u32x2 round_fp8(const float (&f)[8], float inv) {
   return o;
 }
 
-// HELD sets: of 16 rows of 128, or 32 of 64
-template <int D, int HELD>
+// THREADS that hold a run together.  A wave has room for the cosines of one set of rows (4 of 128, 8 of
+// 64), a workgroup for those of 1024 / (D / 8) rows.
+template <int D, int THREADS>
 struct StoreLds {
-  static constexpr int ROWS = 256 / (D / 8);  // of a set
-  float2 cs[HELD * ROWS][D / 2];
-  float top[4];
-  int first[4];
+  static constexpr int ROWS = THREADS / (D / 8);  // of a set
+  static constexpr int TURNED = THREADS == 64 ? 1 : 1024 / THREADS;  // sets whose cosines there is room for
+  float2 cs[TURNED * ROWS][D / 2];
+  float top[THREADS / 64];
+  int first[THREADS / 64];
 };
+// what one thread of a team wrote to LDS is there for the others
+template <int THREADS>
+__device__ __forceinline__ void team_sync() {
+  if constexpr (THREADS > 64) {
+    __syncthreads();
+  } else {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+}
 
-template <int D, int HELD, bool KEYS>
-__device__ void store_run(const StoreParams& p, int64_t t0, int64_t len, int64_t block, int head,
-                          StoreLds<D, HELD>& lds) {
-  constexpr int LPR = D / 8, ROWS = StoreLds<D, HELD>::ROWS, CHUNK = HELD * ROWS;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = threadIdx.x % LPR, sub = threadIdx.x / LPR;
+template <int D, int THREADS>
+__device__ void store_run(const StoreParams& p, bool keys, int t0, int len, int block, int head,
+                          StoreLds<D, THREADS>& lds) {
+  constexpr int LPR = D / 8, ROWS = StoreLds<D, THREADS>::ROWS, CHUNK = HELD * ROWS;
+  const int lane = threadIdx.x & 63, wave = THREADS > 64 ? threadIdx.x >> 6 : 0;  // of the team
+  const int c = lane % LPR, sub = (64 * wave + lane) / LPR;
   const int bs = 1 << p.lb;
   const Rope& r = p.rope;
-  const bool turned = KEYS && r.positions;
-  float* scale_at = (KEYS ? p.k_scale : p.v_scale) + block * p.Hk + head;
+  const bool turned = keys && r.positions;
+  float* scale_at = (keys ? p.k_scale : p.v_scale) + (int64_t)block * p.Hk + head;
   const float old = *scale_at;
   u32x4 held[HELD];
   int place[HELD];  // in the block; bs: no row
   // CHUNK rows of the run, keys rotated.  The rotated key is a bf16 value before it is rounded to 8
   // bits, as it would be between the rotary operator and the store.
-  auto fetch = [&](int64_t row0) {
+  const int64_t st = keys ? p.k_st : p.v_st;
+  const unsigned short* rows_at = (keys ? p.k + head * p.k_sh : p.v + head * p.v_sh) + t0 * st;
+  const int64_t* slots_at = p.slots + t0;
+  const int64_t* positions_at = r.positions + t0;
+  auto fetch = [&](int row0) {
 #pragma unroll
     for (int h = 0; h < HELD; ++h) {
-      const int64_t row = row0 + h * ROWS + sub, t = t0 + row;
+      const int row = row0 + h * ROWS + sub;
       held[h] = u32x4{0, 0, 0, 0};
       place[h] = bs;
       if (row < len) {
-        held[h] = *reinterpret_cast<const u32x4*>((KEYS ? p.k + t * p.k_st + head * p.k_sh
-                                                        : p.v + t * p.v_st + head * p.v_sh) + 8 * c);
-        place[h] = (int)(p.slots[t] & (bs - 1));
+        held[h] = *reinterpret_cast<const u32x4*>(rows_at + row * st + 8 * c);
+        place[h] = (int)slots_at[row] & (bs - 1);
       }
     }
     if (!turned) return;
-    const int rows = (int)min((int64_t)CHUNK, len - row0);
-    __syncthreads();  // what was here before has been read
-    // a lane keeps its pair, and goes over the rows
-    const int side = 64 / r.half, pair = lane % r.half, k0 = wave * side + lane / r.half;
-    if (lane < side * r.half) {
-      const double each = rope_quarters(r, pair);
-#pragma unroll 4
-      for (int k = k0; k < rows; k += 4 * side) lds.cs[k][pair] = rope_cos_sin(r, r.positions[t0 + row0 + k], each);
-    }
-    __syncthreads();
-    const bool mine = 8 * c < 2 * r.half;
+    constexpr int TURNED = StoreLds<D, THREADS>::TURNED;
 #pragma unroll
-    for (int h = 0; h < HELD; ++h) {
-      float f[8];
-      unpack8(held[h], f);
-      const float2* cs = lds.cs[h * ROWS + sub];
-      if (r.neox) {
-        // the other element of each pair is `half` away: half / 8 lanes, in the same row and wave
-        const int away = r.half / 8;
-        const bool second = c >= away;
-        const int from = mine ? (second ? lane - away : lane + away) : lane;
-        u32x4 other;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) other[j] = __shfl(held[h][j], from, 64);
-        float g[8];
-        unpack8(other, g);
-        if (mine && place[h] < bs) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float2 w = cs[(second ? c - away : c) * 8 + j];
-            if (second) turn(g[j], f[j], w);
-            else turn(f[j], g[j], w);
-          }
-        }
-      } else if (mine && place[h] < bs) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) turn(f[2 * j], f[2 * j + 1], cs[c * 4 + j]);
+    for (int h0 = 0; h0 < HELD; h0 += TURNED) {
+      const int from = row0 + h0 * ROWS;
+      if (h0 && from >= len) break;
+      const int rows = min(TURNED * ROWS, len - from);
+      team_sync<THREADS>();  // what was here before has been read
+      // a lane keeps its pair, and goes over the rows
+      const int side = 64 / r.half, pair = lane % r.half, k0 = wave * side + lane / r.half;
+      if (lane < side * r.half) {
+        const double each = rope_quarters(r, pair);
+#pragma unroll 1
+        for (int k = k0; k < rows; k += THREADS / 64 * side)
+          lds.cs[k][pair] = rope_cos_sin(r, positions_at[from + k], each);
       }
-      held[h] = pack8(f);
+      team_sync<THREADS>();
+      const bool mine = 8 * c < 2 * r.half;
+#pragma unroll
+      for (int h = h0; h < h0 + TURNED; ++h) {
+        float f[8];
+        unpack8(held[h], f);
+        const float2* cs = lds.cs[(h - h0) * ROWS + sub];
+        if (r.neox) {
+          // the other element of each pair is `half` away: half / 8 lanes, in the same row and wave
+          const int away = r.half / 8;
+          const bool second = c >= away;
+          const int from = mine ? (second ? lane - away : lane + away) : lane;
+          u32x4 other;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) other[j] = __shfl(held[h][j], from, 64);
+          float g[8];
+          unpack8(other, g);
+          if (mine && place[h] < bs) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float2 w = cs[(second ? c - away : c) * 8 + j];
+              if (second) turn(g[j], f[j], w);
+              else turn(f[j], g[j], w);
+            }
+          }
+        } else if (mine && place[h] < bs) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) turn(f[2 * j], f[2 * j + 1], cs[c * 4 + j]);
+        }
+        held[h] = pack8(f);
+      }
     }
   };
   // the largest finite magnitude and the smallest place in the block
   float top = 0.f;
   int first = bs;
-  for (int64_t row0 = 0; row0 < len; row0 += CHUNK) {
+  for (int row0 = 0; row0 < len; row0 += CHUNK) {
     fetch(row0);
 #pragma unroll
     for (int h = 0; h < HELD; ++h) {
@@ -433,24 +464,26 @@ __device__ void store_run(const StoreParams& p, int64_t t0, int64_t len, int64_t
   top = group_max<64>(top);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) first = min(first, __shfl_xor(first, o, 64));
-  __syncthreads();  // the run before has been read, and every thread has the old scale
-  if (lane == 0) {
-    lds.top[wave] = top;
-    lds.first[wave] = first;
-  }
-  __syncthreads();
+  team_sync<THREADS>();  // the run before has been read, and every thread has the old scale
+  if constexpr (THREADS > 64) {
+    if (lane == 0) {
+      lds.top[wave] = top;
+      lds.first[wave] = first;
+    }
+    __syncthreads();
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    top = fmaxf(top, lds.top[w]);
-    first = min(first, lds.first[w]);
+    for (int w = 0; w < THREADS / 64; ++w) {
+      top = fmaxf(top, lds.top[w]);
+      first = min(first, lds.first[w]);
+    }
   }
   // the smallest power of two with top <= 448 * 2^e: 448 = 1.75 * 2^8
   const unsigned bits = __float_as_uint(top);
   const int e = max(SCALE_EXP_MIN, (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0));
   float scale = __uint_as_float((unsigned)(e + 127) << 23);
-  unsigned char* cache = (KEYS ? p.k_cache : p.v_cache) + block * (KEYS ? p.kc_sb : p.vc_sb) +
-                         head * (KEYS ? p.kc_sh : p.vc_sh) + 8 * c;
-  const int64_t row_bytes = KEYS ? p.kc_st : p.vc_st;
+  unsigned char* cache = (keys ? p.k_cache : p.v_cache) + (int64_t)block * (keys ? p.kc_sb : p.vc_sb) +
+                         head * (keys ? p.kc_sh : p.vc_sh) + 8 * c;
+  const int64_t row_bytes = keys ? p.kc_st : p.vc_st;
   if (first > 0) {
     if (old >= scale) {
       scale = old;
@@ -474,9 +507,9 @@ __device__ void store_run(const StoreParams& p, int64_t t0, int64_t len, int64_t
       }
     }
   }
-  if (threadIdx.x == 0) *scale_at = scale;
+  if (wave == 0 && lane == 0) *scale_at = scale;
   const float inv = 1.f / scale;  // exact: a power of two (a scale that a caller set may be any)
-  for (int64_t row0 = 0; row0 < len; row0 += CHUNK) {
+  for (int row0 = 0; row0 < len; row0 += CHUNK) {
     if (len > CHUNK) fetch(row0);
 #pragma unroll
     for (int h = 0; h < HELD; ++h) {
@@ -487,45 +520,65 @@ __device__ void store_run(const StoreParams& p, int64_t t0, int64_t len, int64_t
   }
 }
 
-template <int D, int HELD>
-__global__ __launch_bounds__(256, 4) void kv_store_kernel(StoreParams p) {
+template <int D, int THREADS>
+__global__ __launch_bounds__(THREADS, 4) void kv_store_kernel(StoreParams p) {
+  constexpr int WAVES = THREADS / 64;
   __shared__ union {
     float2 q[ROPE_MAX_HALF * ROPE_MAX_TOKENS];
-    StoreLds<D, HELD> kv;
+    StoreLds<D, THREADS> kv;
+    StoreLds<D, 64> wave[WAVES];
   } lds;
   if (blockIdx.x >= p.kv_groups) {
     const int64_t t0 = (int64_t)(blockIdx.x - p.kv_groups) * p.q_group;
-    rope_tokens(p.rope, p.q, RopeRows{nullptr, nullptr, 0, 0, 0, 0, 0}, D, t0,
-                (int)min((int64_t)p.q_group, p.tokens - t0), lds.q);
+    rope_tokens<THREADS>(p.rope, p.q, RopeRows{nullptr, nullptr, 0, 0, 0, 0, 0}, D, t0,
+                         (int)min((int64_t)p.q_group, p.tokens - t0), lds.q);
     return;
   }
   // a workgroup: (group of tokens, head, keys or values); each wave finds the runs that begin there
-  const unsigned which = blockIdx.x % (2 * p.Hk);
-  const int64_t g = blockIdx.x / (2 * p.Hk);
-  const int head = (int)(which >> 1);
-  const int lane = threadIdx.x & 63;
-  const int64_t w0 = g * p.group, t = w0 + lane;  // 64 slots: the group's and those behind it
+  const unsigned half = p.kv_groups / 2;
+  const bool keys = blockIdx.x < half;
+  const unsigned part = keys ? blockIdx.x : blockIdx.x - half;
+  const int head = (int)(part % p.Hk);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int w0 = (int)(part / p.Hk) * p.group, t = w0 + lane;  // 64 slots: the group's and those behind it
   const int64_t limit = p.num_blocks << p.lb;
   const int64_t s = t < p.tokens ? p.slots[t] : -1;
   const int64_t before = t > 0 && t < p.tokens ? p.slots[t - 1] : -1;
-  const int64_t block = s < 0 ? -1 : s >> p.lb;
-  unsigned long long todo =
-      __ballot(lane < p.group && s >= 0 && s < limit && (before < 0 || (before >> p.lb) != block));
-  while (todo) {
-    const int l = __ffsll(todo) - 1;
-    todo &= todo - 1;
-    const int64_t mine = __shfl(block, l, 64);
-    // the length of the run: to the first slot of another block, if need be behind these 64
-    int64_t len = 0;
+  const int block = s < 0 || s >= limit ? -1 : (int)(s >> p.lb);
+  const unsigned long long begins =
+      __ballot(lane < p.group && block >= 0 && (before < 0 || (before >> p.lb) != block));
+  // the run that begins at lane l: its block, and its length, to the first slot of another block, if
+  // need be behind these 64
+  auto run_at = [&](int l, int& mine, int& len) {
+    mine = __builtin_amdgcn_readlane(block, l);
+    len = 0;
     unsigned long long out = __ballot(lane >= l && block != mine);
     if (out) len = __ffsll(out) - 1 - l;
-    for (int64_t at = w0 + 64; !out; at += 64) {
+    for (int at = w0 + 64; !out; at += 64) {
       const int64_t s2 = at + lane < p.tokens ? p.slots[at + lane] : -1;
       out = __ballot(s2 < 0 || (s2 >> p.lb) != mine);
       len = at - w0 - l + (out ? __ffsll(out) - 1 : 0);
     }
-    if (which & 1) store_run<D, HELD, false>(p, w0 + l, len, mine, head, lds.kv);
-    else store_run<D, HELD, true>(p, w0 + l, len, mine, head, lds.kv);
+  };
+  // runs that a wave holds go to the waves in turn, the others to all of them together
+  unsigned long long few = 0;
+  constexpr int FEW = HELD * StoreLds<D, 64>::ROWS;
+  int mine, len;
+  for (unsigned long long todo = begins; todo; todo &= todo - 1) {
+    const int l = __ffsll(todo) - 1;
+    run_at(l, mine, len);
+    if (len <= FEW) {
+      few |= 1ull << l;
+      continue;
+    }
+    store_run<D, THREADS>(p, keys, w0 + l, len, mine, head, lds.kv);
+  }
+  if (few != begins) __syncthreads();  // (the LDS is used anew)
+  for (int i = 0; few; few &= few - 1, i = i + 1 == WAVES ? 0 : i + 1) {
+    if (i != wave) continue;
+    const int l = __ffsll(few) - 1;
+    run_at(l, mine, len);
+    store_run<D, 64>(p, keys, w0 + l, len, mine, head, lds.wave[wave]);
   }
 }
 
@@ -637,7 +690,7 @@ extern "C" int mi355_kv_store_fp8(const mi355_kv_store_args* a, void* stream) {
   MI355_REQUIRE(a->D == 64 || a->D == 128, "kv_store_fp8: head size %ld not in {64,128}", (long)a->D);
   MI355_REQUIRE(block_size_ok(a->block_size), "kv_store_fp8: block size %ld must be a power of two in [16, 1024]",
                 (long)a->block_size);
-  MI355_REQUIRE(a->tokens >= 0 && a->tokens < (1ll << 31) && a->Hk > 0 && a->Hk < 65536 && a->Hq >= 0 &&
+  MI355_REQUIRE(a->tokens >= 0 && a->tokens <= (1ll << 31) - 4096 && a->Hk > 0 && a->Hk < 65536 && a->Hq >= 0 &&
                     a->Hq < 65536 && a->num_blocks >= 0 && a->num_blocks < (1ll << 31),
                 "kv_store_fp8: bad shape");
   if (a->tokens == 0) return MI355_OK;
@@ -677,13 +730,16 @@ extern "C" int mi355_kv_store_fp8(const mi355_kv_store_args* a, void* stream) {
   p.num_blocks = a->num_blocks;
   p.Hk = (int)a->Hk;
   p.lb = log2_of(a->block_size);
-  // Tokens that a workgroup looks at for the beginning of a run: one while there are few tokens
-  // (each may be a request of its own, and runs that one workgroup finds are stored one after the
-  // other), then as many as keep the launch to about twice the workgroups that the chip holds: most
-  // of them find no run where tokens follow each other, and take a place for the while (4602 tokens
-  // of 12 prompts, 8 heads: 43 us, with groups of 32 53 us, of 16 54 us).
-  p.group = 1;
-  while (p.group < 64 && (a->tokens + p.group - 1) / p.group * 2 * a->Hk > 2048) p.group *= 2;
+  // Threads for the rows that a run can have: 256 hold 64 rows of 128, 1024 hold 256.
+  const int64_t rows = std::min(a->block_size, a->tokens), held = HELD * 256 * 8 / a->D;
+  const int threads = rows > 2 * held ? 1024 : rows > held ? 512 : 256;
+  // Tokens among which a workgroup looks for the beginning of a run: one for each of its waves while
+  // there are few tokens (each may be a request of its own), then as many as keep the launch to about
+  // twice the workgroups that the chip holds: most find no run where tokens follow each other, and
+  // take a place for the while (4602 tokens of 12 prompts, 8 heads: groups of 64 43 us, of 32 53).
+  const int64_t most = threads > 256 ? 1024 : 2048;
+  p.group = threads / 64;
+  while (p.group < 64 && (a->tokens + p.group - 1) / p.group * 2 * a->Hk > most) p.group *= 2;
   const int64_t units = (a->tokens + p.group - 1) / p.group * 2 * a->Hk;
   MI355_REQUIRE(units + a->tokens < (1ll << 31), "kv_store_fp8: too many tokens and heads for one call");
   p.kv_groups = (unsigned)units;
@@ -693,16 +749,16 @@ extern "C" int mi355_kv_store_fp8(const mi355_kv_store_args* a, void* stream) {
                 a->attn_factor};
   p.q = RopeRows{(const unsigned short*)a->q, (unsigned short*)a->q_out, a->q_st, a->q_sh, a->qo_st, a->qo_sh,
                  (int)a->Hq};
-  const dim3 grid(p.kv_groups + q_groups), block(256);
-  // with one token to look at, runs are likely short: one set of rows, and the registers of one
+  const dim3 grid(p.kv_groups + q_groups);
   hipStream_t st = (hipStream_t)stream;
-  if (a->D == 128) {
-    if (p.group == 1) hipLaunchKernelGGL((kv_store_kernel<128, 1>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((kv_store_kernel<128, 4>), grid, block, 0, st, p);
-  } else {
-    if (p.group == 1) hipLaunchKernelGGL((kv_store_kernel<64, 1>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((kv_store_kernel<64, 4>), grid, block, 0, st, p);
-  }
+  auto launch = [&](auto threads) {
+    constexpr int T = decltype(threads)::value;
+    if (a->D == 128) hipLaunchKernelGGL((kv_store_kernel<128, T>), grid, dim3(T), 0, st, p);
+    else hipLaunchKernelGGL((kv_store_kernel<64, T>), grid, dim3(T), 0, st, p);
+  };
+  if (threads == 1024) launch(std::integral_constant<int, 1024>{});
+  else if (threads == 512) launch(std::integral_constant<int, 512>{});
+  else launch(std::integral_constant<int, 256>{});
   MI355_CHECK_LAUNCH("kv_store_fp8");
   return MI355_OK;
 }

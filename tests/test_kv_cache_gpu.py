@@ -280,6 +280,38 @@ def test_store_many_tokens(device):
     check_store(k, v, kc, vc, ks, vs, whole)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("block,requests,longest", [(16, 5, 3), (16, 700, 2), (64, 300, 40), (128, 20, 300), (256, 900, 1),
+                                                    (512, 9, 600)])
+def test_store_of_many_requests(device, block, requests, longest, D):
+    """Runs of one token to whole blocks side by side, most of them behind tokens of earlier calls,
+    with the rotation, against the two operators apart."""
+    import sgl_kernel
+
+    heads = 2
+    g = torch.Generator().manual_seed(block + requests)
+    lens = torch.exp(torch.rand(requests, generator=g) * math.log(longest + 0.99)).int().tolist()
+    slots, used = [], 0
+    for n in lens:
+        first = int(torch.randint(0, block, (1,), generator=g))
+        slots += [(used + (first + i) // block) * block + (first + i) % block for i in range(n)]
+        used += -(-(first + n) // block)
+    T = len(slots)
+    kc, ks = empty_cache(used, block, heads, D, 16)
+    vc, vs = empty_cache(used, block, heads, D, 17)
+    size = torch.exp(2.0 * torch.randn(T, 1, 1, generator=g))
+    k, v = ((torch.randn(T, heads, D, generator=g) * size).bfloat16().to(DEV) for _ in range(2))
+    f = (10000.0 ** (-torch.arange(0, D, 2, dtype=torch.float64) / D)).to(DEV)
+    positions = torch.randint(0, 100000, (T,), generator=g).to(DEV)
+    both = [t.clone() for t in (kc, vc, ks, vs)]
+    sgl_kernel.store_kv_cache_fp8(k, v, *both, torch.tensor(slots, device=DEV), None, positions, f)
+    turned = k.clone()
+    sgl_kernel.rotary_embedding_scaled(positions, turned, None, f)
+    check_store(turned, v, kc, vc, ks, vs, slots)
+    for a, b in zip((kc, vc, ks, vs), both):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
 def test_store_values_at_the_edges(device):
     """Zeros, the borders of a power of two, tiny and huge values, infinities and NaN."""
     block, heads, D = 16, 1, 64
