@@ -284,10 +284,11 @@ __global__ __launch_bounds__(ROPE_THREADS) void rope_scaled_kernel(Rope r, RopeR
   rope_tokens<ROPE_THREADS>(r, q, k, D, t0, (int)min((int64_t)per_group, tokens - t0), cs);
 }
 
-// Tokens of one workgroup: one while there are few, for the sake of latency, then four, since very
-// many small workgroups are held up by their own dispatch (8191 tokens, 40 heads of 128, half of a
-// head turned: 36.5 us, with one token 38.0, with eight 46.7).
-inline int rope_group(int64_t tokens) { return tokens >= 1024 ? ROPE_MAX_TOKENS : 1; }
+// Tokens of one workgroup: one, until there are some thirty for each CU, since the last round of
+// long workgroups leaves much of the chip idle (1714 tokens, 144 heads of 128: 34 us, by fours 55); then
+// four, since very many small workgroups are held up by their own dispatch (60000 tokens, 3 heads of
+// 64: 17 us, by ones 44; 8191 tokens, 40 heads of 128: 37.4 us, by ones 38.0, by eights 46.7).
+inline int rope_group(int64_t tokens) { return tokens >= 7168 ? ROPE_MAX_TOKENS : 1; }
 
 // ----------------------------------------------------------------------------------- store --
 // A run is the tokens of a call that follow each other into one block, for one head and one of the
@@ -743,7 +744,9 @@ extern "C" int mi355_kv_store_fp8(const mi355_kv_store_args* a, void* stream) {
   const int64_t units = (a->tokens + p.group - 1) / p.group * 2 * a->Hk;
   MI355_REQUIRE(units + a->tokens < (1ll << 31), "kv_store_fp8: too many tokens and heads for one call");
   p.kv_groups = (unsigned)units;
-  p.q_group = rope_group(a->tokens);
+  // tokens of a workgroup that turns queries: with 256 threads two (8 x 600 tokens 37.8 us, one 39.6, four
+  // 38.9), with more four (1842 tokens 24.9, one 29)
+  p.q_group = a->tokens < 1024 ? 1 : threads > 256 ? 4 : 2;
   const unsigned q_groups = a->Hq ? (unsigned)((a->tokens + p.q_group - 1) / p.q_group) : 0;
   p.rope = Rope{a->positions, a->inv_freq, a->inv_freq_is_f64, (int)(a->rot_dim / 2), a->is_neox != 0,
                 a->attn_factor};
