@@ -100,6 +100,7 @@ constexpr int SORTED_SEQS = 16;
 template <int M>
 __device__ __forceinline__ void find_longest(const PagedParams& p, int item, Item* found) {
   const int lane = threadIdx.x;
+  if (lane == 0) found->b = -1;
   const Seq s = seq_of(p, min(lane, p.B - 1));
   const int base = s.len - s.n, tiles = (s.n * p.G + M - 1) / M;
   // levels there are, at most, in tiles of keys; step <= 33
@@ -124,10 +125,7 @@ __device__ __forceinline__ void find_longest(const PagedParams& p, int item, Ite
 #pragma unroll 1
   for (int s2 = step; s2; s2 = s2 > 1 ? 1 : 0) {
     const int n = __popcll(__builtin_amdgcn_ballot_w64(above(level + lane * s2) > item));
-    if (n == 0) {  // behind the last item
-      if (lane == 0) found->b = -1;
-      return;
-    }
+    if (n == 0) return;  // behind the last item
     level += (n - 1) * s2;
   }
   int k = item - above(level + 1);
@@ -399,6 +397,8 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void paged_few_rows_kernel(Pa
   // eight items side by side, so that all heads of an item are on one of the eight XCDs
   const int groups = p.Hk / p.hw, item = (blockIdx.x / (8 * groups)) * 8 + blockIdx.x % 8;
   const int group = (blockIdx.x / 8) % groups;
+  // (the grid is whole eights of items; running sums that are none could find work for the rest)
+  if (item >= p.items) return;
   Item it;
   if (!find_item<M>(p, item, group, &it)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
