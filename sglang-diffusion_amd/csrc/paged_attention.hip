@@ -674,14 +674,17 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void paged_few_rows_kernel(Pa
 // the dense kernel (attention.hip): S^T = K . Q^T with 32x32x16 instructions, the row on the lane;
 // P^T is the second operand of O^T += V^T . P^T as it stands; values through the transposing LDS
 // read.
+// Up to 64 rows (HALVES = 2) two waves share 32 rows, each with half of a tile's keys, since a wave's
+// chain of products, exponentials and products is what a tile then takes: 32 rows over 60 thousand
+// keys 104 us, with two waves idle 116; 64 rows 120 and 143.
 // Prompts of 4096, 1115 and 1341 tokens, 32 heads over 8, in 187-204 us: 0.80-0.87 PF/s, where a large
 // bf16 library product reaches 1.19.  Matrix instructions are busy 0.38 of the time and the vector unit
 // (32 exponentials a lane and tile, and the widening) 0.50; the two hardly overlap, neither
 // across waves nor when the second half's exponentials are put between the first half's products
 // (223 us where this order takes 211).  256 rows with eight waves halve the widening and take as long.
-template <int D, int NW>
+template <int D, int NW, int HALVES>
 __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedParams p) {
-  constexpr int M = 32 * NW, ROWB = 2 * D, CPR = ROWB / 16, KSTEPS = D / 16, DVB = D / 32;
+  constexpr int RANKS = NW / HALVES, M = 32 * RANKS, KB = 2 / HALVES, ROWB = 2 * D, CPR = ROWB / 16, KSTEPS = D / 16, DVB = D / 32;
   constexpr int TILE = KT * ROWB, LOADS = KT * D / 16 / (NW * 32);
   static_assert(LOADS >= 1, "every thread loads");
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -692,15 +695,16 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedP
   const Job job = job_of<M>(p, it, hk);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 31, hh = lane >> 5;
+  const int rank = wave % RANKS, half = wave / RANKS;  // rows, and keys of each tile, of the wave
   auto k_swz = [](int key) { return key & 15 & (CPR - 1); };
   auto v_swz = [](int key) { return (((key & 3) << 2) | ((key >> 2) & 3)) & (CPR - 1); };
 
-  const int row = min(job.row0 + 32 * wave + r, job.rows - 1), tok = row / p.G, head = hk * p.G + row - tok * p.G;
+  const int row = min(job.row0 + 32 * rank + r, job.rows - 1), tok = row / p.G, head = hk * p.G + row - tok * p.G;
   const int base = job.s.len - job.s.n, place = base + tok;
   const int see_hi = min(p.causal ? place : job.s.len - 1, job.s.len - 1);
   const int see_lo = p.window >= 0 ? place - p.window : 0;
   // places of the wave's first and last row
-  const int wave_row = min(job.row0 + 32 * wave, job.rows - 1);
+  const int wave_row = min(job.row0 + 32 * rank, job.rows - 1);
   const int w_lo = base + wave_row / p.G, w_hi = base + min(wave_row + 31, job.rows - 1) / p.G;
   bf16x8 qf[KSTEPS];
   {
@@ -795,7 +799,7 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedP
     sc = scales_of(p, p.ks[at], p.vs[at]);
     store(now, job.t0, 0);
   }
-  const bool live_wave = job.row0 + 32 * wave < job.rows;
+  const bool live_wave = job.row0 + 32 * rank < job.rows;
   // the queries are here before the loop begins: waited for inside it, they would hold up the loads
   // of the next tile with them at every turn
 #pragma unroll
@@ -810,48 +814,50 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedP
     const float ks = p.ks[scale_at], vs = p.vs[scale_at];
     if (more) load(next, t + 1);
     if (live_wave && !(p.causal && key0 > w_hi) && !(p.window >= 0 && key0 + KT - 1 < w_lo - p.window)) {
-      const unsigned char *kt = smem + buf * 2 * TILE, *vt = kt + TILE;
-      f32x16 s[2];
+      const unsigned char *kt = smem + buf * 2 * TILE + half * 32 * ROWB, *vt = kt + TILE;
+      const int key1 = key0 + 32 * half;
+      f32x16 s[KB];
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
+      for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[kb][e] = 0.f;
-      bf16x8 kf[2][2];
+      bf16x8 kf[2][KB];
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) kf[0][kb] = *reinterpret_cast<const bf16x8*>(kt + kb * 32 * ROWB + koff[0]);
+      for (int kb = 0; kb < KB; ++kb) kf[0][kb] = *reinterpret_cast<const bf16x8*>(kt + kb * 32 * ROWB + koff[0]);
 #pragma unroll
       for (int st = 0; st < KSTEPS; ++st) {
         if (st + 1 < KSTEPS) {
 #pragma unroll
-          for (int kb = 0; kb < 2; ++kb)
+          for (int kb = 0; kb < KB; ++kb)
             kf[(st + 1) & 1][kb] = *reinterpret_cast<const bf16x8*>(kt + kb * 32 * ROWB + koff[st + 1]);
         }
         __builtin_amdgcn_sched_barrier(0);  // the reads of a step stay ahead of the products before it
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int kb = 0; kb < KB; ++kb)
           s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[st & 1][kb], qf[st], s[kb], 0, 0, 0);
       }
       const bool masked = key0 + KT > job.s.len || now.ok != 15u || (p.causal && key0 + KT - 1 > w_lo) ||
                           (p.window >= 0 && key0 < w_hi - p.window);
       // as in the kernel above: x[c][e] is element e of piece c
-      float x[4][8], sum[4];
+      float x[2 * KB][8], sum[2 * KB];
+      auto mine = [&](const float (&v)[4], int c) { return HALVES == 2 && half ? v[2 + c % 2] : v[c]; };
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const float add = sc.v_log[c] - m;
+      for (int c = 0; c < 2 * KB; ++c) {
+        const float add = mine(sc.v_log, c) - m, scale = mine(sc.k, c);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[c][e] = fmaf(s[c >> 1][8 * (c & 1) + e], sc.k[c], add);
+        for (int e = 0; e < 8; ++e) x[c][e] = fmaf(s[c >> 1][8 * (c & 1) + e], scale, add);
       }
       if (masked) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < 2 * KB; ++c)
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            x[c][e] = sees((now.ok >> c) & 1, key0 + 16 * c + (e & 3) + 8 * (e >> 2) + 4 * hh, see_lo, see_hi)
+            x[c][e] = sees((now.ok >> (2 * half + c)) & 1, key1 + 16 * c + (e & 3) + 8 * (e >> 2) + 4 * hh, see_lo, see_hi)
                           ? x[c][e] : -INFINITY;
       }
       float top = x[0][0];
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
+      for (int c = 0; c < 2 * KB; ++c)
 #pragma unroll
         for (int e = 0; e < 8; ++e) top = fmaxf(top, x[c][e]);
       if (__builtin_amdgcn_ballot_w64(top > LAZY || l == 0.f) != 0) {
@@ -863,12 +869,12 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedP
 #pragma unroll
           for (int e = 0; e < 16; ++e) o[d][e] *= mv.shrink;
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < 2 * KB; ++c)
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[c][e] -= mv.by;
       }
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < 2 * KB; ++c) {
         sum[c] = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -877,16 +883,16 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedP
         }
       }
 #pragma unroll
-      for (int c = 0; c < 4; ++c) l = fmaf(sum[c], sc.v_inv[c], l);
-      f16x8 pf[2][2];
+      for (int c = 0; c < 2 * KB; ++c) l = fmaf(sum[c], mine(sc.v_inv, c), l);
+      f16x8 pf[KB][2];
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
+      for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int st = 0; st < 2; ++st)
 #pragma unroll
           for (int j = 0; j < 8; ++j) pf[kb][st][j] = (_Float16)x[2 * kb + st][j];
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
+      for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int st = 0; st < 2; ++st)
 #pragma unroll
@@ -930,7 +936,31 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedP
   }
 
   l += __shfl_xor(l, 32, 64);
-  const int in_tile = 32 * wave + r;
+  if constexpr (HALVES == 2) {
+    // the two waves of each row, through LDS as they lie in the lanes
+    float* at = reinterpret_cast<float*>(smem) + rank * (DVB * 16 + 2) * 64 + lane;
+    if (l == 0.f) m = M_EMPTY;
+    __syncthreads();
+    if (half) {
+#pragma unroll
+      for (int d = 0; d < DVB; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) at[(16 * d + e) * 64] = o[d][e];
+      at[16 * DVB * 64] = m;
+      at[(16 * DVB + 1) * 64] = l;
+    }
+    __syncthreads();
+    if (half) return;
+    const float m1 = at[16 * DVB * 64], l1 = at[(16 * DVB + 1) * 64], top = fmaxf(m, m1);
+    const float w0 = __builtin_amdgcn_exp2f(m - top), w1 = __builtin_amdgcn_exp2f(m1 - top);
+#pragma unroll
+    for (int d = 0; d < DVB; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[d][e] = fmaf(o[d][e], w0, at[(16 * d + e) * 64] * w1);
+    l = fmaf(l, w0, l1 * w1);
+    m = top;
+  }
+  const int in_tile = 32 * rank + r;
   if (it.chunks > 1) {
     float* part = p.part + ((int64_t)hk * p.items + item) * (M * (D + 2));
 #pragma unroll
@@ -1161,10 +1191,11 @@ Plan plan_of(const mi355_paged_attn_args* a) {
   Plan w;
   const int64_t G = a->H / a->Hk, rows = a->max_seqlen_q * G;
   const int64_t all_rows = (a->cu_seqlens_q ? a->Sq : a->Sq * a->B) * G;
-  // (two tiles of sixteen rows in the first kernel gain nothing: 32 rows over 8 to 60 thousand keys
-  // take 33 and 116 us there, 23 and 117 us in the second)
+  // three kinds of row tiles: 16, 64 with two waves for each row, 128 (two tiles of sixteen rows in the
+  // first kernel gain nothing: 32 rows over 8 to 60 thousand keys take 33 and 116 us there, 21 and
+  // 104 us with a tile of 64)
   w.few = rows <= 16;
-  w.M = w.few ? 16 : 128;
+  w.M = w.few ? 16 : rows <= 64 ? 64 : 128;
   // as many heads to a workgroup as share its four waves: what they read lies side by side
   w.hw = !w.few ? 1 : a->Hk % 4 == 0 ? 4 : a->Hk % 2 == 0 ? 2 : 1;
   const int64_t tiles = all_rows / w.M + a->B;  // row tiles: at most one not full for each sequence
@@ -1207,28 +1238,34 @@ int check(const mi355_paged_attn_args* a) {
   return MI355_OK;
 }
 
+template <int D, int HALVES>
+int launch_many(const PagedParams& p, dim3 grid, hipStream_t st) {
+  constexpr int LDS = 4 * KT * D * 2;  // two stages of keys and values
+  // the limit of dynamic LDS is an attribute of the function on each device
+  static std::atomic<unsigned long long> known{0};
+  int dev = 0;
+  (void)hipGetDevice(&dev);
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (!(known.load(std::memory_order_acquire) & bit)) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(paged_many_rows_kernel<D, 4, HALVES>),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    if (e != hipSuccess) {
+      mi355_set_error("paged_attn_fp8: cannot reserve %d B of LDS: %s", LDS, hipGetErrorString(e));
+      return MI355_EHIP;
+    }
+    known.fetch_or(bit, std::memory_order_release);
+  }
+  hipLaunchKernelGGL((paged_many_rows_kernel<D, 4, HALVES>), grid, dim3(256), LDS, st, p);
+  return MI355_OK;
+}
+
 template <int D>
 int launch(const PagedParams& p, const Plan& w, hipStream_t st) {
   const dim3 grid((unsigned)(w.few ? (w.items + 7) / 8 * 8 * (p.Hk / w.hw) : w.items * p.Hk));
   if (w.few) {
     hipLaunchKernelGGL(paged_few_rows_kernel<D>, grid, dim3(256), 0, st, p);
   } else {
-    constexpr int LDS = 4 * KT * D * 2;  // two stages of keys and values
-    // the limit of dynamic LDS is an attribute of the function on each device
-    static std::atomic<unsigned long long> known{0};
-    int dev = 0;
-    (void)hipGetDevice(&dev);
-    const unsigned long long bit = 1ull << (dev & 63);
-    if (!(known.load(std::memory_order_acquire) & bit)) {
-      const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(paged_many_rows_kernel<D, 4>),
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
-      if (e != hipSuccess) {
-        mi355_set_error("paged_attn_fp8: cannot reserve %d B of LDS: %s", LDS, hipGetErrorString(e));
-        return MI355_EHIP;
-      }
-      known.fetch_or(bit, std::memory_order_release);
-    }
-    hipLaunchKernelGGL((paged_many_rows_kernel<D, 4>), grid, dim3(256), LDS, st, p);
+    if (int rc = w.M == 64 ? launch_many<D, 2>(p, grid, st) : launch_many<D, 1>(p, grid, st)) return rc;
   }
   MI355_CHECK_LAUNCH("paged_attn_fp8");
   if (w.split) {

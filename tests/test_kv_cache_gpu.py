@@ -673,6 +673,28 @@ def test_attend_scales_far_apart(device, new):
     c.check()
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_attend_17_to_64_rows(device, D):
+    """Two waves for each row, half of the keys of a tile each: rows that see nothing, or keys of one
+    half only, blocks outside the pool in either, NaN in either, one length whole and one split."""
+    c = Case([20, 12, 16, 5], [15, 5000, 37, 100], 12, 3, D, 16, 23)
+    c.check()
+    c.check(window=9)
+    c.check(window=0)
+    c.check(causal=False)
+    c.table[1, 0], c.table[1, 3], c.table[2, 0], c.table[3, 4] = -1, 2 ** 30, -1, -1   # pieces 0 and 3 of tiles
+    c.check()
+    c = Case([20, 12, 16, 5], [150, 5000, 37, 100], 12, 3, D, 16, 24)
+    c.codes = [x.float() for x in c.codes]
+    for b, key, channel in ((0, 140, 3), (1, 4990, 17), (2, 31, 40), (2, 32, 41), (3, 99, 63)):
+        c.codes[1][int(c.table[b, key // 16]), key % 16, :, channel] = math.nan
+    c.codes = [x.to(FP8) for x in c.codes]
+    c.dev = [x.to(DEV) for x in c.codes]
+    got, lse = c.check()
+    assert torch.isnan(got[c.cu[2] - 1, :, 17]).all() and not torch.isnan(got[c.cu[1], :, 17]).any()
+    c.check(window=9)
+
+
 def test_attend_scores_far_apart(device):
     """Scores of some hundreds: all weight on one key, and the reference moving tile after tile."""
     for new in ([1], [5], [100]):
