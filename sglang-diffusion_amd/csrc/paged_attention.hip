@@ -1206,7 +1206,9 @@ Plan plan_of(const mi355_paged_attn_args* a) {
   const int64_t groups = a->Hk / w.hw;
   w.slots = (want + groups - 1) / groups;
   w.chunk_min = w.few ? (w.hw == 4 ? 1 : 4) : 4;
-  const int64_t cap = a->table_width * a->block_size;
+  // keys that a sequence's rows see, at most (were max_seqlen_q too small, more would be read in one piece)
+  const int64_t cap = std::min(a->table_width * a->block_size,
+                               a->window_left < 0 ? INT64_MAX : a->window_left + a->max_seqlen_q + KT);
   // (below that a piece costs less than the join's launch: 1 token over 100 keys 9.5 us, split 13; one
   // prompt of 500 tokens 19 us, split 30)
   w.split = cap > (w.few ? 4 * (4 / w.hw) : 8) * KT && (all_rows / w.M) * groups < 2 * want;
@@ -1234,7 +1236,7 @@ int check(const mi355_paged_attn_args* a) {
   MI355_REQUIRE(a->num_blocks >= 0 && a->num_blocks < (1ll << 31) && a->table_width >= 0 &&
                     a->table_width * a->block_size <= (1ll << 31) - 4096 && a->table_stride >= 0,
                 "paged_attn_fp8: bad page table");
-  MI355_REQUIRE(a->window_left < 0 || a->causal, "paged_attn_fp8: a window needs causal masking");
+  MI355_REQUIRE(a->window_left < (1ll << 40) && (a->window_left < 0 || a->causal), "paged_attn_fp8: a window needs causal masking");
   return MI355_OK;
 }
 

@@ -7,6 +7,8 @@ import torch
 
 from . import _ops  # noqa: F401
 
+_rotary_embedding_scaled = torch.ops.sgl_kernel.rotary_embedding_scaled.default  # (looked up once)
+
 
 def rmsnorm(input: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
             out: Optional[torch.Tensor] = None, enable_pdl: Optional[bool] = None) -> torch.Tensor:
@@ -62,5 +64,4 @@ def rotary_embedding_scaled(positions: torch.Tensor, query: torch.Tensor, key: O
         query_out = query
     if key is not None and key_out is None:
         key_out = key
-    torch.ops.sgl_kernel.rotary_embedding_scaled.default(positions, query, key, inv_freq, attn_factor, is_neox,
-                                                         query_out, key_out)
+    _rotary_embedding_scaled(positions, query, key, inv_freq, attn_factor, is_neox, query_out, key_out)

@@ -7,6 +7,8 @@ import torch
 
 from . import _ops  # noqa: F401
 
+_fwd_paged_fp8 = torch.ops.sgl_kernel.fwd_paged_fp8.default  # (looked up once)
+
 
 def is_fa3_supported(device=None) -> bool:
     """The MI355X kernel serves the same call; kept for callers that probe it."""
@@ -68,7 +70,7 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, qv=None, rotary
                            "an 8-bit cache")
     if isinstance(cache_seqlens, int):
         cache_seqlens = torch.full((page_table.shape[0],), cache_seqlens, dtype=torch.int32, device=q.device)
-    out, softmax_lse = torch.ops.sgl_kernel.fwd_paged_fp8.default(
+    out, softmax_lse = _fwd_paged_fp8(
         q, k_cache, v_cache, k_descale, v_descale, page_table, cache_seqlens, cu_seqlens_q, max_seqlen_q, softmax_scale,
         causal, window_size[0], window_size[1])
     if not return_softmax_lse:

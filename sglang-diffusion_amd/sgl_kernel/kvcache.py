@@ -8,6 +8,10 @@ import torch
 
 from . import _ops  # noqa: F401
 
+# (looked up once)
+_kv_block_plan = torch.ops.sgl_kernel.kv_block_plan.default
+_store_kv_cache_fp8 = torch.ops.sgl_kernel.store_kv_cache_fp8.default
+
 
 def kv_block_plan(context_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor,
                   free_blocks: torch.Tensor, free_begin: torch.Tensor, block_size: int, num_blocks: int,
@@ -25,7 +29,7 @@ def kv_block_plan(context_lens: torch.Tensor, new_lens: torch.Tensor, block_tabl
     `seq_lens` = `context_lens` and `free_end` = `free_begin`.
     Outputs are other memory than the inputs; copy `seq_lens` and `free_end` back for the next step.
     At most 4096 requests in one call."""
-    torch.ops.sgl_kernel.kv_block_plan.default(
+    _kv_block_plan(
         context_lens, new_lens, block_table, free_blocks, free_begin, block_size, num_blocks, slot_mapping,
         positions, cu_seqlens_q, seq_lens, free_end, status)
 
@@ -47,6 +51,6 @@ def store_kv_cache_fp8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Te
     `query_out`, or in place."""
     if query is not None and query_out is None:
         query_out = query
-    torch.ops.sgl_kernel.store_kv_cache_fp8.default(
+    _store_kv_cache_fp8(
         key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping, query, positions, inv_freq, attn_factor,
         is_neox, query_out)
