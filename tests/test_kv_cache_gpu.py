@@ -556,6 +556,48 @@ def test_attend_into_the_memory_of_q(device):
         assert got.data_ptr() == q.data_ptr() and torch.equal(q, want) and torch.equal(lse, lse2)
 
 
+@pytest.mark.parametrize("new", [[1, 1], [3, 2], [14, 9], [90, 40]])
+def test_attend_bad_queries_stay_in_their_rows(device, new):
+    """NaN and infinities in one row and head of q: NaN there, the others as they are."""
+    c = Case(new, [700, 65], 4, 2, 128, 16, 25)
+    c.q[0, 1, 5], c.q[-1, 2, 0], c.q[-1, 3, 100] = math.nan, math.inf, -math.inf
+    got, lse = c.call()
+    want = c.want()
+    c.compare(got, lse, want)
+    bad = torch.isnan(got).any(-1)
+    assert bad[0, 1] and bad[-1, 2] and bad[-1, 3] and bad.sum() == 3
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.2, 1e-30])
+def test_attend_any_scale_of_the_scores(device, scale):
+    for new in ([1, 1], [12, 3], [70, 9]):
+        c = Case(new, [900, 70], 4, 2, 64, 32, 26)
+        c.compare(*c.call(softmax_scale=scale), c.want(scale=scale))
+
+
+def test_attend_no_new_tokens_in_a_padded_batch(device):
+    import sgl_kernel  # noqa: F401
+
+    c = Case([0, 0, 0], [3000, 0, 17], 4, 2, 64, 16, 27)
+    for T in (5, 300):
+        q = torch.full((T, 4, 64), math.nan, device=DEV).bfloat16()
+        out = torch.full_like(q, 3.0)
+        torch.ops.sgl_kernel.fwd.default(
+            q, *c.dev, None, None, None, out, i32(c.cu), None, None, None, i32(c.lens), 1, None, c.table.to(DEV),
+            None, None, None, None, None, None, c.scales[0].to(DEV), c.scales[1].to(DEV), None, True, -1, -1, 0, 0.0,
+            False, None, 0, None, 0, None)
+        assert (out == 3.0).all()
+
+
+def test_store_into_a_pool_without_blocks(device):
+    import sgl_kernel
+
+    k = torch.randn(40, 2, 64, device=DEV).bfloat16()
+    codes, scale = torch.empty(0, 16, 2, 64, device=DEV).to(FP8), torch.empty(0, 2, device=DEV)
+    sgl_kernel.store_kv_cache_fp8(k, k, codes, codes.clone(), scale, scale.clone(), torch.arange(40, device=DEV))
+    torch.cuda.synchronize()
+
+
 def test_attend_rows_that_see_nothing(device):
     """No keys at all, and more new tokens than the cache holds: the first stand before its start."""
     for new, lens in (([1, 1, 1], [0, -4, 5]), ([6, 2], [3, 0]), ([90, 40], [70, 0])):
