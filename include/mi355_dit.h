@@ -541,7 +541,9 @@ int mi355_kv_store_fp8(const mi355_kv_store_args* args, void* stream);
  * flash_extension.cc:25-63).  Sequence b holds cache_seqlens[b] tokens, the new ones among them;
  * new token i of n stands at cache_seqlens[b] - n + i.  causal: it sees the keys up to its own
  * place; window_left >= 0 (with causal): and no further back than window_left.  A row that sees
- * nothing gives 0 and a log-sum-exp of -infinity.
+ * nothing gives 0 and a log-sum-exp of -infinity.  Sums and statistics are fp32; the weights of the
+ * second product are rounded to half: 2^-11 of each, or 2^-33 of the row's largest (weight times value
+ * scale) where they are less than 2^-22 of it.
  * q, out bf16: [Sq, H, D] packed with cu_seqlens_q int32 [B + 1] (rows behind the last sequence
  * are left as they are), or [B, Sq, H, D] with cu_seqlens_q == NULL.  lse fp32 or NULL, element
  * (row, head) at b * lse_sb + head * lse_sh + row.  out may be q.  max_seqlen_q chooses the kernel; any value is

@@ -10,7 +10,9 @@
 //   p~_j = exp2(s_j * (ks * scale * log2 e) + log2(vs_j) - m)      one exponential for each score
 //   O   += p~_j * codes_j,   l += p~_j / vs_j,   out = O / l
 // with m a running reference near the row's maximum of the exponent.  So a value block's scale
-// costs one addend in the exponent, and p~ in half keeps its 11 bits whatever the scales are.
+// costs one addend in the exponent.  p~ is rounded to half for the second product, the only rounding
+// below 32 bits before the output's own: 2^-11 of each weight, where the output's bf16 takes 2^-8.  The
+// row sum l takes p~ as it is, in fp32.
 //
 // Work is cut into items: a tile of rows of one sequence and key/value head against a chunk of
 // its keys.  Lengths are known on the device only, so each workgroup adds up the work of all
@@ -33,7 +35,11 @@ typedef int i32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int KT = 64;               // keys of a tile
 constexpr float M_EMPTY = -1e30f;    // reference of a row without weight, among those that have some
-constexpr float LAZY = 13.f;         // largest exponent against a reference that need not move: 2^13
+// A row's largest weight lies in [2^ROOM, 2^LAZY] of its reference: half holds up to 2^16, and what it
+// cannot hold as a normal number lies 2^22 or more below that weight, off by 2^-33 of it at most.  (With
+// the largest weight at 1, a key of 2^25 times the others took all of theirs: 500 of them, behind a first
+// key of no value, came out as 0.)  The seven steps between keep the reference from moving often.
+constexpr float ROOM = 8.f, LAZY = 15.f;
 
 struct PagedParams {
   const unsigned short* q;
@@ -329,14 +335,14 @@ __device__ __forceinline__ Scales scales_of(const PagedParams& p, float ks, floa
 }
 
 // Where a row's reference goes, by the largest exponent of a tile (relative to the reference) and the
-// weight that the row has so far: up to that exponent, and for a row without weight yet (which
-// starts from 0) also down to it.  Rows that see nothing stay.
+// weight that the row has so far: up to ROOM below that exponent, and for a row without weight yet
+// (which starts from 0) also down to it.  Rows that see nothing stay.
 struct Move {
   float by, shrink;
 };
 __device__ __forceinline__ Move move_reference(float top, float mass) {
-  if (mass == 0.f) return Move{top == -INFINITY ? 0.f : top, 0.f};
-  const float by = fmaxf(top, 0.f);
+  if (mass == 0.f) return Move{top == -INFINITY ? 0.f : top - ROOM, 0.f};
+  const float by = fmaxf(top - ROOM, 0.f);
   return Move{by, __builtin_amdgcn_exp2f(-by)};
 }
 

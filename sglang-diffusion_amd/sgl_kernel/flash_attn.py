@@ -52,7 +52,9 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, qv=None, rotary
     in the cache already (`store_kv_cache_fp8`).  `q` bf16 [B, S, H, D], or packed [T, H, D] with
     `cu_seqlens_q`; rows of a packed q behind the last sequence are not written.  New token i of n stands
     at cache_seqlens - n + i; `causal` hides later keys, `window_size` (w, 0) also those more than w back.
-    A row that sees no key gives 0, and -inf as its log-sum-exp (fp32 [H, T] or [B, H, S]).
+    A row that sees no key gives 0, and -inf as its log-sum-exp (fp32 [H, T] or [B, H, S]).  Scores, sums
+    and the log-sum-exp are fp32; softmax weights are rounded to half (2^-11) for the product with the
+    values, and the output to bf16 (2^-8).
     Everything else of the signature raises RuntimeError instead of being ignored; `num_splits`,
     `pack_gqa` and `sm_margin` are hints that this kernel does not need."""
     if score_mod is not None or aux_tensors is not None:
