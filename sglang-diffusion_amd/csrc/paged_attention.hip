@@ -1010,6 +1010,8 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedP
 }
 
 // ------------------------------------------------------------------------------------- joint --
+// Parts are weighed by 2^(their reference - the row's largest), also where that is 0: a part's NaN is the
+// row's, as it would be in one piece.  Parts that see nothing hold zeros.
 // The sequence and token of row t of q, for a whole wave; false where there is nothing to join: a
 // row behind the last sequence, or one whose keys were not split.
 struct JoinRow {
@@ -1071,7 +1073,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p, int M) {
     const int c = min(c0 + lane, chunks - 1);
     const float* ml = part + c * step + M * D + 2 * in_tile;
     const float w = c0 + lane < chunks ? __builtin_amdgcn_exp2f(ml[0] - top) : 0.f;
-    l = fmaf(w != 0.f ? ml[1] : 0.f, w, l);
+    l = c0 + lane < chunks ? fmaf(ml[1], w, l) : l;
     const int here = min(64, chunks - c0);
     for (int k = wave * 4 * SIDE; k < here; k += 16 * SIDE) {
       f32x4 v[4];
@@ -1081,12 +1083,11 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p, int M) {
         const int at = k + u * SIDE + mine;
         wv[u] = __shfl(w, min(at, 63), 64);
         v[u] = *reinterpret_cast<const f32x4*>(part + min(c0 + at, chunks - 1) * step + in_tile * D + 4 * ch);
-        if (at >= here) wv[u] = 0.f;
       }
 #pragma unroll
       for (int u = 0; u < 4; ++u)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] = wv[u] == 0.f ? acc[i] : fmaf(v[u][i], wv[u], acc[i]);
+        for (int i = 0; i < 4; ++i) acc[i] = k + u * SIDE + mine < here ? fmaf(v[u][i], wv[u], acc[i]) : acc[i];
     }
   }
   l = group_sum<64>(l);
@@ -1151,12 +1152,13 @@ __global__ __launch_bounds__(256) void paged_join_rows_kernel(PagedParams p, int
     for (int n = 0; n < NV; ++n) acc[n] *= shrink;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const float w = c0 + u < chunks ? __builtin_amdgcn_exp2f(m[u] - top) : 0.f;
-      l = w == 0.f ? l : fmaf(lc[u], w, l);
+      const bool there = c0 + u < chunks;
+      const float w = __builtin_amdgcn_exp2f(m[u] - top);
+      l = there ? fmaf(lc[u], w, l) : l;
 #pragma unroll
       for (int n = 0; n < NV; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[n][i] = w == 0.f ? acc[n][i] : fmaf(v[u][n][i], w, acc[n][i]);
+        for (int i = 0; i < 4; ++i) acc[n][i] = there ? fmaf(v[u][n][i], w, acc[n][i]) : acc[n][i];
     }
   }
   if (mine >= H) return;

@@ -64,3 +64,32 @@ def test_many_small_weights_behind_a_large_one(device, new, lens, H, Hk, D):
     recode(c)
     got, lse = c.call(causal=False)
     compare(c, got, lse, c.want(causal=False))
+
+
+# --------------------------------------------------------- NaN in keys that weigh nothing --
+@pytest.mark.parametrize("which", ["key", "value"])
+@pytest.mark.parametrize("place,large", [(100, 8500), (8500, 100)])
+@pytest.mark.parametrize("new,H,Hk", [([1], 8, 2), ([5], 8, 2), ([70], 8, 2), ([70], 32, 2)])
+def test_nan_far_below_the_largest_score(device, new, H, Hk, place, large, which):
+    """A NaN in the cache reaches every row that sees it, also where its piece of the keys has no weight
+    beside another piece: 0 * NaN is NaN, however the keys are cut."""
+    c = Case(new, [9001], H, Hk, 64, 16, 42)
+    c.codes = [x.float() for x in c.codes]
+    c.codes[0][:] = 0.0
+    c.codes[0][int(c.table[0, large // 16]), large % 16] = 16.0     # a score of 200: 2^288 times the others
+    c.scales[0][:] = 2.0 ** -4
+    c.q[:] = 200 / 64 ** 0.5
+    at = int(c.table[0, place // 16]), place % 16
+    if which == "key":
+        c.codes[0][at[0], at[1], 0, 5] = math.nan
+    else:
+        c.codes[1][at[0], at[1], 0, 5] = math.nan
+    recode(c)
+    got, lse = c.call()
+    first = slice(0, H // Hk)                                     # heads of the key head that has it
+    if which == "key":
+        assert torch.isnan(got[:, first]).all() and torch.isnan(lse[first]).all()
+    else:
+        assert torch.isnan(got[:, first, 5]).all() and not torch.isnan(got[:, first, :5]).any()
+        assert not torch.isnan(lse).any()
+    assert not torch.isnan(got[:, H // Hk:]).any()
