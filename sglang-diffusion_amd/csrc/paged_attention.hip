@@ -34,7 +34,9 @@ typedef __fp16 hw_f16x4 __attribute__((__vector_size__(4 * sizeof(__fp16))));
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int KT = 64;               // keys of a tile
-constexpr float M_EMPTY = -1e30f;    // reference of a row without weight, among those that have some
+// Reference of a row without weight, among those that have some: the lowest number, since a row whose
+// scores all lie below -10^30, say, has its weight all the same.
+constexpr float M_EMPTY = -3.402823466e38f;
 // A row's largest weight lies in [2^ROOM, 2^LAZY] of its reference: half holds up to 2^16, and what it
 // cannot hold as a normal number lies 2^22 or more below that weight, off by 2^-33 of it at most.  (With
 // the largest weight at 1, a key of 2^25 times the others took all of theirs: 500 of them, behind a first

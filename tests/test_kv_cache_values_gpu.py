@@ -93,3 +93,27 @@ def test_nan_far_below_the_largest_score(device, new, H, Hk, place, large, which
         assert torch.isnan(got[:, first, 5]).all() and not torch.isnan(got[:, first, :5]).any()
         assert not torch.isnan(lse).any()
     assert not torch.isnan(got[:, H // Hk:]).any()
+
+
+# -------------------------------------------------------------- scores far below all else --
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("new,lens", [([1, 1], [3000, 70]), ([6, 2], [3000, 70]), ([90, 30], [3000, 70])])
+def test_scores_far_below_any_reference(device, new, lens, D):
+    """Every score below -10^33, one key the least so: a row that sees keys has their weight, however low."""
+    c = Case(new, lens, 4, 2, D, 64, 43)
+    c.codes = [torch.full(c.codes[0].shape, -32.0), c.codes[1].float()]
+    c.scales[0][:] = 2.0 ** 50
+    c.scales[1][:] = 2.0 ** -6
+    c.q[:] = 1e17
+    for b, key in ((0, 1234), (1, 30)):
+        c.codes[0][int(c.table[b, key // 64]), key % 64] = -16.0
+    c.codes[1] = c.codes[1].nan_to_num(0)
+    recode(c)
+    got, lse = c.call()
+    out, want_lse, mass = c.want()
+    assert torch.isfinite(want_lse).all() and (want_lse < -1e33).all()
+    # rows that do not see the least low key have equal scores, and rounding decides between them
+    rows = [t for t in range(c.cu[-1]) if not (t >= c.cu[1] and lens[1] - new[1] + t - c.cu[1] < 30)]
+    off = (got.double() - out).abs()[rows]
+    assert (off <= bound(c, out, mass)[rows]).all(), off.max()
+    assert ((lse.double() - want_lse).abs() <= 1e-4 * want_lse.abs()).all()
