@@ -43,8 +43,9 @@ def store_kv_cache_fp8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Te
     tokens with a slot outside the pool are skipped), with one power-of-two scale for each block and
     head in `k_scale`, `v_scale` [blocks, Hk] fp32.  A call that writes a block's first token starts
     its scale anew; any other can raise it, and rounds the block's earlier codes to the larger step.
-    Tokens of one call that go to one block follow each other in the call and in the block, and no
-    slot is given twice.
+    Tokens may come in any order, with skipped ones between them (those of a block that follow each other
+    are fastest); no slot is given twice.  A call keeps what a block holds before the smallest place that
+    it writes there, and nothing behind it.
 
     With `positions` and `inv_freq` the keys are rotated first (as `rotary_embedding_scaled` does,
     rounded to bf16 as it does), and `query` [T, H, D], if given, is rotated in the same launch: into
