@@ -493,8 +493,8 @@ int mi355_kv_block_plan(const int32_t* context_lens, const int32_t* new_lens, in
  * the angle in fp64, one rounding to bf16.  inv_freq [rot_dim / 2], fp64 or fp32; pairs are
  * (i, i + rot_dim / 2) (is_neox) or (2 i, 2 i + 1); elements from rot_dim on are copied.
  * q [tokens, Hq, head_size], k [tokens, Hk, head_size] bf16 with token and head strides, outputs
- * with their own; an output may be its input, and must not overlap it otherwise.  Either tensor
- * may have no heads.  rot_dim % 16 == 0, head_size % 8 == 0 and <= 256, strides % 8 == 0, rows
+ * with their own; an output may be its input row for row, and must not overlap it otherwise, nor the
+ * other tensor.  Either tensor may have no heads.  rot_dim % 16 == 0, head_size % 8 == 0 and <= 256, strides % 8 == 0, rows
  * 16-byte aligned.  |position| < 2^40. */
 int mi355_rope_scaled(const int64_t* positions, const void* q, void* q_out, const void* k, void* k_out,
                       int64_t tokens, int64_t Hq, int64_t Hk, int64_t head_size, int64_t rot_dim,
@@ -510,7 +510,8 @@ int mi355_rope_scaled(const int64_t* positions, const void* q, void* q_out, cons
  * part in the scale.  Tokens of one call that go to one block follow each other in the call and
  * in the block; a slot is given once.
  * positions != NULL: keys are first rotated as by mi355_rope_scaled (and rounded to bf16), and
- * the queries q (Hq heads, or 0) are rotated into q_out in the same launch.
+ * the queries q (Hq heads, or 0) are rotated into q_out in the same launch (q itself, or memory apart
+ * from q, k and v).  The two caches, and their scales, are apart.
  * k, v [tokens, Hk, D] bf16, D 64 or 128; strides in elements (of the cache: bytes), multiples of
  * 8; k, v, q, q_out 16-byte aligned, the caches 8-byte. */
 typedef struct {
@@ -546,7 +547,7 @@ int mi355_kv_store_fp8(const mi355_kv_store_args* args, void* stream);
  * scale) where they are less than 2^-22 of it.
  * q, out bf16: [Sq, H, D] packed with cu_seqlens_q int32 [B + 1] (rows behind the last sequence
  * are left as they are), or [B, Sq, H, D] with cu_seqlens_q == NULL.  lse fp32 or NULL, element
- * (row, head) at b * lse_sb + head * lse_sh + row.  out may be q.  max_seqlen_q chooses the kernel; any value is
+ * (row, head) at b * lse_sb + head * lse_sh + row.  out may be q row for row, and must not overlap it otherwise.  max_seqlen_q chooses the kernel; any value is
  * right.  Lengths beyond the table count as its length; entries of the table that are not in
  * [0, num_blocks) are skipped as if their tokens were masked; entries behind a sequence's end are
  * not read.  Scales are positive, value scales between 2^-64 and 2^120.

@@ -5,6 +5,7 @@
 #include <type_traits>
 
 #include "common.h"
+#include "overlap.h"
 
 namespace {
 
@@ -663,10 +664,13 @@ __global__ __launch_bounds__(THREADS, 4) void kv_store_kernel(StoreParams p) {
   }
 }
 
-// rows that are written must not be the same ones (an expanded tensor's are)
-bool rows_apart(int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t D) {
-  return (n0 <= 1 || s0 >= D) && (n1 <= 1 || s1 >= D);
+using mi355::Rows;
+// [tokens, heads, D] in bf16, strides in elements
+Rows head_rows(const void* at, int64_t tokens, int64_t heads, int64_t D, int64_t st, int64_t sh) {
+  return Rows{at, 2 * D, {1, tokens, heads}, {0, 2 * st, 2 * sh}};
 }
+// an output may be an input of its own, and must not touch it otherwise
+bool same_or_apart(const Rows& out, const Rows& in) { return rows_same(out, in) || rows_apart(out, in); }
 
 bool rope_args_ok(const char* what, int64_t head_size, int64_t rot_dim, const void* inv_freq,
                   const int64_t* positions, int64_t tokens) {
@@ -753,9 +757,14 @@ extern "C" int mi355_rope_scaled(const int64_t* positions, const void* q, void* 
     MI355_REQUIRE(s % 8 == 0, "rope_scaled: strides must be multiples of 8 elements");
   MI355_REQUIRE(((uintptr_t)q | (uintptr_t)q_out | (uintptr_t)k | (uintptr_t)k_out) % 16 == 0,
                 "rope_scaled: rows must be 16-byte aligned");
-  MI355_REQUIRE((Hq == 0 || rows_apart(tokens, qo_st, Hq, qo_sh, head_size)) &&
-                    (Hk == 0 || rows_apart(tokens, ko_st, Hk, ko_sh, head_size)),
-                "rope_scaled: rows of an output overlap each other");
+  const Rows q_in = head_rows(q, tokens, Hq, head_size, q_st, q_sh), k_in = head_rows(k, tokens, Hk, head_size, k_st, k_sh),
+             q_to = head_rows(q_out, tokens, Hq, head_size, qo_st, qo_sh),
+             k_to = head_rows(k_out, tokens, Hk, head_size, ko_st, ko_sh);
+  MI355_REQUIRE(rows_distinct(q_to) && rows_distinct(k_to), "rope_scaled: rows of an output overlap each other");
+  MI355_REQUIRE(same_or_apart(q_to, q_in) && same_or_apart(k_to, k_in),
+                "rope_scaled: an output overlaps its input and is not the same rows");
+  MI355_REQUIRE(rows_apart(q_to, k_in) && rows_apart(k_to, q_in) && rows_apart(q_to, k_to),
+                "rope_scaled: an output overlaps the other tensor");
   Rope r = {positions, inv_freq, inv_freq_is_f64, (int)(rot_dim / 2), is_neox != 0, attn_factor};
   RopeRows a = {(const unsigned short*)q, (unsigned short*)q_out, q_st, q_sh, qo_st, qo_sh, (int)Hq};
   RopeRows b = {(const unsigned short*)k, (unsigned short*)k_out, k_st, k_sh, ko_st, ko_sh, (int)Hk};
@@ -791,11 +800,19 @@ extern "C" int mi355_kv_store_fp8(const mi355_kv_store_args* a, void* stream) {
     return MI355_EINVAL;
   MI355_REQUIRE(a->Hq == 0 || (turn_keys && a->q && a->q_out),
                 "kv_store_fp8: queries need positions and both their pointers");
-  MI355_REQUIRE((a->Hq == 0 || rows_apart(a->tokens, a->qo_st, a->Hq, a->qo_sh, a->D)) &&
-                    rows_apart(a->block_size, a->kc_st, a->Hk, a->kc_sh, a->D) &&
-                    rows_apart(a->block_size, a->vc_st, a->Hk, a->vc_sh, a->D) &&
-                    rows_apart(a->num_blocks, a->kc_sb, a->num_blocks, a->vc_sb, a->D),
+  const Rows q_in = head_rows(a->q, a->tokens, a->Hq, a->D, a->q_st, a->q_sh),
+             q_to = head_rows(a->q_out, a->tokens, a->Hq, a->D, a->qo_st, a->qo_sh),
+             k_in = head_rows(a->k, a->tokens, a->Hk, a->D, a->k_st, a->k_sh),
+             v_in = head_rows(a->v, a->tokens, a->Hk, a->D, a->v_st, a->v_sh),
+             kc = {a->k_cache, a->D, {a->num_blocks, a->block_size, a->Hk}, {a->kc_sb, a->kc_st, a->kc_sh}},
+             vc = {a->v_cache, a->D, {a->num_blocks, a->block_size, a->Hk}, {a->vc_sb, a->vc_st, a->vc_sh}},
+             ks = {a->k_scale, 4 * a->num_blocks * a->Hk, {1, 1, 1}, {0, 0, 0}},
+             vs = {a->v_scale, 4 * a->num_blocks * a->Hk, {1, 1, 1}, {0, 0, 0}};
+  MI355_REQUIRE(rows_distinct(q_to) && rows_distinct(kc) && rows_distinct(vc),
                 "kv_store_fp8: rows of an output overlap each other");
+  MI355_REQUIRE(same_or_apart(q_to, q_in) && rows_apart(q_to, k_in) && rows_apart(q_to, v_in),
+                "kv_store_fp8: the queries' output overlaps keys, values or queries (and is not the same rows)");
+  MI355_REQUIRE(rows_apart(kc, vc) && rows_apart(ks, vs), "kv_store_fp8: the caches or their scales overlap each other");
   StoreParams p;
   p.k = (const unsigned short*)a->k;
   p.v = (const unsigned short*)a->v;

@@ -23,6 +23,7 @@
 #include <atomic>
 
 #include "common.h"
+#include "overlap.h"
 
 namespace {
 
@@ -1312,10 +1313,6 @@ extern "C" int mi355_paged_attn_fp8(const mi355_paged_attn_args* a, void* stream
   const int64_t strides[] = {a->q_sb, a->q_ss, a->q_sh, a->o_sb, a->o_ss, a->o_sh};
   for (int64_t s : strides)
     MI355_REQUIRE(s % 8 == 0, "paged_attn_fp8: strides of q and out must be multiples of 8 elements");
-  const bool batched = a->cu_seqlens_q == nullptr;
-  MI355_REQUIRE((!batched || a->B <= 1 || a->o_sb >= a->D) && (a->Sq <= 1 || a->o_ss >= a->D) &&
-                    (a->H <= 1 || a->o_sh >= a->D),
-                "paged_attn_fp8: rows of out overlap each other");
   const int64_t cache_strides[] = {a->kc_sb, a->kc_st, a->kc_sh, a->vc_sb, a->vc_st, a->vc_sh};
   for (int64_t s : cache_strides)
     MI355_REQUIRE(s % 16 == 0, "paged_attn_fp8: strides of the caches must be multiples of 16 bytes");
@@ -1329,6 +1326,11 @@ extern "C" int mi355_paged_attn_fp8(const mi355_paged_attn_args* a, void* stream
                     (uintptr_t)a->workspace % 16 == 0,
                 "paged_attn_fp8: workspace of %ld bytes needed (16-byte aligned), %ld given",
                 (long)(w.part_bytes + w.info_bytes), (long)a->workspace_bytes);
+  const int64_t batch = a->cu_seqlens_q ? 1 : a->B;
+  const mi355::Rows q = {a->q, 2 * a->D, {batch, a->Sq, a->H}, {2 * a->q_sb, 2 * a->q_ss, 2 * a->q_sh}},
+                    out = {a->out, 2 * a->D, {batch, a->Sq, a->H}, {2 * a->o_sb, 2 * a->o_ss, 2 * a->o_sh}};
+  MI355_REQUIRE(rows_distinct(out), "paged_attn_fp8: rows of out overlap each other");
+  MI355_REQUIRE(rows_same(out, q) || rows_apart(out, q), "paged_attn_fp8: out overlaps q and is not the same rows");
   PagedParams p;
   p.q = (const unsigned short*)a->q;
   p.o = (unsigned short*)a->out;

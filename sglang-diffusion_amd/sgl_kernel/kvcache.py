@@ -49,7 +49,8 @@ def store_kv_cache_fp8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Te
 
     With `positions` and `inv_freq` the keys are rotated first (as `rotary_embedding_scaled` does,
     rounded to bf16 as it does), and `query` [T, H, D], if given, is rotated in the same launch: into
-    `query_out`, or in place."""
+    `query_out`, or in place.  Caches, scales and `query_out` that overlap each other or the inputs in
+    any other way raise."""
     if query is not None and query_out is None:
         query_out = query
     _store_kv_cache_fp8(
