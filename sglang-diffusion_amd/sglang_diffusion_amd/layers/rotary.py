@@ -85,6 +85,16 @@ def apply_flashinfer_rope_qk_inplace(q: torch.Tensor, k: torch.Tensor,
     return q, k
 
 
+# what each rope_type of `scaled_inv_freq` uses
+_ROPE_KEYS = {
+    "default": (),
+    "linear": ("factor",),
+    "llama3": ("factor", "low_freq_factor", "high_freq_factor", "original_max_position_embeddings"),
+    "yarn": ("factor", "original_max_position_embeddings", "beta_fast", "beta_slow", "truncate", "attention_factor",
+             "mscale", "mscale_all_dim"),
+}
+
+
 def scaled_inv_freq(rot_dim: int, base: float = 10000.0, scaling: Optional[dict] = None,
                     device=None) -> Tuple[torch.Tensor, float]:
     """Frequencies base^(-2i / rot_dim) in float64, scaled for contexts longer than the trained one,
@@ -98,34 +108,61 @@ def scaled_inv_freq(rot_dim: int, base: float = 10000.0, scaling: Optional[dict]
       trained length divided by f, those above high_freq_factor kept, the share between
       interpolated over the number of turns.
     * {"rope_type": "yarn", "factor", "original_max_position_embeddings", "beta_fast" (32),
-      "beta_slow" (1), "attention_factor"}: a ramp over the pair index between the pairs that turn
-      beta_fast and beta_slow times; attention_factor defaults to 0.1 ln f + 1."""
+      "beta_slow" (1), "truncate" (True), "attention_factor", "mscale", "mscale_all_dim"}: a ramp over
+      the pair index between the pairs that turn beta_fast and beta_slow times, whole indices unless
+      truncate is false; attention_factor defaults to m(mscale) / m(mscale_all_dim) with
+      m(x) = 0.1 x ln f + 1, and to m(1) without those two.
+
+    A key that the type has no use for raises, since leaving it out may be wrong for the model."""
     if rot_dim <= 0 or rot_dim % 2:
         raise ValueError(f"rot_dim must be positive and even, got {rot_dim}")
     freq = base ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64) / rot_dim)
     attn_factor = 1.0
-    kind = (scaling or {}).get("rope_type", (scaling or {}).get("type", "default"))
+    scaling = dict(scaling or {})
+    kind = scaling.pop("rope_type", None)
+    legacy = scaling.pop("type", None)
+    if kind is not None and legacy is not None and kind != legacy:
+        raise ValueError(f"rope_type {kind!r} and type {legacy!r} differ")
+    kind = kind or legacy or "default"
+    if kind not in _ROPE_KEYS:
+        raise ValueError(f"unknown rope_type {kind!r}")
+    unused = sorted(set(scaling) - set(_ROPE_KEYS[kind]))
+    if unused:
+        raise ValueError(f"rope_type {kind!r} does not use {unused}: not implemented")
     if kind == "linear":
         freq = freq / scaling["factor"]
     elif kind == "llama3":
         turns = scaling["original_max_position_embeddings"] * freq / (2 * math.pi)
         low, high = scaling["low_freq_factor"], scaling["high_freq_factor"]
+        if not low < high:
+            raise ValueError(f"low_freq_factor {low} must be below high_freq_factor {high}")
         keep = ((turns - low) / (high - low)).clamp(0.0, 1.0)
         freq = freq * (keep + (1.0 - keep) / scaling["factor"])
     elif kind == "yarn":
         trained, factor = scaling["original_max_position_embeddings"], scaling["factor"]
 
+        def given(name, otherwise):
+            value = scaling.get(name)
+            return otherwise if value is None else value
+
         def pair_that_turns(times):
             return rot_dim * math.log(trained / (times * 2 * math.pi)) / (2 * math.log(base))
 
-        first = max(math.floor(pair_that_turns(scaling.get("beta_fast") or 32)), 0)
-        last = min(math.ceil(pair_that_turns(scaling.get("beta_slow") or 1)), rot_dim - 1)
+        first, last = pair_that_turns(given("beta_fast", 32)), pair_that_turns(given("beta_slow", 1))
+        if given("truncate", True):
+            first, last = math.floor(first), math.ceil(last)
+        first, last = max(first, 0), min(last, rot_dim - 1)
         ramp = (torch.arange(rot_dim // 2, dtype=torch.float64) - first) / (max(last - first, 0.001))
         keep = 1.0 - ramp.clamp(0.0, 1.0)
         freq = freq * (keep + (1.0 - keep) / factor)
+
+        def growth(x):
+            return 0.1 * x * math.log(factor) + 1.0 if factor > 1 else 1.0
+
         attn_factor = scaling.get("attention_factor")
+        scales = [scaling.get("mscale"), scaling.get("mscale_all_dim")]
         if attn_factor is None:
-            attn_factor = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
-    elif kind != "default":
-        raise ValueError(f"unknown rope_type {kind!r}")
+            if (scales[0] is None) != (scales[1] is None) or 0 in scales:
+                raise ValueError("mscale and mscale_all_dim come together and are not 0 (or attention_factor is given)")
+            attn_factor = growth(1.0) if scales[0] is None else growth(scales[0]) / growth(scales[1])
     return freq.to(device), float(attn_factor)
