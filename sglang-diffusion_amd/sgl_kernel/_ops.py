@@ -398,7 +398,7 @@ def _fake_fwd_paged_fp8_out(q, *rest, **kw):
 
 @torch.library.register_fake("sgl_kernel::fwd")
 def _fake_fwd(q, k, v, k_new, v_new, q_v, out, cu_seqlens_q, cu_seqlens_k, *rest, **kw):
-    o = torch.empty_like(q) if out is None else out
+    o = q.new_empty(q.shape) if out is None else out  # contiguous, whatever q's strides
     if q.dim() == 4:
         lse = q.new_empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32)
     else:
