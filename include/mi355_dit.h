@@ -547,14 +547,16 @@ int mi355_kv_store_fp8(const mi355_kv_store_args* args, void* stream);
  * scale) where they are less than 2^-22 of it.
  * q, out bf16: [Sq, H, D] packed with cu_seqlens_q int32 [B + 1] (rows behind the last sequence
  * are left as they are), or [B, Sq, H, D] with cu_seqlens_q == NULL.  lse fp32 or NULL, element
- * (row, head) at b * lse_sb + head * lse_sh + row.  out may be q row for row, and must not overlap it otherwise.  max_seqlen_q chooses the kernel; any value is
- * right.  Lengths beyond the table count as its length; entries of the table that are not in
+ * (row, head) at b * lse_sb + head * lse_sh + row.  out may be q row for row, and must not overlap it
+ * otherwise.  max_seqlen_q chooses the kernel; any value in [0, 2^31) is right, and so is any window_left.
+ * Lengths beyond the table count as its length; entries of the table that are not in
  * [0, num_blocks) are skipped as if their tokens were masked; entries behind a sequence's end are
  * not read.  Scales are positive, value scales between 2^-64 and 2^120.
  * D 64 or 128; strides of q and out multiples of 8 elements, those of the caches multiples of 16
  * bytes (the token's below 2^24), q, out and the caches 16-byte aligned; a table row holds at most
- * 2^31 - 4096 tokens, rows of the table may be one row.  workspace: mi355_paged_attn_workspace_bytes(args) of device memory (16-byte
- * aligned, no initial contents) that no other call in flight uses. */
+ * 2^31 - 4096 tokens, rows of the table may be one row.  workspace:
+ * mi355_paged_attn_workspace_bytes(args) of device memory (16-byte aligned, no initial contents) that no
+ * other call in flight uses. */
 typedef struct {
   const void* q;
   void* out;

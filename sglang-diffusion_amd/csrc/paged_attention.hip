@@ -1218,8 +1218,9 @@ Plan plan_of(const mi355_paged_attn_args* a) {
   w.slots = (want + groups - 1) / groups;
   w.chunk_min = w.few ? (w.hw == 4 ? 1 : 4) : 4;
   // keys that a sequence's rows see, at most (were max_seqlen_q too small, more would be read in one piece)
-  const int64_t cap = std::min(a->table_width * a->block_size,
-                               a->window_left < 0 ? INT64_MAX : a->window_left + a->max_seqlen_q + KT);
+  const int64_t room = a->table_width * a->block_size;
+  const int64_t cap = a->window_left < 0 || a->window_left >= room
+                          ? room : std::min(room, a->window_left + a->max_seqlen_q + KT);
   // (below that a piece costs less than the join's launch: 1 token over 100 keys 9.5 us, split 13; one
   // prompt of 500 tokens 19 us, split 30)
   w.split = cap > (w.few ? 4 * (4 / w.hw) : 8) * KT && (all_rows / w.M) * groups < 2 * want;
@@ -1247,7 +1248,7 @@ int check(const mi355_paged_attn_args* a) {
   MI355_REQUIRE(a->num_blocks >= 0 && a->num_blocks < (1ll << 31) && a->table_width >= 0 &&
                     a->table_width * a->block_size <= (1ll << 31) - 4096 && a->table_stride >= 0,
                 "paged_attn_fp8: bad page table");
-  MI355_REQUIRE(a->window_left < (1ll << 40) && (a->window_left < 0 || a->causal), "paged_attn_fp8: a window needs causal masking");
+  MI355_REQUIRE(a->window_left < 0 || a->causal, "paged_attn_fp8: a window needs causal masking");
   return MI355_OK;
 }
 
@@ -1356,7 +1357,7 @@ extern "C" int mi355_paged_attn_fp8(const mi355_paged_attn_args* a, void* stream
   p.num_blocks = (int)a->num_blocks;
   p.lb = __builtin_ctzll((unsigned long long)a->block_size);
   p.causal = a->causal != 0;
-  p.window = a->window_left < 0 ? -1 : (int)(a->window_left < (1 << 30) ? a->window_left : (1 << 30));
+  p.window = a->window_left < 0 || a->window_left >= p.cap ? -1 : (int)a->window_left;  // (beyond: hides nothing)
   p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
   p.items = (int)w.items;
   p.slots = (float)w.slots;
