@@ -1241,8 +1241,8 @@ int check(const mi355_paged_attn_args* a) {
                     a->Hk > 0 && a->H % a->Hk == 0 && a->max_seqlen_q >= 0 && a->max_seqlen_q < (1ll << 31),
                 "paged_attn_fp8: bad shape B=%ld Sq=%ld H=%ld Hk=%ld", (long)a->B, (long)a->Sq, (long)a->H,
                 (long)a->Hk);
-  MI355_REQUIRE((a->cu_seqlens_q ? a->Sq : a->Sq * a->B) * (a->H / a->Hk) < (1ll << 31),
-                "paged_attn_fp8: too many rows");
+  const int64_t tokens = a->cu_seqlens_q ? a->Sq : a->Sq * a->B;
+  MI355_REQUIRE(tokens < (1ll << 31) && tokens * (a->H / a->Hk) < (1ll << 31), "paged_attn_fp8: too many rows");
   MI355_REQUIRE(a->block_size >= 16 && a->block_size <= 1024 && (a->block_size & (a->block_size - 1)) == 0,
                 "paged_attn_fp8: block size %ld must be a power of two in [16, 1024]", (long)a->block_size);
   MI355_REQUIRE(a->num_blocks >= 0 && a->num_blocks < (1ll << 31) && a->table_width >= 0 &&

@@ -23,6 +23,13 @@ def workspace(**change):
     return need, lib.mi355_last_error().decode()
 
 
+def test_rows_whose_number_does_not_fit_64_bits():
+    """2^61 rows, and 2^65 and 2^64, which are none in 64 bits."""
+    for B, Sq, heads in ((1 << 20, 1 << 28, 1 << 13), (1 << 23, 1 << 30, 1 << 12), (1 << 22, 1 << 30, 1 << 12)):
+        need, message = workspace(cu_seqlens_q=None, B=B, Sq=Sq, H=heads, Hk=1)
+        assert need == -1 and "too many rows" in message
+
+
 def test_windows():
     need, message = workspace(causal=0, window_left=3)
     assert need == -1 and "causal" in message
