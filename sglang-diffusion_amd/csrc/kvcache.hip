@@ -256,7 +256,8 @@ constexpr int ROPE_THREADS = 256, ROPE_MAX_HALF = 128, ROPE_MAX_TOKENS = 4;
 // The rows of tokens [t0, t0 + nt) of two tensors (the second may have no heads).  Cosine and
 // sine of a token are formed once for all its heads and kept in LDS: with 40 heads of 128 that
 // is 1/40 of the fp64 products that forming them at each pair would take.  Bound by memory from some
-// hundred tokens on: 8191 of 40 heads of 128, 168 MB in 35.8 us = 4.7 TB/s (a large copy: 4.9).
+// hundred tokens on: 8191 of 40 heads of 128, 168 MB in 35.8 us = 4.7 TB/s where nothing of it is in a
+// cache (a large copy: 4.9), over the same memory again and again 28.7.
 template <int THREADS>
 __device__ __forceinline__ void rope_tokens(const Rope& r, const RopeRows& a, const RopeRows& b, int D,
                                             int64_t t0, int nt, float2* cs) {
@@ -303,13 +304,15 @@ inline int rope_group(int64_t tokens) { return tokens >= 7168 ? ROPE_MAX_TOKENS 
 // Keys come first in the grid, then values, then the queries' rotation: what takes longest begins
 // first.
 //
-// 48 runs of one token take 6 us, bound by the chain slot, row and scale, maximum, code; 1200 of them
-// 30 (run after run by whole workgroups: 106).  4602 tokens of 12 prompts (104 MB with 32 heads of
-// queries) take 37.6 us = 2.8 TB/s: 15 for the queries alone, and for keys and values the chain again
-// and the cosines, which each head forms for itself.  Blocks of 256: 1842 tokens 25 us (with 256
-// threads 70).  Measured and slower: keys and values in turn (44), queries in turn with both (52), 128
-// threads with eight rows each (53-62), 512 with two (45), five or more waves a SIMD, which spill
-// (52-80).
+// 48 runs of one token take 6.4 us, bound by the chain slot, row and scale, maximum, code; 1200 of them
+// 31 (run after run by whole workgroups: 106).  4602 tokens of 12 prompts (104 MB with 32 heads of
+// queries) take 32 us = 3.3 TB/s, among other calls 39: 15 for the queries alone, and for keys and values
+// the chain again, the look for tokens elsewhere (3) and the cosines, which each head forms for itself.
+// Blocks of 256: 2420 tokens of 3 prompts 43 us (threads: 1842 tokens took 25 with 1024 and 70 with 256);
+// blocks of 1024: 1400 tokens 126, read twice.  Measured and slower, where these 12 prompts took 38: keys
+// and values in turn (44), queries in turn with both (52), 128 threads with eight rows each (53-62), 512
+// with two (45), five or more waves a SIMD (52-80, more values in scratch memory; at four the instances
+// of 256 and 512 threads keep theirs in 124 registers, that of 1024 puts six out).
 constexpr int HELD = 4;
 struct StoreParams {
   const unsigned short *k, *v;

@@ -102,9 +102,10 @@ struct Item {
 
 // Items of whole rows (no chunks) of a few sequences with causal rows, longest first: what is left
 // for the last round of workgroups is short then, whatever the sequences' order (prompts of 4096,
-// 1115 and 1341 tokens, 32 heads over 8: 215 us, one sequence after the other 224).  Row tiles are put in order by
-// the place of their last row, in levels of `unit` tiles of keys.  Lanes count the tiles at and above
-// 64 levels at a time: two rounds find the level of the item, a walk over the sequences its tile.
+// 1115 and 1341 tokens, 32 heads over 8, the first calls after a pause: 215 us, one sequence after the
+// other 224).  Row tiles are put in order by the place of their last row, in levels of `unit` tiles of
+// keys.  Lanes count the tiles at and above 64 levels at a time: two rounds find the level of the item, a
+// walk over the sequences its tile.
 constexpr int SORTED_SEQS = 16;
 template <int M>
 __device__ __forceinline__ void find_longest(const PagedParams& p, int item, Item* found) {
@@ -686,11 +687,14 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void paged_few_rows_kernel(Pa
 // Up to 64 rows (HALVES = 2) two waves share 32 rows, each with half of a tile's keys, since a wave's
 // chain of products, exponentials and products is what a tile then takes: 32 rows over 60 thousand
 // keys 104 us, with two waves idle 116; 64 rows 120 and 143.
-// Prompts of 4096, 1115 and 1341 tokens, 32 heads over 8, in 187-204 us: 0.80-0.87 PF/s, where a large
-// bf16 library product reaches 1.19.  Matrix instructions are busy 0.38 of the time and the vector unit
-// (32 exponentials a lane and tile, and the widening) 0.50; the two hardly overlap, neither
-// across waves nor when the second half's exponentials are put between the first half's products
-// (223 us where this order takes 211).  256 rows with eight waves halve the widening and take as long.
+// Prompts of 4096, 1115 and 1341 tokens, 32 heads over 8: 188 us = 0.86 PF/s at the clock that a few dozen
+// calls in a row settle to (the first ones after a pause take 217-226, with a profiler or without), 201
+// with other inputs for each call.  A large bf16 library product reaches 1.19 PF/s, this repository's dense
+// kernel 1.17 at 4096 tokens, 0.83 at 1536.  By counters matrix instructions are busy 0.39 of the time
+// (dense: 0.63) and the vector unit (32 exponentials a lane and tile, and the widening) 0.54 (0.48); the
+// two hardly overlap, neither across waves nor when the second half's exponentials are put between the
+// first half's products (223 us where this order took 211, after a pause).  256 rows with eight waves
+// halve the widening and take as long.
 template <int D, int NW, int HALVES>
 __global__ __launch_bounds__(NW * 64, 8 / NW) void paged_many_rows_kernel(PagedParams p) {
   constexpr int RANKS = NW / HALVES, M = 32 * RANKS, KB = 2 / HALVES, ROWB = 2 * D, CPR = ROWB / 16, KSTEPS = D / 16, DVB = D / 32;

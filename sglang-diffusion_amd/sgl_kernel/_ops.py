@@ -7,8 +7,8 @@ are defined from Python and each one is implemented for the `CUDA` dispatch key 
 under PyTorch-ROCm) by a call through the C ABI of include/mi355_dit.h.  There is no CPU
 implementation: CPU tensors hit the dispatcher's "no kernel for backend CPU" error, and a
 missing shared object raises on first use.  (The ops around the paged 8-bit cache are
-implemented in csrc/ops.cpp, which checks the arguments before it refuses CPU tensors.)  `torch.library.register_fake` shims give the
-shape/dtype rules for tracing, as the reference does in
+implemented in csrc/ops.cpp, which checks the arguments before it refuses CPU tensors.)
+`torch.library.register_fake` shims give the shape/dtype rules for tracing, as the reference does in
 python/sglang/srt/layers/quantization/fp8_utils.py:69-81 and fp8_kernel.py:2057-2076.
 
 Conventions kept from the reference: `Tensor!` outputs are caller-allocated and written in
@@ -245,7 +245,8 @@ def _fwd(q, k, v, k_new, v_new, q_v, out, cu_seqlens_q, cu_seqlens_k, cu_seqlens
          rotary_sin, seqlens_rotary, q_descale, k_descale, v_descale, softmax_scale, is_causal,
          window_left, window_right, attention_chunk, softcap, is_rotary_interleaved,
          scheduler_metadata, num_splits, pack_gqa, sm_margin, sinks):
-    """With page_table and e4m3 caches: attention over a paged 8-bit cache (fwd_paged_fp8).  Otherwise
+    """With page_table and e4m3 caches: attention over a paged 8-bit cache (fwd_paged_fp8), whose k_descale
+    and v_descale are [blocks, heads], not [sequences, heads] as the interface's own.  Otherwise
     dense non-causal attention, the only form the diffusion path issues
     (python/sglang/multimodal_gen/runtime/layers/attention/backends/flash_attn.py:517-563).
     Batched [B,S,H,d] inputs, or packed [T,H,d] inputs whose sequences all have the maximum

@@ -58,8 +58,9 @@ def rotary_embedding_scaled(positions: torch.Tensor, query: torch.Tensor, key: O
     [T, Hk, D] bf16 turned by positions[t] * inv_freq[i] (int64, fp64 or fp32; the angle in fp64),
     cosine and sine times `attn_factor`.  The first 2 * len(inv_freq) elements of a head are turned,
     in halves (is_neox) or in neighbouring pairs; the others are copied.  In place without
-    `query_out` / `key_out`; an output that overlaps an input in any other way raises.  sglang_diffusion_amd.layers.rotary.scaled_inv_freq makes the frequencies
-    of the usual long-context scalings."""
+    `query_out` / `key_out`; an output that overlaps an input in any other way raises.
+    sglang_diffusion_amd.layers.rotary.scaled_inv_freq makes the frequencies of the usual long-context
+    scalings."""
     if query_out is None:
         query_out = query
     if key is not None and key_out is None:
