@@ -651,7 +651,8 @@ __global__ __launch_bounds__(THREADS, 4) void kv_store_kernel(StoreParams p) {
     store_run<D, 64>(p, keys, w0 + l, nullptr, __builtin_amdgcn_readlane(run_len, l),
                      __builtin_amdgcn_readlane(block, l), head, lds.wave[wave]);
   }
-  // blocks whose tokens stand apart, with a list of them
+  // blocks whose tokens stand apart, with a list of them: one block after the other (500 x 8 tokens, 8 heads:
+  // in order 23 us, every third one skipped 63, the sequences in turn 214)
   for (unsigned long long todo = more & ~earlier; todo; todo &= todo - 1) {
     const int mine = __builtin_amdgcn_readlane(block, __ffsll(todo) - 1);
     __syncthreads();
