@@ -494,8 +494,8 @@ int mi355_kv_block_plan(const int32_t* context_lens, const int32_t* new_lens, in
  * (i, i + rot_dim / 2) (is_neox) or (2 i, 2 i + 1); elements from rot_dim on are copied.
  * q [tokens, Hq, head_size], k [tokens, Hk, head_size] bf16 with token and head strides, outputs
  * with their own; an output may be its input row for row, and must not overlap it otherwise, nor the
- * other tensor.  Either tensor may have no heads.  rot_dim % 16 == 0, head_size % 8 == 0 and <= 256, strides % 8 == 0, rows
- * 16-byte aligned.  |position| < 2^40. */
+ * other tensor.  Either tensor may have no heads.  rot_dim % 16 == 0, head_size % 8 == 0 and <= 256,
+ * strides % 8 == 0, rows 16-byte aligned.  |position| < 2^40. */
 int mi355_rope_scaled(const int64_t* positions, const void* q, void* q_out, const void* k, void* k_out,
                       int64_t tokens, int64_t Hq, int64_t Hk, int64_t head_size, int64_t rot_dim,
                       int64_t q_st, int64_t q_sh, int64_t qo_st, int64_t qo_sh, int64_t k_st,
@@ -551,7 +551,7 @@ int mi355_kv_store_fp8(const mi355_kv_store_args* args, void* stream);
  * otherwise.  max_seqlen_q chooses the kernel; any value in [0, 2^31) is right, and so is any window_left.
  * Lengths beyond the table count as its length; entries of the table that are not in
  * [0, num_blocks) are skipped as if their tokens were masked; entries behind a sequence's end are
- * not read.  Scales are positive, value scales between 2^-64 and 2^120.
+ * not read.  Scales are positive; value scales outside [2^-64, 2^120] count as the nearer end.
  * D 64 or 128; strides of q and out multiples of 8 elements, those of the caches multiples of 16
  * bytes (the token's below 2^24), q, out and the caches 16-byte aligned; a table row holds at most
  * 2^31 - 4096 tokens, rows of the table may be one row.  workspace:

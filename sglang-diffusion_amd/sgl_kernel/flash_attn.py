@@ -47,11 +47,13 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, qv=None, rotary
     """Attention of the newest tokens of each sequence over a paged cache in 8 bits.
 
     `k_cache`, `v_cache` e4m3 [blocks, block_size, Hk, D] (any strides, D contiguous) with `k_descale`,
-    `v_descale` fp32 [blocks, Hk]: one scale for each block of tokens and head.  `page_table` int32
-    [B, blocks of a sequence], `cache_seqlens` int32 [B] (or one int) counts the new tokens too: they are
-    in the cache already (`store_kv_cache_fp8`).  `q` bf16 [B, S, H, D], or packed [T, H, D] with
-    `cu_seqlens_q`; rows of a packed q behind the last sequence are not written.  New token i of n stands
-    at cache_seqlens - n + i; `causal` hides later keys, `window_size` (w, 0) also those more than w back.
+    `v_descale` fp32 [blocks, Hk]: one positive scale for each block of tokens and head (the interface's
+    own count sequences and heads); value scales outside [2^-64, 2^120] count as the nearer end.
+    `page_table` int32 [B, blocks of a sequence], `cache_seqlens` int32 [B] (or one int) counts the new
+    tokens too: they are in the cache already (`store_kv_cache_fp8`).  `q` bf16 [B, S, H, D], or packed
+    [T, H, D] with `cu_seqlens_q`; rows of a packed q behind the last sequence are not written.  New token
+    i of n stands at cache_seqlens - n + i; `causal` hides later keys, `window_size` (w, 0) also those more
+    than w back.
     A row that sees no key gives 0, and -inf as its log-sum-exp (fp32 [H, T] or [B, H, S]).  Scores, sums
     and the log-sum-exp are fp32; softmax weights are rounded to half (2^-11) for the product with the
     values, and the output to bf16 (2^-8).
